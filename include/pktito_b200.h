@@ -324,6 +324,145 @@ int pkb_tdt_search_dev(void *stream, const pkb_tdt_model *m, const float *f, con
  * of its longest-running segment. No counterpart in the reference. */
 uint64_t pkb_tdt_last_rounds(void);
 
+/* ------------------------------- a key/value cache held in 4 bits -- */
+
+/* K and V rows of many sequences, held in 4 bits a value in pages that
+ * sequences may share, and the attention that reads them: for a streaming
+ * encoder's left context, an attention decoder's own tokens and the
+ * encoder's frames it attends to, and the hypotheses of a beam. No
+ * counterpart in the reference; the block convention is its quantize's.
+ *
+ * What is held. A block is 32 consecutive values of one head of one row.
+ * With amax its largest magnitude: a block that holds a NaN or an infinity,
+ * or whose amax is below 2^-121, is held as zeros (scale 0). Otherwise the
+ * scale s is the largest number of 5 significant bits that is not above
+ * amax / 7 (the float quotient), each value is the code c = rint(x / s),
+ * ties to even, within [-7, 7], and stands for c s, which is exactly a bf16.
+ *
+ * How it lies. A unit is 16 tokens of one head, 18 dk bytes: K's codes
+ * (8 dk), V's codes (8 dk), K's scales bf16 [16][dk/32], V's scales bf16
+ * [dk/32][16]. Codes are nibbles n = c + 8, the lower nibble of a byte
+ * first. K's value d of token r is nibble
+ *     r dk + ((d%32/8) (dk/32) + d/32) 8 + d%8/2 + 4 (d%2),
+ * V's is nibble, with w = d%32,
+ *     ((((d/32) 8 + d%8) 4 + r%8/2) 2 + w/16) 8 + 4 (r%2) + 2 (r/8) + w%16/8,
+ * the orders in which the tensor cores' operands take them. A page is
+ * [n_heads][page_tokens/16] units, the cache [n_layers][n_pages] pages;
+ * every layer has the same table. Token j of sequence s lies in page
+ * table[s][j / page_tokens], place j % page_tokens.
+ *
+ * table, lens and refs are device memory that these calls read and write on
+ * the stream, so a step that takes pages, appends and attends can be
+ * captured in a CUDA graph. A cache in use is consistent: table rows hold
+ * ceil(lens / page_tokens) pages and -1 behind them, refs how many
+ * sequences hold each page (0: free); pkb_cache4_reset_dev makes an empty
+ * one. Two calls that change one cache, or one that changes it and one that
+ * reads it, are ordered by the caller (one stream, or events). */
+typedef struct {
+    uint8_t *pages;       /* [n_layers][n_pages][pkb_cache4_page_bytes], 16-byte aligned */
+    int32_t *table;       /* [max_seqs][max_pages] pages, -1 for none */
+    int32_t *lens;        /* [max_seqs] tokens held */
+    int32_t *refs;        /* [n_pages] sequences that hold the page */
+    uint32_t n_layers, n_pages, max_seqs, max_pages;
+    uint32_t page_tokens; /* 16, 32, 64, 128 or 256 */
+    uint32_t n_heads;     /* K/V heads */
+    uint32_t head_dim;    /* dk: 32, 64, 96, 128 or 256 */
+} pkb_cache4;
+
+/* Types of the rows that the calls below read and write. */
+enum { PKB_F32 = 0, PKB_F16 = 1, PKB_BF16 = 2 };
+
+/* What a page operation found, in *status on the device: nonzero, and
+ * nothing was changed, where there are too few free pages; where a sequence
+ * would need more pages than a table row has; where a sequence is out of
+ * range, listed twice where it is changed, not empty where it has to be, or
+ * shorter than asked for. The largest that applies. */
+enum { PKB_CACHE4_DONE = 0, PKB_CACHE4_FULL = 1, PKB_CACHE4_LONG = 2, PKB_CACHE4_BAD = 3 };
+
+/* The bytes of one page of one layer; 0 where the sizes are not allowed. */
+size_t pkb_cache4_page_bytes(uint32_t page_tokens, uint32_t n_heads, uint32_t head_dim);
+
+/* Device bytes of the work area that the page operations on this cache take
+ * (its sizes alone are read; for pkb_cache4_copy_dev, those of the cache
+ * copied to). 256-byte aligned. Calls in flight at the same time, and
+ * captured graphs that may be, each have one of their own. */
+size_t pkb_cache4_work_bytes(const pkb_cache4 *c);
+
+/* An empty cache: no table entries, no tokens, every page free. */
+int pkb_cache4_reset_dev(void *stream, const pkb_cache4 *c);
+
+/* Room for add[i] >= 0 more tokens at the end of sequence seqs[i], i < n
+ * (device arrays): lens grows, and new pages are the lowest free ones, in
+ * the order listed. The tokens' rows are then appended layer by layer. */
+int pkb_cache4_grow_dev(void *stream, const pkb_cache4 *c, const int32_t *seqs, const int32_t *add, uint32_t n,
+                        int32_t *status, void *work, size_t work_bytes);
+
+/* The empty sequence dst[i] takes the first len[i] tokens of src[i]: it
+ * shares the pages that those fill, and a last page that they do not fill
+ * is copied, in every layer, to the lowest free page in the order listed. */
+int pkb_cache4_fork_dev(void *stream, const pkb_cache4 *c, const int32_t *src, const int32_t *dst, const int32_t *len,
+                        uint32_t n, int32_t *status, void *work, size_t work_bytes);
+
+/* The empty sequence dst[i] of cache `to` takes the first len[i] tokens of
+ * sequence src[i] of `from` in pages of its own, all copied. `to` may be
+ * `from`; else the two are alike in layers, page_tokens, heads and dk and
+ * share no memory. */
+int pkb_cache4_copy_dev(void *stream, const pkb_cache4 *to, const pkb_cache4 *from, const int32_t *src,
+                        const int32_t *dst, const int32_t *len, uint32_t n, int32_t *status, void *work,
+                        size_t work_bytes);
+
+/* The sequences end: no tokens, and pages that no other sequence holds are
+ * free. */
+int pkb_cache4_free_dev(void *stream, const pkb_cache4 *c, const int32_t *seqs, uint32_t n, int32_t *status,
+                        void *work, size_t work_bytes);
+
+/* Pages in use move to the lowest places: with U of them in use (*used, if
+ * not null), the i-th in use at U or above goes, in every layer, to the
+ * i-th free below U, and the tables follow. */
+int pkb_cache4_compact_dev(void *stream, const pkb_cache4 *c, int32_t *used, int32_t *status, void *work,
+                           size_t work_bytes);
+
+/* Quantizes K and V rows into the cache's layer: rows starts[i] ..
+ * starts[i+1] - 1 of k and v (n_heads dk values of the type, rows ks and vs
+ * values apart) are the last tokens of sequence seqs[i], i < n, that lens
+ * counts already. seqs [n] and starts [n+1] are device arrays, starts from
+ * 0 to at most rows; rows behind starts[n] are not read. A sequence
+ * listed twice has no defined content. A sequence out of range, more rows
+ * than tokens or a table entry that is no page sets the device error word's
+ * bit 1, and nothing is written there. */
+int pkb_cache4_append_dev(void *stream, const pkb_cache4 *c, uint32_t layer, const void *k, size_t ks, const void *v,
+                          size_t vs, int type, const int32_t *seqs, const int32_t *starts, uint32_t n, uint32_t rows);
+
+/* The reverse: what the last starts[i+1] - starts[i] tokens of sequence
+ * seqs[i] stand for, into rows of k and v (rounded once for PKB_F16). Rows
+ * behind starts[n] are left as they were. */
+int pkb_cache4_read_dev(void *stream, const pkb_cache4 *c, uint32_t layer, void *k, size_t ks, void *v, size_t vs,
+                        int type, const int32_t *seqs, const int32_t *starts, uint32_t n, uint32_t rows);
+
+/* Device bytes of pkb_attention_cache4_dev's work area, 256-byte aligned,
+ * for up to n sequences and `rows` rows of H heads; 0 for sizes it refuses. */
+size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t rows, uint32_t n);
+
+/* Attention over the cache's layer. Rows starts[i] .. starts[i+1] - 1 of q
+ * (H heads of dk values of the type; H a multiple of n_heads, head h reads
+ * the cache's head h / (H / n_heads)) are the queries of sequence seqs[i]:
+ * with R of them and L = lens[seqs[i]], the r-th stands at position
+ * p = L - R + r. It attends to the tokens j < L, where `causal` is set to
+ * those with j <= p, and where `window` is not 0 to those with
+ * j > p - window:
+ *     o = sum_j softmax_j(scale q.k_j) v_j,
+ * zeros where there is no such j. No sequence has more than max_rows rows
+ * here (a hint: how the work is split depends on it, not what is computed).
+ * Products are exact in the type of q (bf16, two or three bf16 parts for
+ * f16 and f32), sums are float32, o is rounded once. Rows of o behind
+ * starts[n] are left as they were; o must not overlap q. work as for the
+ * page operations. What is out of range sets the device error word's bit
+ * 1, and such rows of o are not defined. */
+int pkb_attention_cache4_dev(void *stream, void *o, size_t os, const void *q, size_t qs, int type, uint32_t H,
+                             const pkb_cache4 *c, uint32_t layer, const int32_t *seqs, const int32_t *starts,
+                             uint32_t n, uint32_t rows, uint32_t max_rows, float scale, int causal, uint32_t window,
+                             void *work, size_t work_bytes);
+
 /* Launches of libpktito_b200 kernels since the process started, on every
  * device: the evidence a benchmark reports for its own kernels' work. */
 uint64_t pkb_launch_count(void);

@@ -126,6 +126,30 @@ _SIGS = {
     "pkb_layernorm_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
                                          ctypes.c_size_t, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p,
                                          ctypes.c_void_p, ctypes.c_float, ctypes.c_int]),
+    "pkb_cache4_page_bytes": (ctypes.c_size_t, [ctypes.c_uint32] * 3),
+    "pkb_cache4_work_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "pkb_cache4_reset_dev": (ctypes.c_int, [ctypes.c_void_p] * 2),
+    "pkb_cache4_grow_dev": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
+                                                                   ctypes.c_size_t]),
+    "pkb_cache4_fork_dev": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
+                                                                   ctypes.c_size_t]),
+    "pkb_cache4_copy_dev": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
+                                                                   ctypes.c_size_t]),
+    "pkb_cache4_free_dev": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
+                                                                   ctypes.c_size_t]),
+    "pkb_cache4_compact_dev": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_size_t]),
+    "pkb_cache4_append_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
+                                             ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int,
+                                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32]),
+    "pkb_cache4_read_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
+                                           ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32]),
+    "pkb_attention_cache4_work_bytes": (ctypes.c_size_t, [ctypes.c_void_p] + [ctypes.c_uint32] * 3),
+    "pkb_attention_cache4_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
+                                                ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32, ctypes.c_void_p,
+                                                ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
+                                                ctypes.c_uint32, ctypes.c_uint32, ctypes.c_float, ctypes.c_int,
+                                                ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t]),
     "pkb_launch_count": (ctypes.c_uint64, []),
     "pkb_tdt_last_rounds": (ctypes.c_uint64, []),
     "pkb_host_bytes": (None, [ctypes.c_void_p, ctypes.c_void_p]),
@@ -377,3 +401,134 @@ def gemm_q8_dev(out, os_: int, wpack, ws, bias, rows: int, q, d, n: int, qb: int
                 rmode: int = RN, stream=None) -> None:
     _check(lib().pkb_gemm_q8_dev(_stream(stream), _ptr(out), os_, _ptr(wpack), _ptr(ws), _ptr(bias), rows,
                                  _ptr(q), _ptr(d), n, qb, T, int(add), rmode))
+
+
+# ------------------------------------ a key/value cache held in 4 bits --
+
+F32, F16, BF16 = 0, 1, 2
+CACHE4_DONE, CACHE4_FULL, CACHE4_LONG, CACHE4_BAD = 0, 1, 2, 3
+
+
+class Cache4(ctypes.Structure):
+    """pkb_cache4 (include/pktito_b200.h): the device memory of a cache held in 4 bits."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "table", "lens", "refs")] + \
+               [(n, ctypes.c_uint32) for n in ("n_layers", "n_pages", "max_seqs", "max_pages", "page_tokens", "n_heads",
+                                               "head_dim")]
+
+    @classmethod
+    def of(cls, pages, table, lens, refs, page_tokens: int, n_heads: int, head_dim: int) -> "Cache4":
+        """The descriptor over device tensors, which it keeps alive: pages
+        uint8 [layers, pages, page bytes], table int32 [sequences, pages a
+        sequence], lens int32 [sequences], refs int32 [pages], all contiguous."""
+        import torch
+        each = cache4_page_bytes(page_tokens, n_heads, head_dim)
+        if not each:
+            raise PkbError(1, f"cache4: pages of {page_tokens} tokens, {n_heads} heads of {head_dim}")
+        for t, kind, shape in ((pages, torch.uint8, (pages.shape[0], refs.shape[0], each)),
+                               (table, torch.int32, (lens.shape[0], table.shape[-1])),
+                               (lens, torch.int32, (lens.shape[0],)), (refs, torch.int32, (refs.shape[0],))):
+            if t.dtype != kind or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != pages.device:
+                raise PkbError(1, f"cache4: a tensor of {t.dtype} {tuple(t.shape)} on {t.device}, contiguous {kind} "
+                                  f"{tuple(shape)} on {pages.device} expected")
+        c = cls(_ptr(pages), _ptr(table), _ptr(lens), _ptr(refs), pages.shape[0], refs.shape[0], *table.shape,
+                page_tokens, n_heads, head_dim)
+        c.tensors = (pages, table, lens, refs)
+        return c
+
+    @classmethod
+    def empty(cls, n_layers: int, n_pages: int, max_seqs: int, max_pages: int, page_tokens: int, n_heads: int,
+              head_dim: int, device="cuda") -> "Cache4":
+        """An empty cache in new tensors (``tensors``: pages, table, lens, refs)."""
+        import torch
+        return cls.of(torch.empty((n_layers, n_pages, cache4_page_bytes(page_tokens, n_heads, head_dim)),
+                                  dtype=torch.uint8, device=device),
+                      torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=device),
+                      torch.zeros(max_seqs, dtype=torch.int32, device=device),
+                      torch.zeros(n_pages, dtype=torch.int32, device=device), page_tokens, n_heads, head_dim)
+
+
+def _type(a) -> int:
+    import torch
+    kind = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(a.dtype)
+    if kind is None:
+        raise PkbError(1, f"a tensor of {a.dtype}: float32, float16 or bfloat16")
+    return kind
+
+
+def _bytes(work) -> int:
+    return work.numel() * work.element_size()
+
+
+def cache4_page_bytes(page_tokens: int, n_heads: int, head_dim: int) -> int:
+    return int(lib().pkb_cache4_page_bytes(page_tokens, n_heads, head_dim))
+
+
+def cache4_work_bytes(cache: Cache4) -> int:
+    return int(lib().pkb_cache4_work_bytes(ctypes.byref(cache)))
+
+
+def cache4_reset_dev(cache: Cache4, stream=None) -> None:
+    _check(lib().pkb_cache4_reset_dev(_stream(stream), ctypes.byref(cache)))
+
+
+def cache4_grow_dev(cache: Cache4, seqs, add, n: int, status, work, stream=None) -> None:
+    """Room for add[i] more tokens of sequence seqs[i]; status (device int32) as CACHE4_*."""
+    _check(lib().pkb_cache4_grow_dev(_stream(stream), ctypes.byref(cache), _ptr(seqs), _ptr(add), n, _ptr(status),
+                                     _ptr(work), _bytes(work)))
+
+
+def cache4_fork_dev(cache: Cache4, src, dst, lens, n: int, status, work, stream=None) -> None:
+    """The empty sequences dst take the first lens tokens of src, sharing their pages."""
+    _check(lib().pkb_cache4_fork_dev(_stream(stream), ctypes.byref(cache), _ptr(src), _ptr(dst), _ptr(lens), n,
+                                     _ptr(status), _ptr(work), _bytes(work)))
+
+
+def cache4_copy_dev(to: Cache4, cache: Cache4, src, dst, lens, n: int, status, work, stream=None) -> None:
+    """The empty sequences dst of `to` take the first lens tokens of src in pages of their own."""
+    _check(lib().pkb_cache4_copy_dev(_stream(stream), ctypes.byref(to), ctypes.byref(cache), _ptr(src), _ptr(dst),
+                                     _ptr(lens), n, _ptr(status), _ptr(work), _bytes(work)))
+
+
+def cache4_free_dev(cache: Cache4, seqs, n: int, status, work, stream=None) -> None:
+    _check(lib().pkb_cache4_free_dev(_stream(stream), ctypes.byref(cache), _ptr(seqs), n, _ptr(status), _ptr(work),
+                                     _bytes(work)))
+
+
+def cache4_compact_dev(cache: Cache4, used, status, work, stream=None) -> None:
+    """Pages in use move to the lowest places; used (device int32 or None): how many there are."""
+    _check(lib().pkb_cache4_compact_dev(_stream(stream), ctypes.byref(cache), _ptr(used), _ptr(status), _ptr(work),
+                                        _bytes(work)))
+
+
+def _same_type(a, b) -> int:
+    if a.dtype != b.dtype:
+        raise PkbError(1, f"tensors of {a.dtype} and {b.dtype}")
+    return _type(a)
+
+
+def cache4_append_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
+                      stream=None) -> None:
+    """K and V rows, ks and vs values apart, into the layer: rows starts[i] .. starts[i+1] - 1 are the last
+    tokens of sequence seqs[i]."""
+    _check(lib().pkb_cache4_append_dev(_stream(stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
+                                       _same_type(k, v), _ptr(seqs), _ptr(starts), n, rows))
+
+
+def cache4_read_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
+                    stream=None) -> None:
+    """What the last tokens of the sequences stand for, into rows of k and v."""
+    _check(lib().pkb_cache4_read_dev(_stream(stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
+                                     _same_type(k, v), _ptr(seqs), _ptr(starts), n, rows))
+
+
+def attention_cache4_work_bytes(cache: Cache4, H: int, rows: int, n: int) -> int:
+    return int(lib().pkb_attention_cache4_work_bytes(ctypes.byref(cache), H, rows, n))
+
+
+def attention_cache4_dev(o, os_: int, q, qs: int, H: int, cache: Cache4, layer: int, seqs, starts, n: int, rows: int,
+                         max_rows: int, scale: float, causal: bool, window: int, work, stream=None) -> None:
+    """Attention of q's rows (H heads) over the cache's layer: rows starts[i] .. starts[i+1] - 1 are the last
+    positions of sequence seqs[i]; window 0: the whole history."""
+    _check(lib().pkb_attention_cache4_dev(_stream(stream), _ptr(o), os_, _ptr(q), qs, _same_type(o, q), H,
+                                          ctypes.byref(cache), layer, _ptr(seqs), _ptr(starts), n, rows, max_rows, scale,
+                                          int(causal), window, _ptr(work), _bytes(work)))

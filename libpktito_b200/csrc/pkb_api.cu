@@ -104,6 +104,7 @@ int current_device(Device** out) {
             d.err = static_cast<uint32_t*>(sym);
             PKB_CUDA(prepare_gemm_q8(), "kernel attributes");
             PKB_CUDA(prepare_attention(), "kernel attributes");
+            PKB_CUDA(prepare_attention4(), "kernel attributes");
             prepare_quantize();
             d.sms = prop.multiProcessorCount;
             wait_limit();
@@ -853,6 +854,8 @@ int current_device_info(int* sms, uint32_t** err_word) {
     *err_word = d->err;
     return PKB_OK;
 }
+
+long long wait_cycles() { return wait_limit(); }
 
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 

@@ -1,0 +1,71 @@
+// The attention over a 4-bit cache: what its kernels share (the call's
+// arguments, the products of one unit, the online softmax).
+#pragma once
+
+#include "pkb_cache4.cuh"
+#include "pkb_device.cuh"
+
+namespace pkb {
+
+struct Attn4Args {
+    Cache4 c;
+    const void* q;
+    void* o;
+    size_t qs, os;
+    const int32_t *seqs, *starts;
+    uint32_t* err;
+    uint32_t layer, n, rows, H, G;  // G: query heads a cached head
+    float scale;                    // times log2 e
+    uint32_t causal, window;
+    long long timeout;
+    uint64_t* base;  // [n + 1] each entry's first tile
+    float* part;     // partial results, two a share
+    uint64_t max_shares;  // that the work area has room for
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// an 8 x 8 tile of 16-bit values, transposed across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+// two floats rounded to bf16, lo in the low half
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// x as PARTS bf16 numbers that add up to it: to its 8 first bits, or (2, 3
+// parts) to all of an f16's 11 and a float's 24. Each remainder is exact.
+template <int PARTS>
+__device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t (&r)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+        r[i] = bf16_pair(lo, hi);
+        if (i + 1 < PARTS) {
+            lo = __fsub_rn(lo, __uint_as_float(r[i] << 16));
+            hi = __fsub_rn(hi, __uint_as_float(r[i] & 0xFFFF0000u));
+        }
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+// e^x / e^m for partial sums: 1 where both are -inf (nothing seen yet)
+__device__ __forceinline__ float rescale(float from, float to) { return from == to ? 1.0f : exp2_fast(__fsub_rn(from, to)); }
+
+}  // namespace pkb

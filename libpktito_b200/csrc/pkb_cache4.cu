@@ -1,0 +1,807 @@
+// The cache held in 4 bits (include/pktito_b200.h, pkb_cache4): rows into its
+// pages and back, and its page operations.
+//
+// Rows. Append reads each value once (2 or 4 bytes) and writes 4.5 bits of
+// it, read does the reverse: both are bound by memory. A warp takes one
+// unit's K or V (16 tokens of one head), 8 blocks of 32 values a pass, four
+// lanes a block, so that a lane's eight values are one word of K's codes. V's
+// words mix 4 tokens and are put together from bytes in shared memory; a
+// byte is one token's, so a unit that the call covers in part is written a
+// byte at a time beside the tokens it leaves alone.
+//
+// Page operations. One block plans (it checks the lists, finds the lowest
+// free pages by a scan of refs, and refuses before anything is changed), a
+// grid applies: table rows, references and the pages' bytes. They are bound
+// by the copied bytes where pages are copied, else by the latency of the
+// plan's few dependent reads.
+
+#include <climits>
+
+#include "pkb_cache4.cuh"
+#include "pkb_device.cuh"
+#include "pkb_internal.h"
+
+namespace pkb {
+
+namespace {
+
+constexpr int ROW_WARPS = 8;
+constexpr uint32_t FULL = 0xFFFFFFFFu;
+
+// The entry i of a call that slot x belongs to. Entry i's units are counted
+// from starts[i] / 16 + 2 i: it has at most (rows + 30) / 16 of them, two
+// fewer than the distance to the next entry's first when rounded down, so
+// no scan over the entries is needed. Thirty-two probes a step.
+__device__ __forceinline__ uint32_t slot_entry(const int32_t* starts, uint32_t n, uint32_t x) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, hi = n;  // the answer is in [lo, hi)
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const bool below = i < hi && static_cast<uint32_t>(starts[i]) / C4_UNIT + 2 * i <= x;
+        const uint32_t last = 31 - __clz(__ballot_sync(FULL, below) | 1u);
+        lo += last * step;
+        hi = lo + step < hi ? lo + step : hi;
+    }
+    return lo;
+}
+
+struct RowArgs {
+    Cache4 c;
+    const int32_t *seqs, *starts;
+    uint32_t* err;
+    size_t ks, vs;
+    uint32_t layer, n, rows, slots;
+};
+
+// Where a warp's unit lies, and which of its tokens the call has: token r is
+// row `row0 + r` for r in [first, last).
+struct UnitRows {
+    uint8_t* bytes;
+    int64_t row0;
+    int first, last;
+};
+
+__device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, uint32_t h) {
+    UnitRows u = {nullptr, 0, 0, 0};
+    const uint32_t i = slot_entry(a.starts, a.n, slot);
+    uint32_t seq, r0;
+    const uint32_t rows = c4_rows(a.c, a.seqs, a.starts, i, a.rows, &seq, &r0, a.err);
+    if (!rows) return u;
+    const uint32_t len = c4_len(a.c, seq, a.err);
+    if (rows > len) {
+        if ((threadIdx.x & 31) == 0) atomicOr(a.err, 2u);
+        return u;
+    }
+    const uint32_t pos0 = len - rows, at = r0 / C4_UNIT + 2 * i, unit = pos0 / C4_UNIT + (slot - at);
+    if (slot < at || unit > (len - 1) / C4_UNIT) return u;  // the entry has no such unit
+    u.bytes = c4_unit(a.c, a.layer, seq, h, unit, a.err);
+    const int64_t t0 = static_cast<int64_t>(unit) * C4_UNIT - pos0;
+    u.row0 = r0 + t0;
+    u.first = t0 < 0 ? static_cast<int>(-t0) : 0;
+    u.last = static_cast<int64_t>(rows) - t0 < C4_UNIT ? static_cast<int>(rows - t0) : C4_UNIT;
+    return u;
+}
+
+template <int NB> __host__ __device__ constexpr int v_row() { return NB * 16 + 8; }  // a token's V bytes, and 8 against bank conflicts
+
+template <typename T, int NB, bool VEC>
+__global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* __restrict__ k, const T* __restrict__ v, RowArgs a) {
+    constexpr int DK = NB * 32;
+    __shared__ alignas(16) uint8_t stage[ROW_WARPS][C4_UNIT * v_row<NB>()];
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + warp;
+    const bool is_v = item & 1;
+    const uint32_t h = static_cast<uint32_t>((item >> 1) % a.c.heads);
+    const size_t slot = (item >> 1) / a.c.heads;
+    if (slot >= a.slots) return;
+    const UnitRows u = warp_unit(a, static_cast<uint32_t>(slot), h);
+    if (!u.bytes) return;
+    const T* x = is_v ? v : k;
+    const size_t xs = is_v ? a.vs : a.ks;
+    uint8_t* codes = u.bytes + (is_v ? 8 * DK : 0);
+    __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(u.bytes + (is_v ? 17 * DK : 16 * DK));
+    uint8_t* vb = stage[warp];
+#pragma unroll 4
+    for (int pass = 0; pass < 2 * NB; pass++) {
+        const int b = pass * 8 + lane / 4, token = b / NB, blk = b % NB, t = lane & 3;
+        const bool valid = token >= u.first && token < u.last;
+        if (!__any_sync(FULL, valid)) continue;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = 0.0f;
+        if (valid) c4_load8<T, VEC>(x + (u.row0 + token) * xs + h * DK + blk * 32 + t * 8, f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max(m, abs_bits(f[i]));
+        m = max(m, __shfl_xor_sync(FULL, m, 1));
+        m = max(m, __shfl_xor_sync(FULL, m, 2));
+        // 5 significant bits of amax / 7, cut: 7 s is at most amax (no
+        // overflow) and amax / s below 7.47, so every code is within 7. The
+        // correctly rounded quotients round to an integer as the exact ones
+        // do: with s of 5 bits x / s is never so near a half, or amax / 7 a
+        // number of 5 bits, that the float quotient would meet it.
+        const bool scaled = block_scaled(m);
+        const float s = scaled ? __uint_as_float(__float_as_uint(__fdiv_rn(__uint_as_float(m), 7.0f)) & 0xFFF80000u) : 1.0f;
+        uint32_t nib[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)  // 8 + rint(x / s) in the low bits of 1.5 * 2^23 + 8 + x / s
+            nib[i] = scaled ? __float_as_uint(__fadd_rn(__fdiv_rn(f[i], s), 12582920.0f)) & 15u : 8u;
+        const __nv_bfloat16 sb = __float2bfloat16_rn(scaled ? s : 0.0f);  // exact: 5 bits
+        if (!is_v) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) w |= nib[i] << (4 * (i / 2) + 16 * (i % 2));
+            if (valid) {
+                reinterpret_cast<uint32_t*>(codes)[(token * 4 + t) * NB + blk] = w;
+                if (t == 0) scales[token * NB + blk] = sb;
+            }
+        } else {
+            const uint32_t lo = nib[0] | nib[1] << 8 | nib[2] << 16 | nib[3] << 24;
+            const uint32_t hi = nib[4] | nib[5] << 8 | nib[6] << 16 | nib[7] << 24;
+            // values 8 apart share a byte: the even lane of a pair makes the first four bytes, the odd one the others
+            const uint32_t got = __shfl_xor_sync(FULL, t & 1 ? lo : hi, 1);
+            const uint32_t w = t & 1 ? got | hi << 4 : lo | got << 4;
+            *reinterpret_cast<uint32_t*>(vb + token * v_row<NB>() + (blk * 2 + t / 2) * 8 + (t & 1) * 4) = w;
+            if (valid && t == 0) scales[blk * C4_UNIT + token] = sb;
+        }
+    }
+    if (!is_v) return;
+    __syncwarp();
+    const uint32_t have = (0xFFFFu >> (C4_UNIT - u.last)) & (0xFFFFu << u.first);
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) {
+        const int wi = i * 32 + lane, blk = wi / 64, g = wi / 8 % 8, t = wi / 2 % 4, j = wi % 2;
+        const uint8_t* at = vb + (blk * 2 + j) * 8 + g;
+        // byte 2 e + c of a word is token 8 c + 2 t + e
+        const uint32_t mine = have >> (2 * t);
+        if ((mine & 0x0303u) == 0) continue;
+        uint8_t y[4];
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) y[2 * e + c] = at[(8 * c + 2 * t + e) * v_row<NB>()];
+        if ((mine & 0x0303u) == 0x0303u) {
+            reinterpret_cast<uint32_t*>(codes)[wi] = y[0] | y[1] << 8 | y[2] << 16 | static_cast<uint32_t>(y[3]) << 24;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+                    if (mine >> (8 * c + e) & 1) codes[4 * wi + 2 * e + c] = y[2 * e + c];
+        }
+    }
+}
+
+template <typename T, int NB, bool VEC>
+__global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* __restrict__ k, T* __restrict__ v, RowArgs a) {
+    constexpr int DK = NB * 32;
+    __shared__ uint32_t stage[ROW_WARPS][NB * 72];  // 64 words a block of V, and 8 against bank conflicts
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + warp;
+    const bool is_v = item & 1;
+    const uint32_t h = static_cast<uint32_t>((item >> 1) % a.c.heads);
+    const size_t slot = (item >> 1) / a.c.heads;
+    if (slot >= a.slots) return;
+    const UnitRows u = warp_unit(a, static_cast<uint32_t>(slot), h);
+    if (!u.bytes) return;
+    T* x = is_v ? v : k;
+    const size_t xs = is_v ? a.vs : a.ks;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(u.bytes + (is_v ? 8 * DK : 0));
+    const uint16_t* scales = reinterpret_cast<const uint16_t*>(u.bytes + (is_v ? 17 * DK : 16 * DK));
+    uint32_t* vw = stage[warp];
+    if (is_v) {
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) vw[i / 2 * 72 + i % 2 * 32 + lane] = codes[i * 32 + lane];
+        __syncwarp();
+    }
+#pragma unroll 4
+    for (int pass = 0; pass < 2 * NB; pass++) {
+        const int b = pass * 8 + lane / 4, token = b / NB, blk = b % NB, t = lane & 3;
+        if (token < u.first || token >= u.last) continue;
+        float f[8];
+        if (!is_v) {
+            const uint32_t w = codes[(token * 4 + t) * NB + blk];
+            const float s = c4_bf16(scales[token * NB + blk]);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                f[i] = __fmul_rn(static_cast<float>(static_cast<int>(w >> (4 * (i / 2) + 16 * (i % 2)) & 15u) - 8), s);
+        } else {
+            const float s = c4_bf16(scales[blk * C4_UNIT + token]);
+            const int shift = 8 * (2 * (token & 1) + token / 8) + 4 * (t & 1);
+#pragma unroll
+            for (int g = 0; g < 8; g++)
+                f[g] = __fmul_rn(
+                    static_cast<float>(static_cast<int>(vw[blk * 72 + g * 8 + token % 8 / 2 * 2 + t / 2] >> shift & 15u) - 8), s);
+        }
+        c4_store8<T, VEC>(x + (u.row0 + token) * xs + h * DK + blk * 32 + t * 8, f);
+    }
+}
+
+// ------------------------------------------------------------ page operations --
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_REFS = 16;  // refs a thread looks at a step
+constexpr uint32_t COPY_CHUNK = 16384;
+
+enum { OP_GROW = 0, OP_FORK = 1, OP_COPY = 2, OP_FREE = 3 };
+
+// The work area: counts, then a mark a sequence, each entry's first new
+// page, the free pages taken, and the pages to copy from and to. compact
+// uses the last three for the holes, the pages that move and where to.
+struct PlanWork {
+    uint32_t* count;  // [0] new pages (compact: pages that move), [1] used pages
+    uint32_t *mark, *first, *page, *from, *to;
+};
+
+struct PlanArgs {
+    Cache4 c, src;  // src: copy's other cache (else c)
+    const int32_t *a, *b, *num;  // sequences (the ones read first), added or taken tokens
+    uint32_t n;
+    int op;
+    int32_t* status;
+    PlanWork w;
+};
+
+// The sum of x over the threads before this one, and over all in *total.
+template <typename T>
+__device__ __forceinline__ T block_scan(T x, T* total, T* buf) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    T s = x;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const T y = __shfl_up_sync(FULL, s, d);
+        if (lane >= d) s += y;
+    }
+    if (lane == 31) buf[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+        T z = buf[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const T y = __shfl_up_sync(FULL, z, d);
+            if (lane >= d) z += y;
+        }
+        buf[lane] = z;
+    }
+    __syncthreads();
+    *total = buf[31];
+    const T before = (warp ? buf[warp - 1] : 0) + s - x;
+    __syncthreads();
+    return before;
+}
+
+__device__ __forceinline__ uint32_t pages_of(const Cache4& c, uint32_t tokens) {
+    return static_cast<uint32_t>((static_cast<uint64_t>(tokens) + (1u << c.pshift) - 1) >> c.pshift);
+}
+
+// Entry i's new pages, and what is wrong with it.
+__device__ __forceinline__ uint32_t plan_entry(const PlanArgs& p, uint32_t i, int* bad) {
+    const int32_t* changed = p.op == OP_FORK || p.op == OP_COPY ? p.b : p.a;
+    const int32_t s = changed[i];
+    if (s < 0 || static_cast<uint32_t>(s) >= p.c.max_seqs) {
+        *bad = PKB_CACHE4_BAD;
+        return 0;
+    }
+    p.w.mark[s] = i;
+    if (p.op == OP_FREE) return 0;
+    const int32_t num = p.num[i], len = p.c.lens[s];
+    const uint64_t room = static_cast<uint64_t>(p.c.max_pages) << p.c.pshift;
+    if (num < 0 || len < 0) {
+        *bad = PKB_CACHE4_BAD;
+        return 0;
+    }
+    if (p.op == OP_GROW) {
+        const uint64_t after = static_cast<uint64_t>(len) + num;
+        if (after > room || after > INT_MAX) {
+            *bad = max(*bad, static_cast<int>(PKB_CACHE4_LONG));
+            return 0;
+        }
+        return pages_of(p.c, static_cast<uint32_t>(after)) - pages_of(p.c, len);
+    }
+    const int32_t r = p.a[i];
+    if (len != 0 || r < 0 || static_cast<uint32_t>(r) >= p.src.max_seqs || num > p.src.lens[r]) {
+        *bad = PKB_CACHE4_BAD;
+        return 0;
+    }
+    if (static_cast<uint64_t>(num) > room || static_cast<uint64_t>(num) > static_cast<uint64_t>(p.src.max_pages) << p.src.pshift) {
+        *bad = max(*bad, static_cast<int>(PKB_CACHE4_LONG));
+        return 0;
+    }
+    return p.op == OP_COPY ? pages_of(p.c, num) : (num & ((1u << p.c.pshift) - 1)) != 0;
+}
+
+__device__ __forceinline__ uint32_t entry_of(const uint32_t* first, uint32_t n, uint32_t j) {
+    uint32_t lo = 0, hi = n;  // the last i with first[i] <= j
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (first[mid] <= j) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// The 16 refs of a thread's step at p0, those past the end as used.
+__device__ __forceinline__ void load_refs(const Cache4& c, uint32_t p0, int32_t (&r)[PLAN_REFS]) {
+    if (p0 + PLAN_REFS <= c.n_pages && (reinterpret_cast<uintptr_t>(c.refs) & 15) == 0) {
+#pragma unroll
+        for (int q = 0; q < PLAN_REFS / 4; q++) {
+            const int4 v = reinterpret_cast<const int4*>(c.refs + p0)[q];
+            r[4 * q] = v.x, r[4 * q + 1] = v.y, r[4 * q + 2] = v.z, r[4 * q + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < PLAN_REFS; q++) r[q] = p0 + q < c.n_pages ? c.refs[p0 + q] : 1;
+    }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
+    __shared__ uint32_t buf[32];
+    __shared__ uint64_t wide[32];
+    __shared__ int worst;
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t tid = threadIdx.x;
+    if (tid == 0) worst = 0;
+    __syncthreads();
+    int bad = 0;
+    uint64_t wanted = 0;  // a sum of wishes, which may pass 32 bits
+    for (uint32_t i0 = 0; i0 < p.n; i0 += PLAN_THREADS) {
+        const uint32_t i = i0 + tid;
+        const uint64_t need = i < p.n ? plan_entry(p, i, &bad) : 0;
+        uint64_t sum;
+        const uint64_t before = block_scan(need, &sum, wide);
+        if (i < p.n) p.w.first[i] = static_cast<uint32_t>(wanted + before);
+        wanted += sum;
+    }
+    if (wanted > p.c.n_pages) bad = max(bad, static_cast<int>(PKB_CACHE4_FULL));
+    const uint32_t total = static_cast<uint32_t>(wanted);
+    __syncthreads();
+    // a sequence listed twice has one of its entries' marks
+    const int32_t* changed = p.op == OP_FORK || p.op == OP_COPY ? p.b : p.a;
+    for (uint32_t i = tid; i < p.n; i += PLAN_THREADS) {
+        const int32_t s = changed[i];
+        if (s >= 0 && static_cast<uint32_t>(s) < p.c.max_seqs && p.w.mark[s] != i) bad = PKB_CACHE4_BAD;
+    }
+    if (bad) atomicMax(&worst, bad);
+    __syncthreads();
+    uint32_t found = 0;
+    if (!worst) {
+        for (uint32_t q0 = 0; q0 < p.c.n_pages && found < total; q0 += PLAN_THREADS * PLAN_REFS) {
+            const uint32_t p0 = q0 + tid * PLAN_REFS;
+            int32_t r[PLAN_REFS];
+            load_refs(p.c, p0, r);
+            uint32_t mine = 0;
+#pragma unroll
+            for (int q = 0; q < PLAN_REFS; q++) mine += r[q] == 0;
+            uint32_t sum;
+            uint32_t at = found + block_scan(mine, &sum, buf);
+#pragma unroll
+            for (int q = 0; q < PLAN_REFS; q++)
+                if (r[q] == 0 && at < total) p.w.page[at++] = p0 + q;
+            found += sum;
+        }
+    }
+    const int status = worst ? worst : found < total ? static_cast<int>(PKB_CACHE4_FULL) : 0;
+    if (tid == 0) {
+        *p.status = status;
+        p.w.count[0] = status ? 0 : total;
+    }
+    if (status) return;
+    __syncthreads();
+    for (uint32_t j = tid; j < total; j += PLAN_THREADS) {
+        const uint32_t i = entry_of(p.w.first, p.n, j), k = j - p.w.first[i], page = p.w.page[j];
+        const uint32_t s = static_cast<uint32_t>(changed[i]);
+        uint32_t place = k;
+        if (p.op == OP_GROW) place += pages_of(p.c, p.c.lens[s]);
+        if (p.op == OP_FORK) place = static_cast<uint32_t>(p.num[i]) >> p.c.pshift;
+        p.c.table[static_cast<size_t>(s) * p.c.max_pages + place] = static_cast<int32_t>(page);
+        p.c.refs[page] = 1;
+        if (p.op != OP_GROW) {
+            const int32_t from = p.src.table[static_cast<size_t>(p.a[i]) * p.src.max_pages + place];
+            p.w.from[j] = static_cast<uint32_t>(from);
+            p.w.to[j] = page;
+        }
+    }
+    if (p.op == OP_GROW) {
+        __syncthreads();  // lens is read above
+        for (uint32_t i = tid; i < p.n; i += PLAN_THREADS) p.c.lens[p.a[i]] += p.num[i];
+    }
+}
+
+// The pages listed in from and to, every layer, COPY_CHUNK bytes a block
+// and step.
+__device__ void copy_pages(const Cache4& c, const Cache4& src, const PlanWork& w, uint32_t* err) {
+    const uint32_t chunks = static_cast<uint32_t>((c.page_bytes + COPY_CHUNK - 1) / COPY_CHUNK);
+    const uint64_t all = static_cast<uint64_t>(w.count[0]) * c.n_layers * chunks;
+    for (uint64_t x = blockIdx.x; x < all; x += gridDim.x) {
+        const uint32_t chunk = static_cast<uint32_t>(x % chunks), layer = static_cast<uint32_t>(x / chunks % c.n_layers);
+        const uint64_t j = x / chunks / c.n_layers;
+        const uint32_t from = w.from[j], to = w.to[j];
+        if (from >= src.n_pages || to >= c.n_pages) {
+            if (threadIdx.x == 0) atomicOr(err, 2u);
+            continue;
+        }
+        const size_t at = static_cast<size_t>(chunk) * COPY_CHUNK;
+        const uint32_t words = static_cast<uint32_t>((c.page_bytes - at < COPY_CHUNK ? c.page_bytes - at : COPY_CHUNK) / 16);
+        const uint4* x4 = reinterpret_cast<const uint4*>(src.pages + layer * src.layer_bytes + from * src.page_bytes + at);
+        uint4* y4 = reinterpret_cast<uint4*>(c.pages + layer * c.layer_bytes + to * c.page_bytes + at);
+        uint4 v[COPY_CHUNK / 16 / 256];
+#pragma unroll
+        for (int q = 0; q < static_cast<int>(COPY_CHUNK / 16 / 256); q++)
+            if (threadIdx.x + q * 256 < words) v[q] = x4[threadIdx.x + q * 256];
+#pragma unroll
+        for (int q = 0; q < static_cast<int>(COPY_CHUNK / 16 / 256); q++)
+            if (threadIdx.x + q * 256 < words) y4[threadIdx.x + q * 256] = v[q];
+    }
+}
+
+// fork's and copy's bytes, and fork's shared pages; free's references.
+__global__ void __launch_bounds__(256) apply_kernel(PlanArgs p, uint32_t* err) {
+    pdl_trigger();
+    pdl_wait();
+    if (*p.status) return;
+    for (uint32_t i = blockIdx.x; i < p.n; i += gridDim.x) {
+        if (p.op == OP_FREE) {
+            const size_t row = static_cast<size_t>(p.a[i]) * p.c.max_pages;
+            for (uint32_t j = threadIdx.x; j < p.c.max_pages; j += 256) {
+                const int32_t page = p.c.table[row + j];
+                if (page < 0) continue;
+                if (static_cast<uint32_t>(page) < p.c.n_pages) atomicSub(p.c.refs + page, 1);
+                else atomicOr(err, 2u);
+                p.c.table[row + j] = -1;
+            }
+            if (threadIdx.x == 0) p.c.lens[p.a[i]] = 0;
+            continue;
+        }
+        if (p.op == OP_FORK) {
+            const size_t from = static_cast<size_t>(p.a[i]) * p.c.max_pages, to = static_cast<size_t>(p.b[i]) * p.c.max_pages;
+            const uint32_t whole = static_cast<uint32_t>(p.num[i]) >> p.c.pshift;
+            for (uint32_t j = threadIdx.x; j < whole; j += 256) {
+                const int32_t page = p.c.table[from + j];
+                p.c.table[to + j] = page;
+                if (page >= 0 && static_cast<uint32_t>(page) < p.c.n_pages) atomicAdd(p.c.refs + page, 1);
+                else atomicOr(err, 2u);
+            }
+        }
+        if (threadIdx.x == 0) p.c.lens[p.b[i]] = p.num[i];
+    }
+    if (p.op != OP_FREE) copy_pages(p.c, p.src, p.w, err);
+}
+
+// compact: the holes below the count of used pages and the used pages from
+// there on, each in order; the i-th of these goes to the i-th of those.
+__global__ void __launch_bounds__(PLAN_THREADS) compact_plan_kernel(Cache4 c, PlanWork w, int32_t* used, int32_t* status) {
+    __shared__ uint32_t buf[32];
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t tid = threadIdx.x;
+    uint32_t count = 0;
+    for (uint32_t p0 = tid * PLAN_REFS; p0 < c.n_pages; p0 += PLAN_THREADS * PLAN_REFS) {
+        int32_t r[PLAN_REFS];
+        load_refs(c, p0, r);
+#pragma unroll
+        for (int q = 0; q < PLAN_REFS; q++) count += p0 + q < c.n_pages && r[q] != 0;
+    }
+    uint32_t total;
+    block_scan(count, &total, buf);
+    uint32_t holes = 0, moves = 0;
+    for (uint32_t q0 = 0; q0 < c.n_pages; q0 += PLAN_THREADS * PLAN_REFS) {
+        const uint32_t p0 = q0 + tid * PLAN_REFS;
+        int32_t r[PLAN_REFS];
+        load_refs(c, p0, r);
+        uint32_t h = 0, m = 0;
+#pragma unroll
+        for (int q = 0; q < PLAN_REFS; q++) {
+            h += p0 + q < total && r[q] == 0;
+            m += p0 + q >= total && p0 + q < c.n_pages && r[q] != 0;
+        }
+        uint32_t hs, ms;
+        uint32_t hat = holes + block_scan(h, &hs, buf), mat = moves + block_scan(m, &ms, buf);
+#pragma unroll
+        for (int q = 0; q < PLAN_REFS; q++) {
+            if (p0 + q < total && r[q] == 0) w.to[hat++] = p0 + q;
+            if (p0 + q >= total && p0 + q < c.n_pages && r[q] != 0) w.from[mat++] = p0 + q;
+        }
+        holes += hs;
+        moves += ms;
+    }
+    __syncthreads();
+    for (uint32_t j = tid; j < moves; j += PLAN_THREADS) w.page[w.from[j]] = w.to[j];
+    if (tid == 0) {
+        w.count[0] = moves;
+        w.count[1] = total;
+        if (used) *used = static_cast<int32_t>(total);
+        *status = PKB_CACHE4_DONE;
+    }
+}
+
+__global__ void __launch_bounds__(256) compact_apply_kernel(Cache4 c, PlanWork w, uint32_t* err) {
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t moves = w.count[0], total = w.count[1];
+    if (!moves) return;
+    const size_t entries = static_cast<size_t>(c.max_seqs) * c.max_pages, first = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    for (size_t i = first; i < entries; i += static_cast<size_t>(gridDim.x) * 256) {
+        const int32_t page = c.table[i];
+        // a page from `total` on that a table names is in use, so it has a place
+        if (page >= static_cast<int32_t>(total) && static_cast<uint32_t>(page) < c.n_pages) c.table[i] = static_cast<int32_t>(w.page[page]);
+    }
+    for (size_t j = first; j < moves; j += static_cast<size_t>(gridDim.x) * 256) {
+        c.refs[w.to[j]] = c.refs[w.from[j]];
+        c.refs[w.from[j]] = 0;
+    }
+    copy_pages(c, c, w, err);
+}
+
+__global__ void __launch_bounds__(256) reset_kernel(Cache4 c) {
+    pdl_trigger();
+    pdl_wait();
+    const size_t first = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<size_t>(gridDim.x) * 256;
+    for (size_t i = first; i < static_cast<size_t>(c.max_seqs) * c.max_pages; i += step) c.table[i] = -1;
+    for (size_t i = first; i < c.max_seqs; i += step) c.lens[i] = 0;
+    for (size_t i = first; i < c.n_pages; i += step) c.refs[i] = 0;
+}
+
+// ------------------------------------------------------------------- host --
+
+size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+size_t plan_layout(const pkb_cache4* c, uint8_t* base, PlanWork* w) {
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(base + at);
+        at += up256(n * 4);
+        return p;
+    };
+    w->count = take(64);
+    w->mark = take(c->max_seqs);
+    w->first = take(static_cast<size_t>(c->max_seqs) + 1);
+    w->page = take(c->n_pages);
+    w->from = take(c->n_pages);
+    w->to = take(c->n_pages);
+    return at;
+}
+
+bool is_aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+int cuda_error(cudaError_t e, const char* who) {
+    return set_error(e == cudaErrorMemoryAllocation ? PKB_ENOMEM : PKB_ECUDA, "%s launch: %s", who, cudaGetErrorString(e));
+}
+
+int check_plan(const pkb_cache4* c, const char* who, int32_t* status, void* work, size_t work_bytes, Cache4* v, PlanWork* w) {
+    int rc = c4_view(c, who, v);
+    if (rc) return rc;
+    if (!status || !work) return set_error(PKB_EINVAL, "%s: null pointer", who);
+    if (!is_aligned(status, 4) || !is_aligned(work, 256)) return set_error(PKB_EINVAL, "%s: misaligned status or work area", who);
+    const size_t need = plan_layout(c, static_cast<uint8_t*>(work), w);
+    if (work_bytes < need) return set_error(PKB_EINVAL, "%s: work area of %zu bytes, %zu needed", who, work_bytes, need);
+    return PKB_OK;
+}
+
+int page_op(cudaStream_t stream, int op, const char* who, const pkb_cache4* c, const pkb_cache4* src, const int32_t* a,
+            const int32_t* b, const int32_t* num, uint32_t n, int32_t* status, void* work, size_t work_bytes) {
+    PlanArgs p = {};
+    int rc = check_plan(c, who, status, work, work_bytes, &p.c, &p.w);
+    if (rc) return rc;
+    p.src = p.c;
+    if (src != c) {
+        if ((rc = c4_view(src, who, &p.src))) return rc;
+        if (src->n_layers != c->n_layers || src->page_tokens != c->page_tokens || src->n_heads != c->n_heads ||
+            src->head_dim != c->head_dim)
+            return set_error(PKB_EINVAL, "%s: the two caches differ in layers, page_tokens, heads or head_dim", who);
+    }
+    if (n > c->max_seqs) return set_error(PKB_EINVAL, "%s: %u entries for %u sequences", who, n, c->max_seqs);
+    const bool two = op == OP_FORK || op == OP_COPY;
+    if (n && (!a || (two && !b) || (op != OP_FREE && !num))) return set_error(PKB_EINVAL, "%s: null pointer", who);
+    if (!is_aligned(a, 4) || !is_aligned(b, 4) || !is_aligned(num, 4)) return set_error(PKB_EINVAL, "%s: misaligned list", who);
+    int sms;
+    uint32_t* err;
+    if ((rc = current_device_info(&sms, &err))) return rc;
+    p.a = a;
+    p.b = b;
+    p.num = num;
+    p.n = n;
+    p.op = op;
+    p.status = status;
+    cudaError_t e = c4_launch(plan_kernel, 1, PLAN_THREADS, 0, stream, p);
+    if (e != cudaSuccess) return cuda_error(e, who);
+    count_launch();
+    if (op == OP_GROW || !n) return PKB_OK;
+    // a block an entry, or enough blocks that a copy keeps every SM's loads in flight
+    const uint64_t most = op == OP_FREE ? n : n + static_cast<uint64_t>(op == OP_FORK ? n : c->n_pages) * c->n_layers *
+                                                      ((p.c.page_bytes + COPY_CHUNK - 1) / COPY_CHUNK);
+    const uint32_t grid = static_cast<uint32_t>(most < 8u * sms ? most : 8u * sms);
+    e = c4_launch(apply_kernel, grid, 256, 0, stream, p, err);
+    if (e != cudaSuccess) return cuda_error(e, who);
+    count_launch();
+    return PKB_OK;
+}
+
+template <typename T, int NB>
+cudaError_t launch_rows(bool append, bool vec, void* k, void* v, const RowArgs& a, cudaStream_t s) {
+    const size_t warps = 2 * static_cast<size_t>(a.slots) * a.c.heads;
+    const dim3 grid(static_cast<uint32_t>((warps + ROW_WARPS - 1) / ROW_WARPS)), block(ROW_WARPS * 32);
+    const T *kc = static_cast<const T*>(k), *vc = static_cast<const T*>(v);
+    T *ko = static_cast<T*>(k), *vo = static_cast<T*>(v);
+    if (append)
+        return vec ? c4_launch(append_kernel<T, NB, true>, grid, block, 0, s, kc, vc, a)
+                   : c4_launch(append_kernel<T, NB, false>, grid, block, 0, s, kc, vc, a);
+    return vec ? c4_launch(read_kernel<T, NB, true>, grid, block, 0, s, ko, vo, a)
+               : c4_launch(read_kernel<T, NB, false>, grid, block, 0, s, ko, vo, a);
+}
+
+template <typename T>
+cudaError_t launch_rows_dk(bool append, bool vec, void* k, void* v, const RowArgs& a, cudaStream_t s) {
+    switch (a.c.dk) {
+        case 32: return launch_rows<T, 1>(append, vec, k, v, a, s);
+        case 64: return launch_rows<T, 2>(append, vec, k, v, a, s);
+        case 96: return launch_rows<T, 3>(append, vec, k, v, a, s);
+        case 128: return launch_rows<T, 4>(append, vec, k, v, a, s);
+        default: return launch_rows<T, 8>(append, vec, k, v, a, s);
+    }
+}
+
+int rows_call(cudaStream_t stream, bool append, const pkb_cache4* c, uint32_t layer, void* k, size_t ks, void* v, size_t vs,
+              int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows) {
+    const char* who = append ? "cache4_append" : "cache4_read";
+    RowArgs a = {};
+    int rc = c4_view(c, who, &a.c);
+    if (rc) return rc;
+    if ((rc = c4_check_type(type, who))) return rc;
+    if (layer >= c->n_layers) return set_error(PKB_EINVAL, "%s: layer %u of %u", who, layer, c->n_layers);
+    if (!n || !rows) return PKB_OK;
+    if (!k || !v || !seqs || !starts) return set_error(PKB_EINVAL, "%s: null pointer", who);
+    const size_t width = static_cast<size_t>(c->n_heads) * c->head_dim, size = c4_type_bytes(type);
+    if (rows > 1 && (ks < width || vs < width)) return set_error(PKB_EINVAL, "%s: a row stride below %zu values", who, width);
+    if (rows == 1) ks = vs = width;
+    if (!is_aligned(k, size) || !is_aligned(v, size) || !is_aligned(seqs, 4) || !is_aligned(starts, 4))
+        return set_error(PKB_EINVAL, "%s: misaligned buffer", who);
+    const uint64_t slots = static_cast<uint64_t>(rows) / C4_UNIT + 2 * static_cast<uint64_t>(n);
+    if (rows > INT_MAX || slots * 2 * c->n_heads / ROW_WARPS >= INT_MAX)
+        return set_error(PKB_EINVAL, "%s: %u rows of %u sequences are too many for one launch", who, rows, n);
+    uint32_t* err;
+    int sms;
+    if ((rc = current_device_info(&sms, &err))) return rc;
+    a.seqs = seqs;
+    a.starts = starts;
+    a.err = err;
+    a.ks = ks;
+    a.vs = vs;
+    a.layer = layer;
+    a.n = n;
+    a.rows = rows;
+    a.slots = static_cast<uint32_t>(slots);
+    const bool vec = is_aligned(k, 16) && is_aligned(v, 16) && ks * size % 16 == 0 && vs * size % 16 == 0;
+    const cudaError_t e = type == PKB_F32   ? launch_rows_dk<float>(append, vec, k, v, a, stream)
+                          : type == PKB_F16 ? launch_rows_dk<__half>(append, vec, k, v, a, stream)
+                                            : launch_rows_dk<__nv_bfloat16>(append, vec, k, v, a, stream);
+    if (e != cudaSuccess) return cuda_error(e, who);
+    count_launch();
+    return PKB_OK;
+}
+
+}  // namespace
+
+int c4_check_type(int type, const char* who) {
+    if (type != PKB_F32 && type != PKB_F16 && type != PKB_BF16) return set_error(PKB_EINVAL, "%s: type %d", who, type);
+    return PKB_OK;
+}
+
+int c4_view(const pkb_cache4* c, const char* who, Cache4* v) {
+    if (!c) return set_error(PKB_EINVAL, "%s: null cache", who);
+    const size_t page = pkb_cache4_page_bytes(c->page_tokens, c->n_heads, c->head_dim);
+    if (!page)
+        return set_error(PKB_EINVAL, "%s: pages of %u tokens, %u heads of %u: 16 to 256 tokens, a power of two; heads of 32, 64, 96, 128 or 256",
+                         who, c->page_tokens, c->n_heads, c->head_dim);
+    if (!c->n_layers || !c->n_pages || !c->max_seqs || !c->max_pages || c->n_pages > INT_MAX || c->max_seqs > INT_MAX ||
+        static_cast<uint64_t>(c->max_pages) * c->page_tokens > INT_MAX)
+        return set_error(PKB_EINVAL, "%s: %u layers, %u pages, %u sequences of up to %u pages", who, c->n_layers, c->n_pages,
+                         c->max_seqs, c->max_pages);
+    if (!c->pages || !c->table || !c->lens || !c->refs) return set_error(PKB_EINVAL, "%s: null pointer in the cache", who);
+    if (!is_aligned(c->pages, 16) || !is_aligned(c->table, 4) || !is_aligned(c->lens, 4) || !is_aligned(c->refs, 4))
+        return set_error(PKB_EINVAL, "%s: the cache's pages must be 16-byte aligned, its lists 4-byte", who);
+    v->pages = c->pages;
+    v->table = c->table;
+    v->lens = c->lens;
+    v->refs = c->refs;
+    v->n_layers = c->n_layers;
+    v->n_pages = c->n_pages;
+    v->max_seqs = c->max_seqs;
+    v->max_pages = c->max_pages;
+    v->heads = c->n_heads;
+    v->dk = c->head_dim;
+    v->pshift = 4;
+    while (1u << v->pshift < c->page_tokens) v->pshift++;
+    v->unit_bytes = 18 * c->head_dim;
+    v->head_bytes = static_cast<size_t>(c->page_tokens / C4_UNIT) * v->unit_bytes;
+    v->page_bytes = page;
+    v->layer_bytes = page * c->n_pages;
+    return PKB_OK;
+}
+
+}  // namespace pkb
+
+using namespace pkb;
+
+extern "C" {
+
+size_t pkb_cache4_page_bytes(uint32_t page_tokens, uint32_t n_heads, uint32_t head_dim) {
+    if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1))) return 0;
+    if (head_dim != 32 && head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256) return 0;
+    if (!n_heads || n_heads > 65535) return 0;
+    return static_cast<size_t>(page_tokens / 16) * 18 * head_dim * n_heads;
+}
+
+size_t pkb_cache4_work_bytes(const pkb_cache4* c) {
+    PlanWork w;
+    if (!c || !c->n_pages || !c->max_seqs) return 0;
+    return plan_layout(c, nullptr, &w);
+}
+
+int pkb_cache4_reset_dev(void* stream, const pkb_cache4* c) {
+    Cache4 v;
+    int rc = c4_view(c, "cache4_reset", &v), sms;
+    uint32_t* err;
+    if (rc || (rc = current_device_info(&sms, &err))) return rc;
+    const cudaError_t e = c4_launch(reset_kernel, static_cast<uint32_t>(2 * sms), 256, 0, static_cast<cudaStream_t>(stream), v);
+    if (e != cudaSuccess) return cuda_error(e, "cache4_reset");
+    count_launch();
+    return PKB_OK;
+}
+
+int pkb_cache4_grow_dev(void* stream, const pkb_cache4* c, const int32_t* seqs, const int32_t* add, uint32_t n,
+                        int32_t* status, void* work, size_t work_bytes) {
+    return page_op(static_cast<cudaStream_t>(stream), OP_GROW, "cache4_grow", c, c, seqs, nullptr, add, n, status, work, work_bytes);
+}
+
+int pkb_cache4_fork_dev(void* stream, const pkb_cache4* c, const int32_t* src, const int32_t* dst, const int32_t* len,
+                        uint32_t n, int32_t* status, void* work, size_t work_bytes) {
+    return page_op(static_cast<cudaStream_t>(stream), OP_FORK, "cache4_fork", c, c, src, dst, len, n, status, work, work_bytes);
+}
+
+int pkb_cache4_copy_dev(void* stream, const pkb_cache4* to, const pkb_cache4* from, const int32_t* src,
+                        const int32_t* dst, const int32_t* len, uint32_t n, int32_t* status, void* work,
+                        size_t work_bytes) {
+    return page_op(static_cast<cudaStream_t>(stream), OP_COPY, "cache4_copy", to, from, src, dst, len, n, status, work, work_bytes);
+}
+
+int pkb_cache4_free_dev(void* stream, const pkb_cache4* c, const int32_t* seqs, uint32_t n, int32_t* status,
+                        void* work, size_t work_bytes) {
+    return page_op(static_cast<cudaStream_t>(stream), OP_FREE, "cache4_free", c, c, seqs, nullptr, nullptr, n, status, work, work_bytes);
+}
+
+int pkb_cache4_compact_dev(void* stream, const pkb_cache4* c, int32_t* used, int32_t* status, void* work,
+                           size_t work_bytes) {
+    const char* who = "cache4_compact";
+    Cache4 v;
+    PlanWork w;
+    int rc = check_plan(c, who, status, work, work_bytes, &v, &w), sms;
+    if (rc) return rc;
+    if (!is_aligned(used, 4)) return set_error(PKB_EINVAL, "%s: misaligned list", who);
+    uint32_t* err;
+    if ((rc = current_device_info(&sms, &err))) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = c4_launch(compact_plan_kernel, 1, PLAN_THREADS, 0, s, v, w, used, status);
+    if (e != cudaSuccess) return cuda_error(e, who);
+    count_launch();
+    e = c4_launch(compact_apply_kernel, static_cast<uint32_t>(8 * sms), 256, 0, s, v, w, err);
+    if (e != cudaSuccess) return cuda_error(e, who);
+    count_launch();
+    return PKB_OK;
+}
+
+int pkb_cache4_append_dev(void* stream, const pkb_cache4* c, uint32_t layer, const void* k, size_t ks, const void* v,
+                          size_t vs, int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows) {
+    return rows_call(static_cast<cudaStream_t>(stream), true, c, layer, const_cast<void*>(k), ks, const_cast<void*>(v), vs,
+                     type, seqs, starts, n, rows);
+}
+
+int pkb_cache4_read_dev(void* stream, const pkb_cache4* c, uint32_t layer, void* k, size_t ks, void* v, size_t vs,
+                        int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows) {
+    return rows_call(static_cast<cudaStream_t>(stream), false, c, layer, k, ks, v, vs, type, seqs, starts, n, rows);
+}
+
+}  // extern "C"

@@ -16,6 +16,9 @@ int set_error(int code, const char* fmt, ...);
 // and the device address of its error word.
 int current_device_info(int* sms, uint32_t** err_word);
 
+// SM clock cycles that a kernel's wait may last.
+long long wait_cycles();
+
 // One more kernel launched (pkb_launch_count).
 void count_launch();
 
@@ -148,6 +151,10 @@ cudaError_t launch_attention(const AttArgs& a, bool panels, int rmode, cudaStrea
 cudaError_t prepare_attention();
 // The dynamic shared memory an attention CTA may take (set by prepare_attention).
 size_t attention_smem_max();
+
+// The attention over a 4-bit cache's launch attributes (pkb_attn4.cu), once
+// a device at its set-up.
+cudaError_t prepare_attention4();
 
 // ------------------------------------------------ the TDT search (pkb_tdt.cu) --
 
