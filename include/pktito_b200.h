@@ -451,10 +451,9 @@ size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t
  * those with j <= p, and where `window` is not 0 to those with
  * j > p - window:
  *     o = sum_j softmax_j(scale q.k_j) v_j,
- * zeros where there is no such j. No sequence has more than max_rows rows
- * here (a hint: how the work is split depends on it, not what is computed).
- * Products are exact in the type of q (bf16, two or three bf16 parts for
- * f16 and f32), sums are float32, o is rounded once. Rows of o behind
+ * zeros where there is no such j. A sequence has at most max_rows rows (one
+ * that has more is out of range). Products are exact to the type of q, sums
+ * are float32, o is rounded once. Rows of o behind
  * starts[n] are left as they were; o must not overlap q. work as for the
  * page operations. What is out of range sets the device error word's bit
  * 1, and such rows of o are not defined. */

@@ -13,14 +13,16 @@
 // a pair (pkb_cache4.cuh); their order in the cache is that operand's, so
 // no value crosses a lane.
 //
-// The split. All (sequence, head, block of rows) items' tiles of 32 keys are
-// laid end to end and divided evenly over all warps of the GPU, whatever
-// the sequences' lengths: a warp's share begins and ends inside items. A warp
-// streams its tiles through a ring of its own in shared memory (bulk
-// copies of whole units, 18 dk bytes, completing on its mbarriers), so warps
-// never wait for one another. An item that one warp has whole is written
-// at once; of the others each warp leaves its part (m, l, O) in the work
-// area, and a second kernel joins an item's parts in a fixed order.
+// The split. A team of up to 16 cached heads' warps goes over the same
+// tiles of 32 keys side by side, each for its own head, so that what they
+// fetch lies together in a page. All (sequence, team, block of rows) items'
+// tiles are laid end to end and divided evenly over all teams of warps on the
+// GPU, whatever the sequences' lengths: a share begins and ends inside
+// items. One warp a block fetches for the others (bulk copies of whole
+// units, 18 dk bytes, into a ring of each warp's own), so warps never wait
+// for one another. An item that one share has whole is written at once; of
+// the others each share leaves its part (m, l, O) in the work area, and a
+// second kernel joins an item's parts in a fixed order.
 
 #include <climits>
 
@@ -32,77 +34,97 @@ namespace pkb {
 namespace {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
-constexpr int WARPS = 8;
+constexpr int JOIN_WARPS = 8;
 constexpr int TILE = 32;            // keys of a tile: two units
-constexpr uint32_t MAX_ENTRIES = 1024;  // sequences of one launch
-constexpr int MAX_GRID = 320;
-constexpr uint64_t MIN_TILES = 2;   // of a warp's share, where there are so many
+constexpr uint32_t MAX_ENTRIES = 512;  // sequences of one launch
+constexpr uint32_t MAX_TEAM = 16;
+constexpr uint32_t SPLIT_ROWS = 128;   // rows of an entry and cached head that are split along the keys; more are many
+constexpr int MAX_GRID = 160;
+constexpr int MAX_WORKERS = 15;
+// What it costs to begin and end an item, in tiles: shares are of equal
+// cost, not of equal tiles. An item is START places of no work, then its
+// tiles.
+constexpr uint32_t START = 2;
 
-template <int NB> __host__ __device__ constexpr int stages() { return NB <= 2 ? 4 : NB == 3 ? 3 : 2; }
+// Warps of a block that compute, beside one that fetches; one block an SM.
+// Fifteen leave a thread 128 registers, seven 255.
+template <int NB, int NT> __host__ __device__ constexpr int workers() { return NB * NT <= 4 ? 15 : 7; }
+template <int NB, int NT> __host__ __device__ constexpr int stages() { return workers<NB, NT>() == 15 ? (NB <= 2 ? 4 : 3) : NB == 8 ? 3 : 4; }
 template <int NB> __host__ __device__ constexpr int tile_bytes() { return 2 * 18 * 32 * NB; }
 template <int NB, int NT> __host__ __device__ constexpr int part_regs() { return NT * (NB * 8 + 4); }  // a lane's of one part
-template <int NB, int NT, int PARTS> constexpr int blocks_per_sm() { return NB * 8 * NT + NB * 4 * NT * PARTS <= 80 && NB <= 4 ? 2 : 1; }
 
-// One entry's shape: its rows, tokens, and the units its rows can see.
+// One entry's rows and tokens, and of what its rows can see the units and
+// the places (START and the tiles, 0 where nothing is seen).
 struct Entry {
-    uint32_t seq, r0, rows, len, unit0, units, tiles, blocks;
+    uint32_t seq, r0, rows, len;
+    __device__ __forceinline__ uint32_t unit0(const Attn4Args& a) const {
+        // the first row's window begins furthest back; the last row's causal end is len
+        const int64_t lo = a.window ? static_cast<int64_t>(len) - rows - a.window + 1 : 0;
+        return lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
+    }
+    __device__ __forceinline__ uint32_t units(const Attn4Args& a) const { return (len + C4_UNIT - 1) / C4_UNIT - unit0(a); }
+    __device__ __forceinline__ uint32_t places(const Attn4Args& a) const { return len ? START + (units(a) + 1) / 2 : 0; }
+    template <int NT>
+    __device__ __forceinline__ uint32_t blocks(const Attn4Args& a) const { return (rows * a.G + 8 * NT - 1) / (8 * NT); }
 };
 
-template <int NT>
 __device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
     Entry e;
     e.rows = c4_rows(a.c, a.seqs, a.starts, i, a.rows, &e.seq, &e.r0, a.err);
+    if (e.rows > a.max_rows) {
+        atomicOr(a.err, PKB_DEVERR_ARGS);
+        e.rows = 0;
+    }
     e.len = e.rows ? c4_len(a.c, e.seq, a.err) : 0;
-    // the first row's window begins furthest back; the last row's causal end is len
-    const int64_t lo = a.window ? static_cast<int64_t>(e.len) - e.rows - a.window + 1 : 0;
-    e.unit0 = lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
-    e.units = (e.len + C4_UNIT - 1) / C4_UNIT - e.unit0;
-    e.tiles = (e.units + 1) / 2;
-    e.blocks = static_cast<uint32_t>((static_cast<uint64_t>(e.rows) * a.G + 8 * NT - 1) / (8 * NT));
     return e;
 }
 
-// how many warps share `total` tiles, and where warp w's share begins
-__device__ __forceinline__ uint64_t shares(const Attn4Args& a, uint64_t total, uint64_t warps) {
-    const uint64_t most = (total + MIN_TILES - 1) / MIN_TILES, room = warps < a.max_shares ? warps : a.max_shares;
-    return most < room ? most : room;
-}
-__device__ __forceinline__ uint64_t share_begin(uint64_t w, uint64_t total, uint64_t n) { return w * total / n; }
+// `total` places over `n` shares, the first ones one more than the others.
+struct Split {
+    uint32_t n, each, more;
+    __device__ __forceinline__ Split(uint32_t total, uint32_t most) {
+        n = total < most ? total : most;
+        each = n ? total / n : 0;
+        more = n ? total - each * n : 0;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t s) const { return s * each + (s < more ? s : more); }
+    __device__ __forceinline__ uint32_t of(uint32_t x) const {
+        const uint32_t wide = more * (each + 1);
+        return x < wide ? x / (each + 1) : more + (x - wide) / each;
+    }
+};
 
-// A lane's two columns of each eight rows: where they end up and what they
-// may see.
-template <int NT>
-struct Columns {
-    int64_t row[2 * NT];  // of o, -1: none
-    uint32_t head[2 * NT];
-    int32_t lo[2 * NT], hi[2 * NT];  // keys [lo, hi)
+// A lane's columns are rows 8 j + 2 t + {0, 1} of a block of 8 NT: their
+// token in the entry, and what they may see. All of it is cheap to make
+// again, so none of it is held over the loop on the tiles.
+struct Column {
+    uint32_t r, tok;
+    bool valid;
+    int32_t lo, hi;  // keys [lo, hi)
 };
 
 template <int NT>
-__device__ __forceinline__ void load_columns(const Attn4Args& a, const Entry& e, uint32_t h, uint32_t block, Columns<NT>& col) {
-    const uint32_t t = threadIdx.x & 3;
-    const uint64_t all = static_cast<uint64_t>(e.rows) * a.G;
-#pragma unroll
-    for (int i = 0; i < 2 * NT; i++) {
-        const uint64_t r = static_cast<uint64_t>(block) * (8 * NT) + i / 2 * 8 + 2 * t + i % 2;
-        const uint64_t tok = r / a.G;
-        const int64_t pos = static_cast<int64_t>(e.len) - e.rows + static_cast<int64_t>(tok);
-        const int64_t hi = a.causal ? pos + 1 : e.len, lo = a.window ? pos - a.window + 1 : 0;
-        col.row[i] = r < all ? static_cast<int64_t>(e.r0 + tok) : -1;
-        col.head[i] = h * a.G + static_cast<uint32_t>(r % a.G);
-        col.hi[i] = r < all ? static_cast<int32_t>(hi < 0 ? 0 : hi > e.len ? e.len : hi) : 0;
-        col.lo[i] = static_cast<int32_t>(lo < 0 ? 0 : lo > INT_MAX ? INT_MAX : lo);
-    }
+__device__ __forceinline__ Column column(const Attn4Args& a, const Entry& e, uint32_t block, int i) {
+    Column c;
+    c.r = block * (8 * NT) + i / 2 * 8 + 2 * (threadIdx.x & 3) + i % 2;
+    c.tok = c.r / a.G;
+    c.valid = c.tok < e.rows;
+    const int64_t pos = static_cast<int64_t>(e.len) - e.rows + c.tok;
+    const int64_t hi = a.causal ? pos + 1 : e.len, lo = a.window ? pos - a.window + 1 : 0;
+    c.hi = c.valid ? static_cast<int32_t>(hi < 0 ? 0 : hi > e.len ? e.len : hi) : 0;
+    c.lo = static_cast<int32_t>(lo < 0 ? 0 : lo > INT_MAX ? INT_MAX : lo);
+    return c;
 }
 
 template <typename T, int NB, int NT>
-__device__ __forceinline__ void write_rows(const Attn4Args& a, const Columns<NT>& col, const float (&o)[2 * NB][NT][4],
-                                           const float (&l)[2 * NT]) {
+__device__ __forceinline__ void write_rows(const Attn4Args& a, const Entry& e, uint32_t h, uint32_t block,
+                                           const float (&o)[2 * NB][NT][4], const float (&l)[2 * NT]) {
     const uint32_t g = (threadIdx.x & 31) / 4;
 #pragma unroll
     for (int i = 0; i < 2 * NT; i++) {
-        if (col.row[i] < 0) continue;
-        T* out = static_cast<T*>(a.o) + col.row[i] * a.os + static_cast<size_t>(col.head[i]) * (NB * 32) + g;
+        const Column c = column<NT>(a, e, block, i);
+        if (!c.valid) continue;
+        T* out = static_cast<T*>(a.o) + static_cast<size_t>(e.r0 + c.tok) * a.os + (h * a.G + c.r - c.tok * a.G) * (NB * 32) + g;
         // a row that sees nothing has sum 0 and is zeros; a NaN sum gives NaNs
         const float inv = l[i] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[i]);
 #pragma unroll
@@ -144,87 +166,161 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
     }
 }
 
-// One tile of two units at `buf`: its scores, the softmax's step, its values.
-// MASK: some key of it is hidden from some row, or lies past the last token.
-template <int NB, int NT, int PARTS, bool MASK>
-__device__ __forceinline__ void tile_step(const uint8_t* buf, const uint32_t (&q)[NB][2][NT][PARTS][2], const Columns<NT>& col,
-                                          int32_t key0, int32_t len, float scale, float (&o)[2 * NB][NT][4], float (&m)[2 * NT],
-                                          float (&l)[2 * NT]) {
-    constexpr int DK = NB * 32;
+// A block's rows of q as the second operand of the products with K, which
+// are taken in f16: K's codes are whole numbers there (c4_whole), two thirds
+// of the instructions of scaled bf16 values, and their scales multiply the
+// sums of a block of 32. A row is brought to a largest value in [2^14, 2^15)
+// by a power of two, which its sums get back with the softmax's scale, and
+// is one f16 (bf16 and f16 rows) or two (float rows, PARTS 3): exact but for
+// 2^-24 of a float, and for 2^-39 of the row's largest value.
+template <int NB, int NT, int PARTS>
+struct Query {
+    static constexpr bool EXACT = PARTS == 3;
+    static constexpr int P = EXACT ? 2 : 1;
+    uint32_t w[NB][2][NT][P][2];
+    float bias[NB][2 * NT];  // unless EXACT: where the sums start, -8 and -72 times the elements
+    float scale[2 * NT];     // of each of the lane's columns
+};
+
+template <typename T, int NB, int NT, int PARTS>
+__device__ __forceinline__ void load_query(const Attn4Args& a, const Entry& e, uint32_t h, uint32_t block, Query<NB, NT, PARTS>& q) {
+    constexpr int P = Query<NB, NT, PARTS>::P;
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
-    float s[2][NT][4];
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        const uint8_t* unit = buf + u * 18 * DK;
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) s[u][j][x] = 0.0f;
-        uint32_t w[2][NB];
-        lds_words<NB>(unit + (g * 4 + t) * NB * 4, w[0]);
-        lds_words<NB>(unit + ((g + 8) * 4 + t) * NB * 4, w[1]);
+    for (int j = 0; j < NT; j++) {
+        const uint32_t r = block * (8 * NT) + j * 8 + g, tok = r / a.G;
+        const T* qp = static_cast<const T*>(a.q) + static_cast<size_t>(e.r0 + tok) * a.qs + (h * a.G + r - tok * a.G) * (NB * 32) + 8 * t;
+        float f[NB][8];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            uint32_t s2[2], ms[2];
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const uint32_t half = *reinterpret_cast<const uint16_t*>(unit + 16 * DK + ((g + 8 * r) * NB + b) * 2);
-                s2[r] = half | half << 16;
-                ms[r] = c4_m24(s2[r]);
+            for (int y = 0; y < 8; y++) f[b][y] = 0.0f;
+            if (tok < e.rows) {
+                if (a.vec) c4_load8<T, true>(qp + b * 32, f[b]);
+                else c4_load8<T, false>(qp + b * 32, f[b]);
             }
-            float fresh[NT][4];
-            if constexpr (PARTS == 3) {
+        }
+        float top = 0.0f;  // NaNs pass the maximum by and stay NaNs below
 #pragma unroll
-                for (int j = 0; j < NT; j++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int x = 0; x < 4; x++) fresh[j][x] = 0.0f;
+            for (int y = 0; y < 8; y++) top = fmaxf(top, fabsf(f[b][y]));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        // 2^(14 - x) for a largest value in [2^x, 2^(x+1)); an infinite one makes the row NaNs
+        const int x = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -110);
+        const float up = __uint_as_float(x == 128 ? 0x7FC00000u : static_cast<uint32_t>(141 - x) << 23);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                uint32_t parts[P];
+                f16_parts<P>(f[b][2 * y] * up, f[b][2 * y + 1] * up, parts);
+#pragma unroll
+                for (int z = 0; z < P; z++) q.w[b][y / 2][j][z][y % 2] = parts[z];
             }
+            if constexpr (!Query<NB, NT, PARTS>::EXACT) {
+                const uint32_t c[4] = {0xC800C800u, 0xC800C800u, 0xD480D480u, 0xD480D480u};  // -8, -72
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int step = 0; step < 2; step++) {
-                uint32_t a[4];
-                if (step == 0) {
-                    a[0] = c4_pair<0>(w[0][b], s2[0], ms[0]);
-                    a[1] = c4_pair<0>(w[1][b], s2[1], ms[1]);
-                    a[2] = c4_pair<1>(w[0][b], s2[0], ms[0]);
-                    a[3] = c4_pair<1>(w[1][b], s2[1], ms[1]);
-                } else {
-                    a[0] = c4_pair<2>(w[0][b], s2[0], ms[0]);
-                    a[1] = c4_pair<2>(w[1][b], s2[1], ms[1]);
-                    a[2] = c4_pair<3>(w[0][b], s2[0], ms[0]);
-                    a[3] = c4_pair<3>(w[1][b], s2[1], ms[1]);
-                }
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-#pragma unroll
-                    for (int p = PARTS - 1; p >= 0; p--)
-                        mma_bf16(PARTS == 3 ? fresh[j] : s[u][j], a, q[b][step][j][p][0], q[b][step][j][p][1]);
+                for (int step = 0; step < 2; step++) mma_f16(d, c, q.w[b][step][j][0][0], q.w[b][step][j][0][1]);
+                q.bias[b][2 * j] = d[0];
+                q.bias[b][2 * j + 1] = d[1];
             }
-            // the tensor cores cut what they add; for float rows each
-            // block's sum is added by a rounded addition instead
-            if constexpr (PARTS == 3) {
+        }
+        const float back = fminf(fmaxf(__fmul_rn(a.scale * 6.103515625e-5f, __uint_as_float(static_cast<uint32_t>(min(x, 127) + 127) << 23)),
+                                       -3.0e38f), 3.0e38f);  // scale 2^(x - 14)
+        q.scale[2 * j] = __shfl_sync(FULL, back, static_cast<int>(2 * t * 4));
+        q.scale[2 * j + 1] = __shfl_sync(FULL, back, static_cast<int>((2 * t + 1) * 4));
+    }
+}
+
+// Scores of one unit, before the scale: S^T[keys g, g + 8][columns 2t, 2t + 1].
+template <int NB, int NT, int PARTS>
+__device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB, NT, PARTS>& q, float (&s)[NT][4]) {
+    constexpr int DK = NB * 32, P = Query<NB, NT, PARTS>::P;
+    constexpr bool EXACT = Query<NB, NT, PARTS>::EXACT;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+    uint32_t w[2][NB];
+    lds_words<NB>(unit + (g * 4 + t) * NB * 4, w[0]);
+    lds_words<NB>(unit + ((g + 8) * 4 + t) * NB * 4, w[1]);
+    uint32_t sc[2][(NB + 1) / 2];
 #pragma unroll
-                for (int j = 0; j < NT; j++)
+    for (int r = 0; r < 2; r++) {
+        const uint8_t* at = unit + 16 * DK + (g + 8 * r) * NB * 2;
+        if constexpr (NB % 2 == 0) {
+            lds_words<NB / 2>(at, sc[r]);
+        } else {
 #pragma unroll
-                    for (int x = 0; x < 4; x++) s[u][j][x] = __fadd_rn(s[u][j][x], fresh[j][x]);
+            for (int b = 0; b < NB; b += 2) {
+                sc[r][b / 2] = *reinterpret_cast<const uint16_t*>(at + 2 * b);
+                if (b + 1 < NB) sc[r][b / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + 2 * b + 2)) << 16;
             }
         }
     }
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        float k[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) k[r] = __uint_as_float(b % 2 ? sc[r][b / 2] & 0xFFFF0000u : sc[r][b / 2] << 16);
+        const uint32_t a0[4] = {c4_whole<0, EXACT>(w[0][b]), c4_whole<0, EXACT>(w[1][b]), c4_whole<1, EXACT>(w[0][b]), c4_whole<1, EXACT>(w[1][b])};
+        const uint32_t a1[4] = {c4_whole<2, EXACT>(w[0][b]), c4_whole<2, EXACT>(w[1][b]), c4_whole<3, EXACT>(w[0][b]), c4_whole<3, EXACT>(w[1][b])};
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (!EXACT) d[0] = d[2] = q.bias[b][2 * j], d[1] = d[3] = q.bias[b][2 * j + 1];
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--) {
+                mma_f16(d, a0, q.w[b][0][j][p][0], q.w[b][0][j][p][1]);
+                mma_f16(d, a1, q.w[b][1][j][p][0], q.w[b][1][j][p][1]);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) s[j][x] = b ? __fmaf_rn(d[x], k[x / 2], s[j][x]) : __fmul_rn(d[x], k[x / 2]);
+        }
+    }
+}
+
+// One tile of two units at `buf`: its scores, the softmax's step, its values.
+// mask: some key of it is hidden from some row, or lies past the last one
+// that was fetched (limit).
+template <int NB, int NT, int PARTS>
+__device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, const Entry& e, uint32_t block, const uint8_t* buf,
+                                          const Query<NB, NT, PARTS>& q, int32_t key0, int32_t limit,
+                                          float (&o)[2 * NB][NT][4], float (&m)[2 * NT], float (&l)[2 * NT]) {
+    constexpr int DK = NB * 32;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+    float s[2][NT][4];
+    unit_scores<NB, NT, PARTS>(buf, q, s[0]);
+    unit_scores<NB, NT, PARTS>(buf + 18 * DK, q, s[1]);
     bool above = false;
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int i = 0; i < 2 * NT; i++) {
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                float y = __fmul_rn(s[u][j][x], scale);
-                const int i = 2 * j + (x & 1);
-                if constexpr (MASK) {
-                    const int32_t key = key0 + 16 * u + static_cast<int32_t>(g) + 8 * (x / 2);
-                    y = key >= col.lo[i] && key < col.hi[i] ? y : NEG_INF;
+            for (int r = 0; r < 2; r++) s[u][i / 2][i % 2 + 2 * r] = __fmul_rn(s[u][i / 2][i % 2 + 2 * r], q.scale[i]);
+    }
+    if (mask) {
+#pragma unroll
+        for (int i = 0; i < 2 * NT; i++) {
+            const Column c = column<NT>(args, e, block, i);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const int32_t key = key0 + 16 * u + static_cast<int32_t>(g) + 8 * r;
+                    if (key < c.lo || key >= c.hi) s[u][i / 2][i % 2 + 2 * r] = NEG_INF;
                 }
-                above |= y > m[i] + 8.0f;
-                s[u][j][x] = y;
-            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NT; i++) {
+        const float limit = m[i] + 8.0f;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) above |= s[u][i / 2][i % 2 + 2 * r] > limit;
+    }
     // The maximum is raised only where some score passes it by 8: sums and
     // weights then stay below 2^8 times the keys, far inside a float, and
     // most tiles need one vote instead of the reductions.
@@ -279,10 +375,10 @@ __device__ __forceinline__ void tile_step(const uint8_t* buf, const uint32_t (&q
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 s2[c] = *reinterpret_cast<const uint32_t*>(unit + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
-                if constexpr (MASK) {  // scales past the last token may be anything, and 0 times a NaN is one
+                if (mask) {  // scales past the limit may be anything, and 0 times a NaN is one
                     const int32_t key = key0 + 16 * u + 8 * c + 2 * static_cast<int32_t>(t);
-                    if (key >= len) s2[c] = 0;
-                    else if (key + 1 >= len) s2[c] &= 0xFFFFu;
+                    if (key >= limit) s2[c] = 0;
+                    else if (key + 1 >= limit) s2[c] &= 0xFFFFu;
                 }
                 ms[c] = c4_m24(s2[c]);
             }
@@ -313,333 +409,455 @@ __device__ __forceinline__ void tile_step(const uint8_t* buf, const uint32_t (&q
 }
 
 template <typename T, int NB, int NT, int PARTS>
-__global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NB, NT, PARTS>()) split_kernel(Attn4Args a) {
-    constexpr int DK = NB * 32, STAGES = stages<NB>(), BYTES = tile_bytes<NB>();
+__global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(Attn4Args a) {
+    constexpr int DK = NB * 32, WORKERS = workers<NB, NT>(), THREADS = (WORKERS + 1) * 32, STAGES = stages<NB, NT>(), BYTES = tile_bytes<NB>();
+    constexpr int EACH = (MAX_ENTRIES + THREADS - 1) / THREADS;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bars[WARPS][STAGES];
-    __shared__ uint64_t sums[WARPS];
+    __shared__ uint64_t full[WORKERS][STAGES], empty[WORKERS][STAGES];
+    __shared__ uint32_t sums[WORKERS + 1];
     __shared__ volatile int gave_up;
-    uint64_t* base = reinterpret_cast<uint64_t*>(smem + WARPS * STAGES * BYTES);
+    Entry* entries = reinterpret_cast<Entry*>(smem + WORKERS * STAGES * BYTES);
+    uint32_t* base = reinterpret_cast<uint32_t*>(entries + a.n);  // each entry's first place
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
-    if (lane == 0) {
-        for (int i = 0; i < STAGES; i++) mbar_init(&bars[warp][i], 1);
+    if (lane == 0 && warp < WORKERS) {
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(&full[warp][i], 1);
+            mbar_init(&empty[warp][i], 1);
+        }
         fence_mbar_init();
     }
     if (tid == 0) gave_up = 0;
     pdl_trigger();
     pdl_wait();
-    // each entry's first tile: four entries a thread, a scan over the block
-    uint64_t mine[MAX_ENTRIES / (WARPS * 32)], own = 0;
+    uint32_t own = 0;
 #pragma unroll
-    for (int x = 0; x < static_cast<int>(MAX_ENTRIES / (WARPS * 32)); x++) {
-        const uint32_t i = tid * (MAX_ENTRIES / (WARPS * 32)) + x;
-        mine[x] = own;
+    for (int x = 0; x < EACH; x++) {
+        const uint32_t i = tid * EACH + x;
         if (i < a.n) {
-            const Entry e = load_entry<NT>(a, i);
-            own += static_cast<uint64_t>(e.tiles) * a.c.heads * e.blocks;
+            const Entry e = load_entry(a, i);
+            entries[i] = e;
+            base[i] = own;
+            own += e.places(a) * a.teams * e.blocks<NT>(a);
         }
     }
-    uint64_t scan = own;
+    uint32_t scan = own;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const uint64_t y = __shfl_up_sync(FULL, scan, d);
+        const uint32_t y = __shfl_up_sync(FULL, scan, d);
         if (lane >= static_cast<uint32_t>(d)) scan += y;
     }
     if (lane == 31) sums[warp] = scan;
     __syncthreads();
-    uint64_t total = 0;
-    for (uint32_t w = 0; w < WARPS; w++) {
+    uint32_t total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w <= WORKERS; w++) {
         if (w == warp) scan += total - own;
         total += sums[w];
     }
 #pragma unroll
-    for (int x = 0; x < static_cast<int>(MAX_ENTRIES / (WARPS * 32)); x++) {
-        const uint32_t i = tid * (MAX_ENTRIES / (WARPS * 32)) + x;
-        if (i < a.n) {
-            base[i] = scan + mine[x];
-            if (blockIdx.x == 0) a.base[i] = scan + mine[x];
-        }
+    for (int x = 0; x < EACH; x++) {
+        const uint32_t i = tid * EACH + x;
+        if (i < a.n) base[i] += scan;
     }
-    if (tid == 0) {
-        base[a.n] = total;
-        if (blockIdx.x == 0) a.base[a.n] = total;
-    }
+    if (tid == 0) base[a.n] = total;
     __syncthreads();
-    // entries that see no tokens: rows of zeros
-    for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-        if (base[i + 1] != base[i]) continue;
-        const Entry e = load_entry<NT>(a, i);
-        const uint32_t width = a.H * DK;
-        for (uint64_t x = tid; x < static_cast<uint64_t>(e.rows) * width; x += WARPS * 32)
-            static_cast<T*>(a.o)[(e.r0 + x / width) * a.os + x % width] = c4_round<T>(0.0f);
-    }
-    // warps side by side in a share's order lie on different SMs
-    const uint64_t w = static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x;
-    const uint64_t n_shares = shares(a, total, static_cast<uint64_t>(gridDim.x) * WARPS);
-    if (w >= n_shares) return;
-    const uint64_t begin = share_begin(w, total, n_shares), end = share_begin(w + 1, total, n_shares);
-    uint8_t* ring = smem + warp * STAGES * BYTES;
-
-    // where a tile lies: its entry, and its item within it
-    auto entry_at = [&](uint64_t x) {
+    const Split split(total, min(gridDim.x * WORKERS / a.team, a.max_shares));
+    // where a place lies: its entry, its item of that, and its place in the item
+    struct Item {
+        uint32_t entry, head0, block, place, places;
+    };
+    auto item_at = [&](uint32_t x) {
+        Item it;
         uint32_t lo = 0, hi = a.n;
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
             if (base[mid] <= x) lo = mid; else hi = mid;
         }
-        return lo;
+        it.entry = lo;
+        const Entry& e = entries[lo];
+        it.places = e.places(a);
+        const uint32_t at = x - base[lo], i = at / it.places, blocks = e.blocks<NT>(a), t = i / blocks;
+        it.place = at - i * it.places;
+        it.block = i - t * blocks;
+        it.head0 = t * a.team;
+        return it;
     };
-    // the producer's place: lanes 0 and 1 fetch a tile's two units
-    uint64_t px = begin;
-    Entry pe = {};
-    uint32_t pi = 0, ptile = 0, ph = 0;
-    uint64_t pitem = 0;
-    auto p_enter = [&](uint64_t x) {
-        pi = entry_at(x);
-        pe = load_entry<NT>(a, pi);
-        pitem = (x - base[pi]) / pe.tiles;
-        ptile = static_cast<uint32_t>((x - base[pi]) % pe.tiles);
-        ph = static_cast<uint32_t>(pitem / pe.blocks);
-    };
-    const uint8_t* src = nullptr;
-    uint32_t fetch = 0;  // units of the next tile
-    auto p_look = [&]() {
-        if (px >= end) return;
-        const uint32_t u = 2 * ptile;
-        fetch = pe.units - u < 2 ? 1 : 2;
-        src = nullptr;
-        if (lane < fetch) {
-            src = c4_unit(a.c, a.layer, pe.seq, ph, pe.unit0 + u + lane, a.err);
-            // a table entry that is no page: any page will do, the rows are not defined
-            if (!src) src = a.c.pages;
-        }
-    };
-    auto p_issue = [&](int stage) {
-        if (px >= end) return;
-        if (lane == 0) mbar_arrive_expect_tx(&bars[warp][stage], fetch * 18 * DK);
-        __syncwarp();
-        if (lane < fetch) bulk_load(ring + stage * BYTES + lane * 18 * DK, src, 18 * DK, &bars[warp][stage]);
-        px++;
-        if (px < end) {
-            if (++ptile == pe.tiles) {
-                ptile = 0;
-                if (++pitem == static_cast<uint64_t>(a.c.heads) * pe.blocks) p_enter(px);
-                else ph = static_cast<uint32_t>(pitem / pe.blocks);
-            }
-            p_look();
-        }
-    };
-    p_enter(px);
-    p_look();
-#pragma unroll
-    for (int i = 0; i < STAGES; i++) p_issue(i);
 
+    if (warp == WORKERS) {
+        // the producer: lanes 2 w and 2 w + 1 fetch the units of worker w's tiles
+        const uint32_t mate = lane & 1, to = lane / 2, v = to * gridDim.x + blockIdx.x;
+        const uint32_t share = v / a.team, member = v - share * a.team;
+        const bool mine = to < WORKERS && share < split.n;
+        uint32_t x = mine ? split.begin(share) : 0;
+        const uint32_t end = mine ? split.begin(share + 1) : 0;
+        uint64_t* bars = full[mine ? to : 0];
+        uint8_t* ring = smem + ((mine ? to : 0) * STAGES * 2 + mate) * 18 * DK;
+        uint32_t left = 0, unit = 0, stop = 0;  // tiles of the item that are left in the share; this lane's next unit, and the item's end
+        const uint8_t* head = nullptr;          // the head's first unit in page 0
+        const int32_t* row = nullptr;           // the sequence's table
+        int32_t page = 0;                       // of this lane's next unit, asked for a tile ahead
+        const uint32_t per = a.c.pshift - 4;
+        // the first tile from place x on
+        auto enter = [&]() {
+            while (x < end) {
+                const Item it = item_at(x);
+                const Entry e = entries[it.entry];
+                const uint32_t skip = it.place < START ? START - it.place : 0, here = min(it.places - it.place, end - x);
+                x += here;
+                if (here <= skip || it.head0 + member >= a.c.heads) continue;
+                left = here - skip;
+                unit = e.unit0(a) + 2 * (it.place + skip - START) + mate;
+                stop = e.unit0(a) + e.units(a);
+                row = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
+                head = a.c.pages + a.layer * a.c.layer_bytes + (it.head0 + member) * a.c.head_bytes;
+                break;
+            }
+            if (left && unit < stop) page = row[unit >> per];
+        };
+        enter();
+        int stage = 0;
+        uint32_t phase = 0, issued = 0;
+        long long since = clock64();
+        while (__any_sync(FULL, left)) {
+            bool go = left && mbar_test_wait(&empty[to][stage], phase ^ 1);
+            go = __shfl_sync(FULL, go, static_cast<int>(lane & ~1u));
+            const bool has = unit < stop, both = __shfl_down_sync(FULL, has, 1);
+            if (go && !mate) mbar_arrive_expect_tx(&bars[stage], (both ? 2 : 1) * 18 * DK);
+            __syncwarp();
+            if (go) {
+                if (has) {
+                    if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
+                        atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
+                        page = 0;
+                    }
+                    bulk_load(ring + stage * BYTES, head + static_cast<uint32_t>(page) * a.c.page_bytes + (unit & ((1u << per) - 1)) * (18 * DK),
+                              18 * DK, &bars[stage]);
+                }
+                issued++;
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+                if (--left) {
+                    unit += 2;
+                    if (unit < stop) page = row[unit >> per];
+                } else {
+                    enter();
+                }
+            }
+            if (__any_sync(FULL, go)) since = clock64();
+            else if (gave_up || clock64() - since > a.timeout) break;
+            else __nanosleep(64);  // the rings are full
+        }
+        if (left) {
+            gave_up = 1;
+            atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+        }
+        // whatever the workers did, the copies in flight land before the block leaves its memory
+        for (int i = 0; i < STAGES && i < static_cast<int>(issued); i++) {
+            if (--stage < 0) stage = STAGES - 1, phase ^= 1;
+            mbar_drain(&bars[stage], phase, a.timeout);
+        }
+        return;
+    }
+
+    // a team's warps lie on neighbouring SMs, and so do shares
+    const uint32_t v = warp * gridDim.x + blockIdx.x, share = v / a.team, member = v - share * a.team;
+    const uint8_t* ring = smem + warp * STAGES * BYTES;
     int stage = 0;
     uint32_t phase = 0;
-    uint64_t x = begin;
-    Entry e = {};
-    uint32_t entry = FULL;
-    while (x < end) {
-        // one item, or the part of it in this share
-        if (entry == FULL || x >= base[entry + 1]) {
-            entry = entry_at(x);
-            e = load_entry<NT>(a, entry);
-        }
-        const uint64_t item = (x - base[entry]) / e.tiles;
-        const uint32_t first = static_cast<uint32_t>((x - base[entry]) % e.tiles);
-        const uint32_t last = static_cast<uint32_t>(end - x < e.tiles - first ? first + (end - x) : e.tiles);
-        const uint32_t h = static_cast<uint32_t>(item / e.blocks), block = static_cast<uint32_t>(item % e.blocks);
-        Columns<NT> col;
-        load_columns<NT>(a, e, h, block, col);
-        uint32_t q[NB][2][NT][PARTS][2];
-        {
-            const uint32_t g = lane / 4, t = lane & 3;
-            const uint64_t all = static_cast<uint64_t>(e.rows) * a.G;
+    if (share < split.n) {
+        uint32_t x = split.begin(share);
+        const uint32_t end = split.begin(share + 1);
+        while (x < end) {
+            // one item, or the part of it in this share
+            const Item it = item_at(x);
+            const uint32_t x0 = x - it.place, here = min(it.places - it.place, end - x), stop = it.place + here;
+            x += here;
+            const uint32_t h = it.head0 + member;
+            if (stop <= START || h >= a.c.heads) continue;
+            const Entry e = entries[it.entry];
+            const uint32_t first = it.place < START ? 0 : it.place - START, block = it.block;
+            Query<NB, NT, PARTS> q;
+            load_query<T, NB, NT, PARTS>(a, e, h, block, q);
+            int32_t all_lo = 0, all_hi = INT_MAX;  // the keys that every row of the block sees
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const uint64_t r = static_cast<uint64_t>(block) * (8 * NT) + j * 8 + g;
-                const T* qp = static_cast<const T*>(a.q) + (e.r0 + r / a.G) * a.qs + (static_cast<size_t>(h) * a.G + r % a.G) * DK + 8 * t;
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    float f[8];
-#pragma unroll
-                    for (int y = 0; y < 8; y++) f[y] = r < all ? c4_float<T>(qp[b * 32 + y]) : 0.0f;
-#pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        uint32_t parts[PARTS];
-                        bf16_parts<PARTS>(f[2 * y], f[2 * y + 1], parts);
-#pragma unroll
-                        for (int z = 0; z < PARTS; z++) q[b][y / 2][j][z][y % 2] = parts[z];
-                    }
+            for (int i = 0; i < 2 * NT; i++) {
+                const Column c = column<NT>(a, e, block, i);
+                if (c.valid) {
+                    all_lo = max(all_lo, c.lo);
+                    all_hi = min(all_hi, c.hi);
                 }
             }
-        }
-        // the keys that every row of the block sees
-        int32_t all_lo = 0, all_hi = INT_MAX;
-#pragma unroll
-        for (int i = 0; i < 2 * NT; i++)
-            if (col.row[i] >= 0) {
-                all_lo = max(all_lo, col.lo[i]);
-                all_hi = min(all_hi, col.hi[i]);
-            }
-        all_lo = __reduce_max_sync(FULL, all_lo);
-        all_hi = __reduce_min_sync(FULL, all_hi);
-        float o[2 * NB][NT][4], m[2 * NT], l[2 * NT];
-#pragma unroll
-        for (int d = 0; d < 2 * NB; d++)
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-#pragma unroll
-                for (int y = 0; y < 4; y++) o[d][j][y] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
-        for (uint32_t tile = first; tile < last; tile++) {
-            if (!mbar_wait(&bars[warp][stage], phase, &gave_up, a.timeout)) {
-                // a copy that does not come: say so, let those in flight land, leave
-                gave_up = 1;
-                if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
-                for (int i = 0; i < STAGES && x + i < px; i++) {
-                    mbar_drain(&bars[warp][stage], phase, a.timeout);
-                    if (++stage == STAGES) stage = 0, phase ^= 1;
-                }
-                return;
-            }
-            const uint8_t* buf = ring + stage * BYTES;
-            const int32_t key0 = static_cast<int32_t>((e.unit0 + 2 * tile) * C4_UNIT);
-            // warp-uniform: tiles at the window's start, the causal edge and the last token
-            if (key0 < all_lo || static_cast<int64_t>(key0) + TILE > all_hi)
-                tile_step<NB, NT, PARTS, true>(buf, q, col, key0, static_cast<int32_t>(e.len), a.scale, o, m, l);
-            else
-                tile_step<NB, NT, PARTS, false>(buf, q, col, key0, static_cast<int32_t>(e.len), a.scale, o, m, l);
-            __syncwarp();
-            p_issue(stage);
-            x++;
-            if (++stage == STAGES) stage = 0, phase ^= 1;
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * NT; i++) l[i] = column_sum(l[i]);
-        if (first == 0 && last == e.tiles) {
-            write_rows<T, NB, NT>(a, col, o, l);
-        } else {
-            float* part = a.part + ((2 * w + (first == 0)) * part_regs<NB, NT>()) * 32 + lane;
+            all_lo = __reduce_max_sync(FULL, all_lo);
+            all_hi = __reduce_min_sync(FULL, all_hi);
+            float o[2 * NB][NT][4], m[2 * NT], l[2 * NT];
 #pragma unroll
             for (int d = 0; d < 2 * NB; d++)
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
-                    for (int y = 0; y < 4; y++) part[((d * NT + j) * 4 + y) * 32] = o[d][j][y];
+                    for (int y = 0; y < 4; y++) o[d][j][y] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2 * NT; i++) {
-                part[(NB * 8 * NT + i) * 32] = m[i];
-                part[(NB * 8 * NT + 2 * NT + i) * 32] = l[i];
+            for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
+            int32_t key0 = static_cast<int32_t>((e.unit0(a) + 2 * first) * C4_UNIT);
+            for (uint32_t left = stop - START - first; left; left--) {
+                if (!mbar_wait(&full[warp][stage], phase, &gave_up, a.timeout)) {
+                    gave_up = 1;  // the producer lets what is in flight land
+                    if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                    return;
+                }
+                const uint8_t* buf = ring + stage * BYTES;
+                // warp-uniform: tiles at the window's start, the causal edge and the last token
+                const bool mask = key0 < all_lo || static_cast<int64_t>(key0) + TILE > all_hi;
+                tile_step<NB, NT, PARTS>(mask, a, e, block, buf, q, key0, static_cast<int32_t>(e.len), o, m, l);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[warp][stage]);
+                key0 += TILE;
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * NT; i++) l[i] = column_sum(l[i]);
+            const bool whole = first == 0 && stop == it.places;
+            if (whole) {
+                write_rows<T, NB, NT>(a, e, h, block, o, l);
+            } else {
+                float4* part = reinterpret_cast<float4*>(a.part) + static_cast<size_t>(2 * v + (first == 0)) * (part_regs<NB, NT>() / 4) * 32 + lane;
+#pragma unroll
+                for (int d = 0; d < 2 * NB; d++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) part[(d * NT + j) * 32] = make_float4(o[d][j][0], o[d][j][1], o[d][j][2], o[d][j][3]);
+#pragma unroll
+                for (int j = 0; j < NT; j++) part[(NB * 2 * NT + j) * 32] = make_float4(m[2 * j], m[2 * j + 1], l[2 * j], l[2 * j + 1]);
+            }
+            // the share with an item's last tile says which shares have parts of it
+            if (stop == it.places && lane == 0) {
+                const uint32_t team = it.head0 / a.team;
+                a.joins[((static_cast<size_t>(it.entry) * a.teams + team) * a.max_blocks + block) * a.team + member] =
+                    Attn4Join{whole ? Attn4Join::NONE : split.of(x0 + START), share};
             }
         }
+    }
+    // entries that see no tokens: rows of zeros, and nothing to join
+    for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+        if (base[i + 1] != base[i]) continue;
+        const Entry e = entries[i];
+        for (uint32_t x = tid; x < a.teams * a.max_blocks * a.team; x += WORKERS * 32)
+            a.joins[static_cast<size_t>(i) * a.teams * a.max_blocks * a.team + x].first = Attn4Join::NONE;
+        const uint32_t width = a.H * DK;
+        for (uint64_t x = tid; x < static_cast<uint64_t>(e.rows) * width; x += WORKERS * 32)
+            static_cast<T*>(a.o)[(e.r0 + x / width) * a.os + x % width] = c4_round<T>(0.0f);
     }
 }
 
-// Joins the parts of the items that several shares have: one block an item,
-// its warps take the parts in turn, then each other's, in the same order
-// always.
+// Joins the parts of the items that several shares have. A warp takes 16
+// dimensions of eight rows (a float4 a lane) over every `ways`-th of an
+// item's parts; `ways` warps then join theirs, always in the same order. Many
+// items have few parts each and take one way, a few long ones take up to
+// eight, so that no warp reads many parts one after another.
 template <typename T, int NB, int NT>
-__global__ void __launch_bounds__(WARPS * 32) join_kernel(Attn4Args a, uint64_t warps) {
-    constexpr int REGS = NB * 8 * NT;
-    __shared__ float sm[WARPS][4 * NT][32];
-    extern __shared__ float so[];  // [WARPS][REGS][32]
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint32_t ways) {
+    constexpr int QUADS = 2 * NB * NT, STRIDE = part_regs<NB, NT>() / 4;  // float4s of a lane: [dims 16][eight rows], then m and l
+    __shared__ float4 sm[2][JOIN_WARPS][32];
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const uint32_t i = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
-    const uint64_t total = a.base[a.n], first = a.base[i];
-    if (a.base[i + 1] == first) return;
-    const uint64_t n_shares = shares(a, total, warps);
-    const Entry e = load_entry<NT>(a, i);
-    for (uint32_t block = blockIdx.y; block < e.blocks; block += gridDim.y) {
-        const uint64_t x0 = first + (static_cast<uint64_t>(h) * e.blocks + block) * e.tiles, x1 = x0 + e.tiles - 1;
-        const uint64_t w0 = ((x0 + 1) * n_shares - 1) / total, w1 = ((x1 + 1) * n_shares - 1) / total;
-        if (w0 == w1) continue;  // one share has it whole and wrote it
-        float o[REGS], m[2 * NT], l[2 * NT];
-#pragma unroll
-        for (int r = 0; r < REGS; r++) o[r] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 2 * NT; c++) m[c] = NEG_INF, l[c] = 0.0f;
-        for (uint64_t w = w0 + warp; w <= w1; w += WARPS) {
-            const float* part = a.part + ((2 * w + (w == w0)) * part_regs<NB, NT>()) * 32 + lane;
-            float f[2 * NT], k[2 * NT];
-#pragma unroll
-            for (int c = 0; c < 2 * NT; c++) {
-                const float pm = part[(REGS + c) * 32], pl = part[(REGS + 2 * NT + c) * 32];
-                const float top = fmaxf(m[c], pm);
-                k[c] = rescale(m[c], top);
-                f[c] = rescale(pm, top);
-                m[c] = top;
-                l[c] = l[c] * k[c] + pl * f[c];
-            }
-#pragma unroll
-            for (int r = 0; r < REGS; r++) {
-                const int c = 2 * (r / 4 % NT) + r % 2;
-                o[r] = o[r] * k[c] + part[r * 32] * f[c];
-            }
+    // the item: [entry][team][block][member]
+    const uint32_t member = blockIdx.x % a.team, block = blockIdx.x / a.team % a.max_blocks, it = blockIdx.x / a.team / a.max_blocks;
+    const uint32_t entry = it / a.teams, h = it % a.teams * a.team + member;
+    if (h >= a.c.heads) return;
+    const Entry e = load_entry(a, entry);
+    if (block >= e.blocks<NT>(a)) return;
+    const Attn4Join item = a.joins[blockIdx.x];
+    if (item.first == Attn4Join::NONE) return;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, warp = threadIdx.x / 32, way = warp % ways;
+    const uint32_t z = blockIdx.y * (JOIN_WARPS / ways) + warp / ways;
+    const uint32_t d = z / NT, j = z % NT;
+    float m0 = NEG_INF, m1 = NEG_INF, l0 = 0.0f, l1 = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (z < QUADS) {
+        const float4* part = reinterpret_cast<const float4*>(a.part) + lane;
+        auto at = [&](uint32_t s, uint32_t r) {
+            return part[(static_cast<size_t>(2 * (s * a.team + member) + (s == item.first)) * STRIDE + r) * 32];
+        };
+#pragma unroll 8
+        for (uint32_t s = item.first + way; s <= item.last; s += ways) {
+            const float4 v = at(s, QUADS + j);
+            m0 = fmaxf(m0, v.x);
+            m1 = fmaxf(m1, v.y);
         }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 2 * NT; c++) sm[warp][c][lane] = m[c], sm[warp][2 * NT + c][lane] = l[c];
-#pragma unroll
-        for (int r = 0; r < REGS; r++) so[(warp * REGS + r) * 32 + lane] = o[r];
-        __syncthreads();
-        // the rows' weights of each warp's sum, then REGS / WARPS of a row's values a warp
-        float f[WARPS][2 * NT];
-#pragma unroll
-        for (int c = 0; c < 2 * NT; c++) {
-            float top = NEG_INF;
-#pragma unroll
-            for (int w = 0; w < WARPS; w++) top = fmaxf(top, sm[w][c][lane]);
-            l[c] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WARPS; w++) {
-                f[w][c] = rescale(sm[w][c][lane], top);
-                l[c] += sm[w][2 * NT + c][lane] * f[w][c];
-            }
-        }
-        Columns<NT> col;
-        load_columns<NT>(a, e, h, block, col);
-        const uint32_t g = lane / 4;
-#pragma unroll
-        for (int z = 0; z < REGS / WARPS; z++) {
-            // registers of a lane: [dims 16][columns][row g, g + 8][two columns]
-            const int r = z * WARPS + static_cast<int>(warp);
-            float sum = 0.0f;
-            const int j = r / 4 % NT, c = 2 * j + r % 2;
-            float lc = 0.0f;
-            int64_t row = -1;
-            uint32_t head = 0;
-#pragma unroll
-            for (int y = 0; y < 2 * NT; y++)
-                if (y == c) {
-                    lc = l[y], row = col.row[y], head = col.head[y];
-#pragma unroll
-                    for (int w = 0; w < WARPS; w++) sum += so[(w * REGS + r) * 32 + lane] * f[w][y];
-                }
-            if (row < 0) continue;
-            const float inv = lc == 0.0f ? 0.0f : __fdiv_rn(1.0f, lc);
-            static_cast<T*>(a.o)[row * a.os + static_cast<size_t>(head) * (NB * 32) + r / (4 * NT) * 16 + r % 4 / 2 * 8 + g] =
-                c4_round<T>(__fmul_rn(sum, inv));
+#pragma unroll 8
+        for (uint32_t s = item.first + way; s <= item.last; s += ways) {
+            const float4 v = at(s, QUADS + j), x = at(s, z);
+            const float f0 = rescale(v.x, m0), f1 = rescale(v.y, m1);
+            l0 = __fmaf_rn(v.z, f0, l0);
+            l1 = __fmaf_rn(v.w, f1, l1);
+            o[0] = __fmaf_rn(x.x, f0, o[0]);
+            o[1] = __fmaf_rn(x.y, f1, o[1]);
+            o[2] = __fmaf_rn(x.z, f0, o[2]);
+            o[3] = __fmaf_rn(x.w, f1, o[3]);
         }
     }
+    if (ways > 1) {
+        sm[0][warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+        sm[1][warp][lane] = make_float4(m0, m1, l0, l1);
+        __syncthreads();
+        if (way) return;
+        for (uint32_t w = 1; w < ways; w++) {
+            const float4 v = sm[1][warp + w][lane], x = sm[0][warp + w][lane];
+            const float t0 = fmaxf(m0, v.x), t1 = fmaxf(m1, v.y);
+            const float k0 = rescale(m0, t0), k1 = rescale(m1, t1), f0 = rescale(v.x, t0), f1 = rescale(v.y, t1);
+            m0 = t0, m1 = t1;
+            l0 = l0 * k0 + v.z * f0;
+            l1 = l1 * k1 + v.w * f1;
+            o[0] = o[0] * k0 + x.x * f0;
+            o[1] = o[1] * k1 + x.y * f1;
+            o[2] = o[2] * k0 + x.z * f0;
+            o[3] = o[3] * k1 + x.w * f1;
+        }
+    }
+    if (z >= QUADS) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const Column c = column<NT>(a, e, block, 2 * j + i);
+        if (!c.valid) continue;
+        const float l = i ? l1 : l0, inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        T* out = static_cast<T*>(a.o) + static_cast<size_t>(e.r0 + c.tok) * a.os + (h * a.G + c.r - c.tok * a.G) * (NB * 32) + d * 16 + g;
+        out[0] = c4_round<T>(__fmul_rn(o[i], inv));
+        out[8] = c4_round<T>(__fmul_rn(o[2 + i], inv));
+    }
+}
+
+// ---------------------------------------------------------- many rows --
+//
+// Prompts and long chunks: a block takes ROW_WARPS blocks of rows of one
+// entry and head, a warp each, and its warps read the same tiles from one
+// ring, so that a tile is fetched once for 64 or 128 rows. Nothing is split
+// along the keys. A warp leaves out the tiles that its own rows cannot see.
+// Bound by mma.sync's rate: 2 (bf16), 3 (f16) or 5 (float rows) products of
+// 16 keys and 8 rows a 16 values.
+
+constexpr int ROW_WARPS = 8;
+constexpr int ROW_STAGES = 8;
+
+template <typename T, int NB, int NT, int PARTS>
+__global__ void __launch_bounds__((ROW_WARPS + 1) * 32, 1) rows_kernel(Attn4Args a) {
+    constexpr int DK = NB * 32, BYTES = tile_bytes<NB>();
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t full[ROW_STAGES], empty[ROW_STAGES];
+    __shared__ volatile int gave_up;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    if (tid == 0) {
+        for (int i = 0; i < ROW_STAGES; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], ROW_WARPS);
+        }
+        fence_mbar_init();
+        gave_up = 0;
+    }
+    pdl_trigger();
+    pdl_wait();
+    __syncthreads();
+    const uint32_t h = blockIdx.y;
+    const Entry e = load_entry(a, blockIdx.z);
+    // the last rows, which see most, begin first
+    const uint32_t groups = (e.blocks<NT>(a) + ROW_WARPS - 1) / ROW_WARPS;
+    if (blockIdx.x >= groups) return;
+    const uint32_t group = groups - 1 - blockIdx.x, block = group * ROW_WARPS + warp;
+    // the units that the block's rows can see
+    const uint32_t tok0 = group * ROW_WARPS * 8 * NT / a.G, tok1 = min((group + 1) * ROW_WARPS * 8 * NT - 1, e.rows * a.G - 1) / a.G;
+    const int64_t pos0 = static_cast<int64_t>(e.len) - e.rows + tok0, pos1 = static_cast<int64_t>(e.len) - e.rows + tok1;
+    const int64_t lo = a.window && pos0 - a.window + 1 > 0 ? pos0 - a.window + 1 : 0;
+    const int64_t hi = a.causal ? (pos1 + 1 < e.len ? pos1 + 1 : e.len) : e.len;
+    const uint32_t unit0 = static_cast<uint32_t>(lo / C4_UNIT);
+    const uint32_t units = hi > lo ? static_cast<uint32_t>((hi + C4_UNIT - 1) / C4_UNIT) - unit0 : 0, tiles = (units + 1) / 2;
+
+    if (warp == ROW_WARPS) {
+        const uint32_t per = a.c.pshift - 4;
+        const int32_t* row = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
+        const uint8_t* head = a.c.pages + a.layer * a.c.layer_bytes + h * a.c.head_bytes;
+        int32_t page = lane < 2 && lane < units ? row[(unit0 + lane) >> per] : 0;
+        uint32_t issued = 0;
+        for (uint32_t i = 0; i < tiles; i++, issued++) {
+            const int stage = i % ROW_STAGES;
+            if (!mbar_wait(&empty[stage], (i / ROW_STAGES & 1) ^ 1, &gave_up, a.timeout)) {
+                gave_up = 1;
+                if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                break;
+            }
+            const uint32_t unit = unit0 + 2 * i + lane;
+            if (lane == 0) mbar_arrive_expect_tx(&full[stage], (units - 2 * i < 2 ? 1 : 2) * 18 * DK);
+            __syncwarp();
+            if (lane < 2 && 2 * i + lane < units) {
+                if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
+                    atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
+                    page = 0;
+                }
+                bulk_load(smem + stage * BYTES + lane * 18 * DK, head + static_cast<uint32_t>(page) * a.c.page_bytes + (unit & ((1u << per) - 1)) * (18 * DK),
+                          18 * DK, &full[stage]);
+                if (2 * i + 2 + lane < units) page = row[(unit + 2) >> per];
+            }
+        }
+        // whatever the others did, the copies in flight land before the block leaves its memory
+        for (uint32_t i = issued < ROW_STAGES ? 0 : issued - ROW_STAGES; i < issued; i++)
+            mbar_drain(&full[i % ROW_STAGES], i / ROW_STAGES & 1, a.timeout);
+        return;
+    }
+
+    Query<NB, NT, PARTS> q;
+    load_query<T, NB, NT, PARTS>(a, e, h, block, q);
+    int32_t all_lo = 0, all_hi = INT_MAX, any_lo = INT_MAX, any_hi = 0;  // the keys that every row, and that any row of the warp sees
+#pragma unroll
+    for (int i = 0; i < 2 * NT; i++) {
+        const Column c = column<NT>(a, e, block, i);
+        if (c.valid) {
+            all_lo = max(all_lo, c.lo);
+            all_hi = min(all_hi, c.hi);
+            any_lo = min(any_lo, c.lo);
+            any_hi = max(any_hi, c.hi);
+        }
+    }
+    all_lo = __reduce_max_sync(FULL, all_lo);
+    all_hi = __reduce_min_sync(FULL, all_hi);
+    any_lo = __reduce_min_sync(FULL, any_lo);
+    any_hi = __reduce_max_sync(FULL, any_hi);
+    float o[2 * NB][NT][4], m[2 * NT], l[2 * NT];
+#pragma unroll
+    for (int d = 0; d < 2 * NB; d++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) o[d][j][y] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
+    int32_t key0 = static_cast<int32_t>(unit0 * C4_UNIT);
+    for (uint32_t i = 0; i < tiles; i++, key0 += TILE) {
+        const int stage = i % ROW_STAGES;
+        if (!mbar_wait(&full[stage], i / ROW_STAGES & 1, &gave_up, a.timeout)) {
+            gave_up = 1;  // the producer lets what is in flight land
+            if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+            return;
+        }
+        if (key0 < any_hi && static_cast<int64_t>(key0) + TILE > any_lo) {
+            const bool mask = key0 < all_lo || static_cast<int64_t>(key0) + TILE > all_hi;
+            tile_step<NB, NT, PARTS>(mask, a, e, block, smem + stage * BYTES, q, key0, static_cast<int32_t>(hi), o, m, l);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NT; i++) l[i] = column_sum(l[i]);
+    write_rows<T, NB, NT>(a, e, h, block, o, l);
 }
 
 // ------------------------------------------------------------------- host --
 
-template <int NB> size_t split_smem(uint32_t n) { return WARPS * stages<NB>() * tile_bytes<NB>() + (static_cast<size_t>(n) + 1) * 8; }
-template <int NB, int NT> size_t join_smem() { return static_cast<size_t>(WARPS) * NB * 8 * NT * 32 * 4; }
+template <int NB, int NT> size_t split_smem(uint32_t n) {
+    return workers<NB, NT>() * stages<NB, NT>() * tile_bytes<NB>() + static_cast<size_t>(n) * (sizeof(Entry) + 4) + 4;
+}
 
 template <typename T, int NB, int NT, int PARTS>
 cudaError_t prepare_one() {
-    cudaError_t e = cudaFuncSetAttribute(split_kernel<T, NB, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(split_smem<NB>(MAX_ENTRIES)));
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(join_kernel<T, NB, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(join_smem<NB, NT>()));
-    return e;
+    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, NB, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               ROW_STAGES * tile_bytes<NB>());
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(split_kernel<T, NB, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(split_smem<NB, NT>(MAX_ENTRIES)));
 }
 
 template <typename T, int PARTS>
@@ -653,45 +871,72 @@ cudaError_t prepare_type() {
 }
 
 template <typename T, int NB, int NT, int PARTS>
-cudaError_t launch_one(const Attn4Args& a, uint32_t max_rows, int sms, cudaStream_t s) {
-    const uint32_t grid = static_cast<uint32_t>(blocks_per_sm<NB, NT, PARTS>() * sms < MAX_GRID ? blocks_per_sm<NB, NT, PARTS>() * sms : MAX_GRID);
-    cudaError_t e = c4_launch(split_kernel<T, NB, NT, PARTS>, grid, WARPS * 32, split_smem<NB>(a.n), s, a);
+cudaError_t launch_one(Attn4Args a, int sms, cudaStream_t s) {
+    if (a.max_rows * a.G > SPLIT_ROWS) {
+        const uint32_t most = ROW_WARPS * 8 * NT;
+        const dim3 grid((a.max_rows * a.G + most - 1) / most, a.c.heads, a.n);
+        const cudaError_t e = c4_launch(rows_kernel<T, NB, NT, PARTS>, grid, (ROW_WARPS + 1) * 32, ROW_STAGES * tile_bytes<NB>(), s, a);
+        if (e == cudaSuccess) count_launch();
+        return e;
+    }
+    const uint32_t grid = static_cast<uint32_t>(sms < MAX_GRID ? sms : MAX_GRID);
+    a.max_blocks = (a.max_rows * a.G + 8 * NT - 1) / (8 * NT);
+    cudaError_t e = c4_launch(split_kernel<T, NB, NT, PARTS>, grid, (workers<NB, NT>() + 1) * 32, split_smem<NB, NT>(a.n), s, a);
     if (e != cudaSuccess) return e;
     count_launch();
-    const uint64_t blocks = (static_cast<uint64_t>(max_rows) * a.G + 8 * NT - 1) / (8 * NT);
-    const dim3 jgrid(a.n * a.c.heads, static_cast<uint32_t>(blocks < 1 ? 1 : blocks > 65535 ? 65535 : blocks));
-    e = c4_launch(join_kernel<T, NB, NT>, jgrid, WARPS * 32, join_smem<NB, NT>(), s, a, static_cast<uint64_t>(grid) * WARPS);
+    // parts an item has about, if all have as many: more than four go two ways and so on
+    const uint64_t items = static_cast<uint64_t>(a.n) * a.teams * a.max_blocks, most = grid * workers<NB, NT>() / a.team;
+    const uint64_t shares = most < a.max_shares ? most : a.max_shares;
+    uint32_t ways = 1;
+    while (ways < 8 && shares > 4 * ways * items) ways *= 2;
+    const uint32_t quads = JOIN_WARPS / ways;
+    e = c4_launch(join_kernel<T, NB, NT>, dim3(static_cast<uint32_t>(items * a.team), (2 * NB * NT + quads - 1) / quads), JOIN_WARPS * 32, 0, s, a, ways);
     if (e == cudaSuccess) count_launch();
     return e;
 }
 
 template <typename T, int PARTS>
-cudaError_t launch_type(const Attn4Args& a, uint32_t max_rows, int sms, cudaStream_t s) {
-    const bool two = static_cast<uint64_t>(max_rows) * a.G > 8;  // more than eight rows: two blocks of eight share the codes' conversion
+cudaError_t launch_type(const Attn4Args& a, int sms, cudaStream_t s) {
+    const bool two = static_cast<uint64_t>(a.max_rows) * a.G > 8;  // more than eight rows: two blocks of eight share the codes' conversion
     switch (a.c.dk) {
-        case 32: return two ? launch_one<T, 1, 2, PARTS>(a, max_rows, sms, s) : launch_one<T, 1, 1, PARTS>(a, max_rows, sms, s);
-        case 64: return two ? launch_one<T, 2, 2, PARTS>(a, max_rows, sms, s) : launch_one<T, 2, 1, PARTS>(a, max_rows, sms, s);
-        case 96: return two ? launch_one<T, 3, 2, PARTS>(a, max_rows, sms, s) : launch_one<T, 3, 1, PARTS>(a, max_rows, sms, s);
-        case 128: return two ? launch_one<T, 4, 2, PARTS>(a, max_rows, sms, s) : launch_one<T, 4, 1, PARTS>(a, max_rows, sms, s);
-        default: return launch_one<T, 8, 1, PARTS>(a, max_rows, sms, s);
+        case 32: return two ? launch_one<T, 1, 2, PARTS>(a, sms, s) : launch_one<T, 1, 1, PARTS>(a, sms, s);
+        case 64: return two ? launch_one<T, 2, 2, PARTS>(a, sms, s) : launch_one<T, 2, 1, PARTS>(a, sms, s);
+        case 96: return two ? launch_one<T, 3, 2, PARTS>(a, sms, s) : launch_one<T, 3, 1, PARTS>(a, sms, s);
+        case 128: return two ? launch_one<T, 4, 2, PARTS>(a, sms, s) : launch_one<T, 4, 1, PARTS>(a, sms, s);
+        default: return launch_one<T, 8, 1, PARTS>(a, sms, s);
     }
 }
 
-constexpr size_t BASE_BYTES = (MAX_ENTRIES + 32) * 8;
-
 bool is_aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// The shares that a call can have at most, and the bytes of their parts.
-uint64_t most_shares(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
-    const uint64_t tiles = static_cast<uint64_t>(c->max_pages) * c->page_tokens / TILE + 1;
-    const uint64_t blocks = n + static_cast<uint64_t>(rows) * (H / c->n_heads) / 8;
-    const uint64_t most = static_cast<uint64_t>(MAX_GRID) * WARPS;
-    return blocks >= most || blocks * c->n_heads * tiles >= most ? most : blocks * c->n_heads * tiles;
+// Cached heads as teams of at most MAX_TEAM, of one size but for the last.
+void teams_of(uint32_t heads, uint32_t* team, uint32_t* teams) {
+    *teams = (heads + MAX_TEAM - 1) / MAX_TEAM;
+    *team = (heads + *teams - 1) / *teams;
 }
 
-size_t work_bytes_for(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
-    const uint64_t nt = c->head_dim == 256 ? 1 : 2;
-    return BASE_BYTES + 2 * most_shares(c, H, rows, n) * nt * (c->head_dim / 4 + 4) * 128;
+// A call's bounds, over any lengths that the cache's table has room for: the
+// entries of a launch, its shares, and the bytes of the work area: a join an
+// item (an entry, head and eight rows), two parts a share and head. Only
+// entries of up to SPLIT_ROWS rows are split.
+struct Bounds {
+    uint64_t entries, shares, join_bytes, bytes;
+};
+
+Bounds bounds_of(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
+    uint32_t team, teams;
+    teams_of(c->n_heads, &team, &teams);
+    const uint64_t G = H / c->n_heads, tiles = static_cast<uint64_t>(c->max_pages) * c->page_tokens / TILE + 1 + START;
+    const uint64_t blocks = rows * G < SPLIT_ROWS ? (rows * G + 7) / 8 : SPLIT_ROWS / 8;
+    Bounds b;
+    b.entries = n < MAX_ENTRIES ? n : MAX_ENTRIES;
+    // places are counted in 32 bits
+    if (b.entries > INT_MAX / (teams * tiles * blocks)) b.entries = INT_MAX / (teams * tiles * blocks);
+    const uint64_t most = static_cast<uint64_t>(MAX_GRID) * MAX_WORKERS / team, places = b.entries * teams * tiles * blocks;
+    b.shares = places < most ? places : most;
+    b.join_bytes = (b.entries * teams * team * blocks * sizeof(Attn4Join) + 255) & ~static_cast<uint64_t>(255);
+    b.bytes = b.join_bytes + 2 * b.shares * team * (c->head_dim == 256 ? 1 : 2) * (c->head_dim / 4 + 4) * 128;
+    return b;
 }
 
 }  // namespace
@@ -711,7 +956,7 @@ extern "C" {
 
 size_t pkb_attention_cache4_work_bytes(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
     if (!c || !pkb_cache4_page_bytes(c->page_tokens, c->n_heads, c->head_dim) || !H || H % c->n_heads) return 0;
-    return work_bytes_for(c, H, rows, n);
+    return rows && n ? bounds_of(c, H, rows, n).bytes : 0;
 }
 
 int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, size_t qs, int type, uint32_t H,
@@ -731,7 +976,7 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     if (!o || !q || !seqs || !starts || !work) return set_error(PKB_EINVAL, "%s: null pointer", who);
     if (!max_rows || max_rows > rows) return set_error(PKB_EINVAL, "%s: max_rows = %u of %u rows", who, max_rows, rows);
     const size_t width = static_cast<size_t>(H) * c->head_dim, size = c4_type_bytes(type);
-    if (width > UINT_MAX / 2 || rows > INT_MAX) return set_error(PKB_EINVAL, "%s: %u rows of %zu values", who, rows, width);
+    if (width > UINT_MAX / 2 || rows > INT_MAX || static_cast<uint64_t>(rows) * (H / c->n_heads) > INT_MAX) return set_error(PKB_EINVAL, "%s: %u rows of %zu values", who, rows, width);
     if (rows > 1 && (qs < width || os < width)) return set_error(PKB_EINVAL, "%s: a row stride below %zu values", who, width);
     if (rows == 1) qs = os = width;
     if (!is_aligned(o, size) || !is_aligned(q, size) || !is_aligned(seqs, 4) || !is_aligned(starts, 4))
@@ -739,10 +984,11 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), q1 = q0 + ((rows - 1) * qs + width) * size;
     const uintptr_t o0 = reinterpret_cast<uintptr_t>(o), o1 = o0 + ((rows - 1) * os + width) * size;
     if (o0 < q1 && q0 < o1) return set_error(PKB_EINVAL, "%s: o overlaps q", who);
-    const size_t need = work_bytes_for(c, H, rows, n);
-    if (work_bytes < need || !is_aligned(work, 256))
-        return set_error(PKB_EINVAL, "%s: work area of %zu bytes (%zu needed, 256-byte aligned)", who, work_bytes, need);
-    if (static_cast<uint64_t>(MAX_ENTRIES) * c->n_heads > INT_MAX) return set_error(PKB_EINVAL, "%s: %u heads", who, c->n_heads);
+    const Bounds bounds = bounds_of(c, H, rows, n);
+    if (work_bytes < bounds.bytes || !is_aligned(work, 256))
+        return set_error(PKB_EINVAL, "%s: work area of %zu bytes (%zu needed, 256-byte aligned)", who, work_bytes, static_cast<size_t>(bounds.bytes));
+    if (!bounds.entries || (static_cast<uint64_t>(max_rows) * (H / c->n_heads) > SPLIT_ROWS && c->n_heads > 65535))
+        return set_error(PKB_EINVAL, "%s: %u heads of sequences of up to %u pages are too many", who, c->n_heads, c->max_pages);
     int sms;
     if ((rc = current_device_info(&sms, &a.err))) return rc;
     a.q = q;
@@ -753,21 +999,25 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     a.rows = rows;
     a.H = H;
     a.G = H / c->n_heads;
+    a.vec = is_aligned(q, 16) && qs * size % 16 == 0;
     a.scale = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074);  // log2 e
     a.causal = causal ? 1 : 0;
     a.window = window;
     a.timeout = wait_cycles();
-    a.base = static_cast<uint64_t*>(work);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + BASE_BYTES);
-    a.max_shares = most_shares(c, H, rows, n);
+    a.max_rows = max_rows;
+    teams_of(c->n_heads, &a.team, &a.teams);
+    a.joins = static_cast<Attn4Join*>(work);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + bounds.join_bytes);
+    a.max_shares = static_cast<uint32_t>(bounds.shares);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    for (uint32_t i = 0; i < n; i += MAX_ENTRIES) {
+    const uint32_t step = static_cast<uint32_t>(bounds.entries);
+    for (uint32_t i = 0; i < n; i += step) {
         a.seqs = seqs + i;
         a.starts = starts + i;
-        a.n = n - i < MAX_ENTRIES ? n - i : MAX_ENTRIES;
-        const cudaError_t e = type == PKB_F32   ? launch_type<float, 3>(a, max_rows, sms, s)
-                              : type == PKB_F16 ? launch_type<__half, 2>(a, max_rows, sms, s)
-                                                : launch_type<__nv_bfloat16, 1>(a, max_rows, sms, s);
+        a.n = n - i < step ? n - i : step;
+        const cudaError_t e = type == PKB_F32   ? launch_type<float, 3>(a, sms, s)
+                              : type == PKB_F16 ? launch_type<__half, 2>(a, sms, s)
+                                                : launch_type<__nv_bfloat16, 1>(a, sms, s);
         if (e != cudaSuccess)
             return set_error(e == cudaErrorMemoryAllocation ? PKB_ENOMEM : PKB_ECUDA, "%s launch: %s", who, cudaGetErrorString(e));
     }

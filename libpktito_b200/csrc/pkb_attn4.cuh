@@ -7,6 +7,13 @@
 
 namespace pkb {
 
+// The parts of an item that shares first .. last have; NONE for an item that
+// one share has whole, or that sees no tokens.
+struct Attn4Join {
+    uint32_t first, last;
+    static constexpr uint32_t NONE = 0xFFFFFFFFu;
+};
+
 struct Attn4Args {
     Cache4 c;
     const void* q;
@@ -15,16 +22,25 @@ struct Attn4Args {
     const int32_t *seqs, *starts;
     uint32_t* err;
     uint32_t layer, n, rows, H, G;  // G: query heads a cached head
+    uint32_t max_rows, max_blocks;  // of an entry: rows, and blocks of rows
+    uint32_t team, teams;           // cached heads that go together, and how many times that (`team` times `teams` covers them)
     float scale;                    // times log2 e
     uint32_t causal, window;
+    uint32_t vec;                   // q's rows are 16-byte aligned
     long long timeout;
-    uint64_t* base;  // [n + 1] each entry's first tile
-    float* part;     // partial results, two a share
-    uint64_t max_shares;  // that the work area has room for
+    Attn4Join* joins;               // of each item: [n][teams][max_blocks][team]
+    float* part;                    // partial results, two a share and head of its team
+    uint32_t max_shares;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -55,6 +71,39 @@ __device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t (&r)[PAR
             hi = __fsub_rn(hi, __uint_as_float(r[i] & 0xFFFF0000u));
         }
     }
+}
+
+// x as PARTS f16 numbers that add up to it: to 11 and to 23 bits.
+template <int PARTS>
+__device__ __forceinline__ void f16_parts(float lo, float hi, uint32_t (&r)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        r[i] = *reinterpret_cast<const uint32_t*>(&h);
+        if (i + 1 < PARTS) {
+            lo = __fsub_rn(lo, __low2float(h));
+            hi = __fsub_rn(hi, __high2float(h));
+        }
+    }
+}
+
+// The codes of a word as f16 pairs of small whole numbers, without the
+// scale: the nibbles in place in the mantissa of 1024 (pairs 0 and 2) and of
+// 64 (pairs 1 and 3), so that a word takes one shift and four ANDs. EXACT:
+// c itself; else n (c + 8) of pairs 0 and 2 and 64 + n of 1 and 3, where the
+// accumulator starts at what that adds to the sum.
+template <int J, bool EXACT>
+__device__ __forceinline__ uint32_t c4_whole(uint32_t w) {
+    const uint32_t at = J < 2 ? w : w >> 8;
+    uint32_t r;
+    if constexpr (J % 2 == 0) {
+        asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r) : "r"(at));
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(EXACT ? 0xE408E408u : 0xE400E400u));  // -1032, -1024
+    } else {
+        asm("lop3.b32 %0, %1, 0x00F000F0, 0x54005400, 0xEA;" : "=r"(r) : "r"(at));
+        if constexpr (EXACT) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xD480D480u));  // -72
+    }
+    return r;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
