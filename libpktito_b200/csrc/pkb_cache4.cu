@@ -69,7 +69,7 @@ __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, u
     if (!rows) return u;
     const uint32_t len = c4_len(a.c, seq, a.err);
     if (rows > len) {
-        if ((threadIdx.x & 31) == 0) atomicOr(a.err, 2u);
+        if ((threadIdx.x & 31) == 0) atomicOr(a.err, PKB_DEVERR_ARGS);
         return u;
     }
     const uint32_t pos0 = len - rows, at = r0 / C4_UNIT + 2 * i, unit = pos0 / C4_UNIT + (slot - at);
@@ -337,7 +337,20 @@ __device__ __forceinline__ void load_refs(const Cache4& c, uint32_t p0, int32_t 
     }
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
+// free's part for entry i: its pages lose a user, its row is emptied.
+__device__ __forceinline__ void free_place(const PlanArgs& p, uint32_t i, uint32_t j, uint32_t* err) {
+    int32_t* at = p.c.table + static_cast<size_t>(p.a[i]) * p.c.max_pages + j;
+    const int32_t page = *at;
+    if (page >= 0) {
+        if (static_cast<uint32_t>(page) < p.c.n_pages) atomicSub(p.c.refs + page, 1);
+        else atomicOr(err, PKB_DEVERR_ARGS);
+        *at = -1;
+    }
+    if (j == 0) p.c.lens[p.a[i]] = 0;
+}
+
+// alone: free, all of it in this block
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p, bool alone, uint32_t* err) {
     __shared__ uint32_t buf[32];
     __shared__ uint64_t wide[32];
     __shared__ int worst;
@@ -390,6 +403,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
         p.w.count[0] = status ? 0 : total;
     }
     if (status) return;
+    if (p.op == OP_FREE) {
+        for (uint32_t x = tid; alone && x < p.n * p.c.max_pages; x += PLAN_THREADS) free_place(p, x / p.c.max_pages, x % p.c.max_pages, err);
+        return;
+    }
     __syncthreads();
     for (uint32_t j = tid; j < total; j += PLAN_THREADS) {
         const uint32_t i = entry_of(p.w.first, p.n, j), k = j - p.w.first[i], page = p.w.page[j];
@@ -421,7 +438,7 @@ __device__ void copy_pages(const Cache4& c, const Cache4& src, const PlanWork& w
         const uint64_t j = x / chunks / c.n_layers;
         const uint32_t from = w.from[j], to = w.to[j];
         if (from >= src.n_pages || to >= c.n_pages) {
-            if (threadIdx.x == 0) atomicOr(err, 2u);
+            if (threadIdx.x == 0) atomicOr(err, PKB_DEVERR_ARGS);
             continue;
         }
         const size_t at = static_cast<size_t>(chunk) * COPY_CHUNK;
@@ -445,15 +462,7 @@ __global__ void __launch_bounds__(256) apply_kernel(PlanArgs p, uint32_t* err) {
     if (*p.status) return;
     for (uint32_t i = blockIdx.x; i < p.n; i += gridDim.x) {
         if (p.op == OP_FREE) {
-            const size_t row = static_cast<size_t>(p.a[i]) * p.c.max_pages;
-            for (uint32_t j = threadIdx.x; j < p.c.max_pages; j += 256) {
-                const int32_t page = p.c.table[row + j];
-                if (page < 0) continue;
-                if (static_cast<uint32_t>(page) < p.c.n_pages) atomicSub(p.c.refs + page, 1);
-                else atomicOr(err, 2u);
-                p.c.table[row + j] = -1;
-            }
-            if (threadIdx.x == 0) p.c.lens[p.a[i]] = 0;
+            for (uint32_t j = threadIdx.x; j < p.c.max_pages; j += 256) free_place(p, i, j, err);
             continue;
         }
         if (p.op == OP_FORK) {
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(256) apply_kernel(PlanArgs p, uint32_t* err) {
                 const int32_t page = p.c.table[from + j];
                 p.c.table[to + j] = page;
                 if (page >= 0 && static_cast<uint32_t>(page) < p.c.n_pages) atomicAdd(p.c.refs + page, 1);
-                else atomicOr(err, 2u);
+                else atomicOr(err, PKB_DEVERR_ARGS);
             }
         }
         if (threadIdx.x == 0) p.c.lens[p.b[i]] = p.num[i];
@@ -606,10 +615,12 @@ int page_op(cudaStream_t stream, int op, const char* who, const pkb_cache4* c, c
     p.n = n;
     p.op = op;
     p.status = status;
-    cudaError_t e = c4_launch(plan_kernel, 1, PLAN_THREADS, 0, stream, p);
+    // a few rows' pages are freed by the block that checked them: a second launch takes as long as some 16,000 places
+    const bool alone = op == OP_FREE && static_cast<uint64_t>(n) * c->max_pages <= 16384;
+    cudaError_t e = c4_launch(plan_kernel, 1, PLAN_THREADS, 0, stream, p, alone, err);
     if (e != cudaSuccess) return cuda_error(e, who);
     count_launch();
-    if (op == OP_GROW || !n) return PKB_OK;
+    if (op == OP_GROW || alone || !n) return PKB_OK;
     // a block an entry, or enough blocks that a copy keeps every SM's loads in flight
     const uint64_t most = op == OP_FREE ? n : n + static_cast<uint64_t>(op == OP_FORK ? n : c->n_pages) * c->n_layers *
                                                       ((p.c.page_bytes + COPY_CHUNK - 1) / COPY_CHUNK);
