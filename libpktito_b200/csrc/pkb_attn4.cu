@@ -41,10 +41,6 @@ constexpr uint32_t MAX_TEAM = 16;
 constexpr uint32_t SPLIT_ROWS = 128;   // rows of an entry and cached head that are split along the keys; more are many
 constexpr int MAX_GRID = 160;
 constexpr int MAX_WORKERS = 15;
-// What it costs to begin and end an item, in tiles: shares are of equal
-// cost, not of equal tiles. An item is START places of no work, then its
-// tiles.
-constexpr uint32_t START = 2;
 
 // Warps of a block that compute, beside one that fetches; one block an SM.
 // Fifteen leave a thread 128 registers, seven 255.
@@ -52,32 +48,6 @@ template <int NB, int NT> __host__ __device__ constexpr int workers() { return N
 template <int NB, int NT> __host__ __device__ constexpr int stages() { return workers<NB, NT>() == 15 ? (NB <= 2 ? 4 : 3) : NB == 8 ? 3 : 4; }
 template <int NB> __host__ __device__ constexpr int tile_bytes() { return 2 * 18 * 32 * NB; }
 template <int NB, int NT> __host__ __device__ constexpr int part_regs() { return NT * (NB * 8 + 4); }  // a lane's of one part
-
-// One entry's rows and tokens, and of what its rows can see the units and
-// the places (START and the tiles, 0 where nothing is seen).
-struct Entry {
-    uint32_t seq, r0, rows, len;
-    __device__ __forceinline__ uint32_t unit0(const Attn4Args& a) const {
-        // the first row's window begins furthest back; the last row's causal end is len
-        const int64_t lo = a.window ? static_cast<int64_t>(len) - rows - a.window + 1 : 0;
-        return lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
-    }
-    __device__ __forceinline__ uint32_t units(const Attn4Args& a) const { return (len + C4_UNIT - 1) / C4_UNIT - unit0(a); }
-    __device__ __forceinline__ uint32_t places(const Attn4Args& a) const { return len ? START + (units(a) + 1) / 2 : 0; }
-    template <int NT>
-    __device__ __forceinline__ uint32_t blocks(const Attn4Args& a) const { return (rows * a.G + 8 * NT - 1) / (8 * NT); }
-};
-
-__device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
-    Entry e;
-    e.rows = c4_rows(a.c, a.seqs, a.starts, i, a.rows, &e.seq, &e.r0, a.err);
-    if (e.rows > a.max_rows) {
-        atomicOr(a.err, PKB_DEVERR_ARGS);
-        e.rows = 0;
-    }
-    e.len = e.rows ? c4_len(a.c, e.seq, a.err) : 0;
-    return e;
-}
 
 // `total` places over `n` shares, the first ones one more than the others.
 struct Split {
@@ -599,7 +569,7 @@ __global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(
             for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
             int32_t key0 = static_cast<int32_t>((e.unit0(a) + 2 * first) * C4_UNIT);
             for (uint32_t left = stop - START - first; left; left--) {
-                if (!mbar_wait(&full[warp][stage], phase, &gave_up, a.timeout)) {
+                if (!warp_wait(&full[warp][stage], phase, &gave_up, a.timeout)) {
                     gave_up = 1;  // the producer lets what is in flight land
                     if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
                     return;
@@ -790,7 +760,7 @@ __global__ void __launch_bounds__((ROW_WARPS + 1) * 32, 1) rows_kernel(Attn4Args
         uint32_t issued = 0;
         for (uint32_t i = 0; i < tiles; i++, issued++) {
             const int stage = i % ROW_STAGES;
-            if (!mbar_wait(&empty[stage], (i / ROW_STAGES & 1) ^ 1, &gave_up, a.timeout)) {
+            if (!warp_wait(&empty[stage], (i / ROW_STAGES & 1) ^ 1, &gave_up, a.timeout)) {
                 gave_up = 1;
                 if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
                 break;
@@ -843,7 +813,7 @@ __global__ void __launch_bounds__((ROW_WARPS + 1) * 32, 1) rows_kernel(Attn4Args
     int32_t key0 = static_cast<int32_t>(unit0 * C4_UNIT);
     for (uint32_t i = 0; i < tiles; i++, key0 += TILE) {
         const int stage = i % ROW_STAGES;
-        if (!mbar_wait(&full[stage], i / ROW_STAGES & 1, &gave_up, a.timeout)) {
+        if (!warp_wait(&full[stage], i / ROW_STAGES & 1, &gave_up, a.timeout)) {
             gave_up = 1;  // the producer lets what is in flight land
             if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
             return;
@@ -960,6 +930,7 @@ cudaError_t prepare_attention4() {
     cudaError_t e = prepare_type<float, 3>();
     if (e == cudaSuccess) e = prepare_type<__half, 2>();
     if (e == cudaSuccess) e = prepare_type<__nv_bfloat16, 1>();
+    if (e == cudaSuccess) e = prepare_attention4_tc();
     return e;
 }
 
@@ -1015,6 +986,7 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     a.H = H;
     a.G = H / c->n_heads;
     a.vec = is_aligned(q, 16) && qs * size % 16 == 0;
+    a.vec_o = is_aligned(o, 16) && os * size % 16 == 0;
     a.scale = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074);  // log2 e
     a.causal = causal ? 1 : 0;
     a.window = window;
@@ -1030,7 +1002,9 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
         a.seqs = seqs + i;
         a.starts = starts + i;
         a.n = n - i < step ? n - i : step;
-        const cudaError_t e = type == PKB_F32   ? launch_type<float, 3>(a, sms, s)
+        const bool many = a.max_rows * a.G > SPLIT_ROWS;
+        const cudaError_t e = many && attention4_tc_takes(a, type) ? launch_attention4_tc(a, s)
+                              : type == PKB_F32   ? launch_type<float, 3>(a, sms, s)
                               : type == PKB_F16 ? launch_type<__half, 2>(a, sms, s)
                                                 : launch_type<__nv_bfloat16, 1>(a, sms, s);
         if (e != cudaSuccess)

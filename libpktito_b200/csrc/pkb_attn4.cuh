@@ -26,7 +26,7 @@ struct Attn4Args {
     uint32_t team, teams;           // cached heads that go together, and how many times that (`team` times `teams` covers them)
     float scale;                    // times log2 e
     uint32_t causal, window;
-    uint32_t vec;                   // q's rows are 16-byte aligned
+    uint32_t vec, vec_o;            // q's and o's rows are 16-byte aligned
     long long timeout;
     Attn4Join* joins;               // of each item: [n][teams][max_blocks][team]
     float* part;                    // partial results, two a share and head of its team
@@ -112,9 +112,51 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
+// A warp's wait: every lane gives up if one does.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, long long limit) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort, limit));
+}
+
 constexpr float NEG_INF = -__builtin_huge_valf();
 
 // e^x / e^m for partial sums: 1 where both are -inf (nothing seen yet)
 __device__ __forceinline__ float rescale(float from, float to) { return from == to ? 1.0f : exp2_fast(__fsub_rn(from, to)); }
+
+// What it costs to begin and end an item, in tiles: shares are of equal
+// cost, not of equal tiles. An item is START places of no work, then its
+// tiles.
+constexpr uint32_t START = 2;
+
+// One entry's rows and tokens, and of what its rows can see the units and
+// the places (START and the tiles, 0 where nothing is seen).
+struct Entry {
+    uint32_t seq, r0, rows, len;
+    __device__ __forceinline__ uint32_t unit0(const Attn4Args& a) const {
+        // the first row's window begins furthest back; the last row's causal end is len
+        const int64_t lo = a.window ? static_cast<int64_t>(len) - rows - a.window + 1 : 0;
+        return lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
+    }
+    __device__ __forceinline__ uint32_t units(const Attn4Args& a) const { return (len + C4_UNIT - 1) / C4_UNIT - unit0(a); }
+    __device__ __forceinline__ uint32_t places(const Attn4Args& a) const { return len ? START + (units(a) + 1) / 2 : 0; }
+    template <int NT>
+    __device__ __forceinline__ uint32_t blocks(const Attn4Args& a) const { return (rows * a.G + 8 * NT - 1) / (8 * NT); }
+};
+
+__device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
+    Entry e;
+    e.rows = c4_rows(a.c, a.seqs, a.starts, i, a.rows, &e.seq, &e.r0, a.err);
+    if (e.rows > a.max_rows) {
+        atomicOr(a.err, PKB_DEVERR_ARGS);
+        e.rows = 0;
+    }
+    e.len = e.rows ? c4_len(a.c, e.seq, a.err) : 0;
+    return e;
+}
+
+// Many bf16 rows on the fifth-generation tensor cores (pkb_attn4_tc.cu): whether
+// it takes a call, its set-up, and its launch.
+bool attention4_tc_takes(const Attn4Args& a, int type);
+cudaError_t prepare_attention4_tc();
+cudaError_t launch_attention4_tc(const Attn4Args& a, cudaStream_t stream);
 
 }  // namespace pkb

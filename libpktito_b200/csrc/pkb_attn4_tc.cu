@@ -1,0 +1,489 @@
+// Attention over a cache held in 4 bits, many bf16 rows (prompts), on the
+// fifth-generation tensor cores.
+//
+// A block takes 256 rows (tokens times the query heads of one cached head) as
+// two tiles of 128 and goes over its keys 128 at a time:
+//     S = Q K^T   (tcgen05, Q and K from shared memory, S in TMEM)
+//     P = 2^(scale log2e S - m), row sums l, a row a thread
+//     O += P V    (tcgen05, P from TMEM, where it takes S's place, V from shared memory)
+// While the tensor cores work on one tile of rows, the other one's softmax
+// runs: 2 x (128 x 128 x dk) products each for S and O against 2 x 16,384
+// powers of two a step, some 2,048 cycles of either at dk 128.
+//
+// Four warps turn K's and V's codes into the bf16 values that they stand for
+// (exactly: pkb_cache4.cuh) in the 128-byte swizzled tiles that the tensor
+// cores read: K as [keys][dk], V as [dk][keys], which is how a lane's codes
+// lie in the cache, in stores without bank conflicts. One warp fetches whole
+// units (bulk copies) three half tiles ahead, one thread issues the products,
+// eight warps have the rows.
+//
+// The maximum of a row is raised only where a score passes it by 8 (a factor
+// of 2^8, far inside a float), so O is rescaled in few steps. P is rounded to
+// bf16 once, as V's type asks; l sums what was rounded.
+
+#include <climits>
+
+#include "pkb_attn4.cuh"
+#include "pkb_internal.h"
+
+namespace pkb {
+
+namespace {
+
+constexpr uint32_t FULL = 0xFFFFFFFFu;
+constexpr int SOFT_WARPS = 8, CODE_WARPS = 4, MMA_WARP = SOFT_WARPS + CODE_WARPS, FETCH_WARP = MMA_WARP + 1;
+constexpr int THREADS = (FETCH_WARP + 1) * 32;
+constexpr int ROWS = 256;       // of a block, two tiles of 128
+constexpr int KEYS = 128;       // of a step
+constexpr int RAW_STAGES = 3;   // half steps of codes: 64 keys, four units
+constexpr int KV_STAGES = 2;    // steps of K and of V as bf16
+constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;  // S (and P) of the tiles at 0 and 128, O at 256 and 384
+
+template <int NB> constexpr int slabs() { return (NB + 1) / 2; }             // of 64 dimensions, 128 rows of 128 bytes each
+template <int NB> constexpr int row_tile() { return slabs<NB>() * 16384; }    // 128 rows of Q or of K
+template <int NB> constexpr int v_tile() { return NB * 32 * 256; }            // dk rows of 128 keys, two slabs of 64 keys
+template <int NB> constexpr int raw_bytes() { return 4 * 18 * 32 * NB; }
+template <int NB> constexpr int smem_bytes() {
+    return 2 * row_tile<NB>() + KV_STAGES * (row_tile<NB>() + v_tile<NB>()) + RAW_STAGES * raw_bytes<NB>() + 1024;
+}
+
+struct Bars {
+    uint64_t raw_full[RAW_STAGES], raw_empty[RAW_STAGES];
+    uint64_t k_full[KV_STAGES], k_empty[KV_STAGES], v_full[KV_STAGES], v_empty[KV_STAGES];
+    uint64_t s_full[2], p_full[2], o_full[2], drain;
+};
+
+// D[tmem] (+)= A[tmem] B[smem]^T, a K step of 16, issued by one thread
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 16 registers into 16 consecutive TMEM columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_st_x16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// byte offset of a 16-byte chunk of a row in a slab of 128-byte swizzled rows
+__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// What the rows of a block may see: keys [lo, hi)
+struct Span {
+    int64_t lo, hi;
+};
+__device__ __forceinline__ Span span_of(const Attn4Args& a, const Entry& e, uint32_t tok) {
+    const int64_t pos = static_cast<int64_t>(e.len) - e.rows + tok;
+    const int64_t hi = a.causal ? pos + 1 : e.len, lo = a.window ? pos - a.window + 1 : 0;
+    return {lo < 0 ? 0 : lo, hi < 0 ? 0 : hi > e.len ? e.len : hi};
+}
+
+// K of a unit (16 keys) into rows row0 .. of a tile. A lane has the words of
+// keys g and g + 8: eight values of a block, a 16-byte chunk. Lanes of odd g
+// take a pair of blocks the other way round, so that the eight lanes of a
+// store's quarter meet eight different banks.
+template <int NB>
+__device__ __forceinline__ void write_k(const uint8_t* unit, uint8_t* tile, uint32_t row0) {
+    constexpr int DK = NB * 32;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const uint32_t row = row0 + g + 8 * r;
+        uint32_t w[NB], s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            w[b] = reinterpret_cast<const uint32_t*>(unit)[((g + 8 * r) * 4 + t) * NB + b];
+            s[b] = reinterpret_cast<const uint16_t*>(unit + 16 * DK)[(g + 8 * r) * NB + b];
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            constexpr int PAIRED = NB / 2 * 2;
+            const bool odd = b < PAIRED && (g & 1);
+            const uint32_t x = odd ? w[b < PAIRED ? b ^ 1 : b] : w[b], sc = odd ? s[b < PAIRED ? b ^ 1 : b] : s[b];
+            const uint32_t block = odd ? b ^ 1 : b, s2 = sc | sc << 16, ms = c4_m24(s2), chunk = 4 * block + t;
+            const uint4 v = make_uint4(c4_pair<0>(x, s2, ms), c4_pair<1>(x, s2, ms), c4_pair<2>(x, s2, ms), c4_pair<3>(x, s2, ms));
+            *reinterpret_cast<uint4*>(tile + (chunk / 8) * 16384 + swizzled(row, chunk & 7)) = v;
+        }
+    }
+}
+
+// V of a unit into 16 columns of a slab of 64 keys (quarter 0 .. 3 of it): a
+// lane's pairs of keys go to rows of dimensions 8 apart. Keys from `limit` on
+// become zeros: what lies there may be anything.
+template <int NB>
+__device__ __forceinline__ void write_v(const uint8_t* unit, uint8_t* slab, uint32_t quarter, int32_t key0, int32_t limit) {
+    constexpr int DK = NB * 32;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+    const bool edge = key0 + C4_UNIT > limit;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * DK + ((b * 8 + g) * 4 + t) * 8);
+        uint32_t s2[2], ms[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            s2[c] = *reinterpret_cast<const uint32_t*>(unit + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
+            if (edge) {
+                const int32_t key = key0 + 8 * c + 2 * static_cast<int32_t>(t);
+                if (key >= limit) s2[c] = 0;
+                else if (key + 1 >= limit) s2[c] &= 0xFFFFu;
+            }
+            ms[c] = c4_m24(s2[c]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t x = j ? w.y : w.x, dim = 32 * b + 16 * j + g;
+            uint8_t* at = slab + 4 * t;
+            *reinterpret_cast<uint32_t*>(at + swizzled(dim, 2 * quarter)) = c4_pair<0>(x, s2[0], ms[0]);
+            *reinterpret_cast<uint32_t*>(at + swizzled(dim + 8, 2 * quarter)) = c4_pair<1>(x, s2[0], ms[0]);
+            *reinterpret_cast<uint32_t*>(at + swizzled(dim, 2 * quarter + 1)) = c4_pair<2>(x, s2[1], ms[1]);
+            *reinterpret_cast<uint32_t*>(at + swizzled(dim + 8, 2 * quarter + 1)) = c4_pair<3>(x, s2[1], ms[1]);
+        }
+    }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
+    constexpr int DK = NB * 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Bars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int gave_up;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* q_tile = smem;
+    uint8_t* k_tile = q_tile + 2 * row_tile<NB>();
+    uint8_t* v_tiles = k_tile + KV_STAGES * row_tile<NB>();
+    uint8_t* raw = v_tiles + KV_STAGES * v_tile<NB>();
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    if (tid == 0) {
+        for (int i = 0; i < RAW_STAGES; i++) mbar_init(&bars.raw_full[i], 1), mbar_init(&bars.raw_empty[i], CODE_WARPS);
+        for (int i = 0; i < KV_STAGES; i++) {
+            mbar_init(&bars.k_full[i], CODE_WARPS), mbar_init(&bars.v_full[i], CODE_WARPS);
+            mbar_init(&bars.k_empty[i], 1), mbar_init(&bars.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_full[i], 4), mbar_init(&bars.o_full[i], 1);
+        mbar_init(&bars.drain, 1);
+        fence_mbar_init();
+        gave_up = 0;
+    }
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t h = blockIdx.y;
+    const Entry e = load_entry(a, blockIdx.z);
+    const uint32_t all = e.rows * a.G, groups = (all + ROWS - 1) / ROWS;
+    if (blockIdx.x >= groups) return;  // the whole block
+    // the last rows, which see most, begin first
+    const uint32_t group = groups - 1 - blockIdx.x, row0 = group * ROWS, tiles = all - row0 > 128 ? 2 : 1;
+    const uint32_t last = min(row0 + ROWS, all) - 1;
+    const int64_t lo = span_of(a, e, row0 / a.G).lo, hi = span_of(a, e, last / a.G).hi;
+    const uint32_t unit0 = static_cast<uint32_t>(lo / C4_UNIT);
+    const uint32_t units = hi > lo ? static_cast<uint32_t>((hi + C4_UNIT - 1) / C4_UNIT) - unit0 : 0;
+    const uint32_t steps = (units * C4_UNIT + KEYS - 1) / KEYS;
+    const int32_t key_base = static_cast<int32_t>(unit0 * C4_UNIT);
+    if (warp == MMA_WARP) {
+        tmem_alloc(&tmem_slot, TMEM_COLS);
+        tmem_relinquish();
+    }
+    // Q, zeros for rows there are none of; a negative scale's sign goes with it
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    for (uint32_t x = tid; x < tiles * 128 * (DK / 8); x += THREADS) {
+        const uint32_t r = x / (DK / 8), chunk = x % (DK / 8), row = row0 + r, tok = row / a.G;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < all) {
+            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(e.r0 + tok) * a.qs +
+                                     static_cast<size_t>(h * a.G + row - tok * a.G) * DK + 8 * chunk;
+            if (a.vec) {
+                v = __ldg(reinterpret_cast<const uint4*>(p));
+            } else {
+                alignas(16) __nv_bfloat16 y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = p[i];
+                v = *reinterpret_cast<const uint4*>(y);
+            }
+            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        }
+        *reinterpret_cast<uint4*>(q_tile + (r / 128) * row_tile<NB>() + (chunk / 8) * 16384 + swizzled(r % 128, chunk & 7)) = v;
+    }
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == FETCH_WARP) {
+        // a lane a unit of the half step
+        const uint32_t per = a.c.pshift - 4, halves = (units + 3) / 4;
+        const int32_t* table = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
+        const uint8_t* head = a.c.pages + a.layer * a.c.layer_bytes + h * a.c.head_bytes;
+        int32_t page = lane < 4 && lane < units ? table[(unit0 + lane) >> per] : 0;
+        uint32_t issued = 0;
+        for (uint32_t i = 0; i < halves; i++, issued++) {
+            const int st = i % RAW_STAGES;
+            if (!warp_wait(&bars.raw_empty[st], (i / RAW_STAGES & 1) ^ 1, &gave_up, a.timeout)) {
+                gave_up = 1;
+                if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&bars.raw_full[st], min(4u, units - 4 * i) * 18 * DK);
+            __syncwarp();
+            const uint32_t u = 4 * i + lane, unit = unit0 + u;
+            if (lane < 4 && u < units) {
+                if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
+                    atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
+                    page = 0;
+                }
+                bulk_load(raw + st * raw_bytes<NB>() + lane * 18 * DK,
+                          head + static_cast<uint32_t>(page) * a.c.page_bytes + (unit & ((1u << per) - 1)) * (18 * DK), 18 * DK, &bars.raw_full[st]);
+                if (u + 4 < units) page = table[(unit + 4) >> per];
+            }
+        }
+        // whatever the others did, the copies in flight land before the block leaves its memory
+        for (uint32_t i = issued < RAW_STAGES ? 0 : issued - RAW_STAGES; i < issued; i++)
+            mbar_drain(&bars.raw_full[i % RAW_STAGES], i / RAW_STAGES & 1, a.timeout);
+    } else if (warp == MMA_WARP) {
+        if (lane == 0 && steps) {
+            const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_tile), v_at = smem_u32(v_tiles);
+            constexpr uint32_t QK = bf16_instr_desc(128, KEYS), PV = bf16_instr_desc(128, DK);
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                ok = ok && mbar_wait(bar, parity, &gave_up, a.timeout);
+                if (ok) tc_fence_after();
+                return ok;
+            };
+            auto scores = [&](uint32_t t, uint32_t i) {
+                const uint32_t qa = q_at + t * row_tile<NB>(), ka = k_at + i % KV_STAGES * row_tile<NB>();
+#pragma unroll
+                for (int k = 0; k < DK / 16; k++)
+                    umma_bf16(tmem + S_COL + 128 * t, sw128_kmajor_desc(qa + k / 4 * 16384 + k % 4 * 32),
+                              sw128_kmajor_desc(ka + k / 4 * 16384 + k % 4 * 32), QK, k > 0);
+                umma_commit(&bars.s_full[t]);
+            };
+            auto values = [&](uint32_t t, uint32_t i) {
+                const uint32_t va = v_at + i % KV_STAGES * v_tile<NB>();
+#pragma unroll
+                for (int k = 0; k < KEYS / 16; k++)
+                    umma_bf16_ts(tmem + O_COL + 128 * t, tmem + S_COL + 128 * t + 8 * k, sw128_kmajor_desc(va + k / 4 * (DK * 128) + k % 4 * 32), PV,
+                                 i > 0 || k > 0);
+            };
+            if (wait(&bars.k_full[0], 0)) {
+                for (uint32_t t = 0; t < tiles; t++) scores(t, 0);
+                umma_commit(&bars.k_empty[0]);
+            }
+            // a tile's next scores follow its values: they take P's place in
+            // TMEM, and products of one thread run in their order
+            for (uint32_t i = 0; ok && i < steps; i++) {
+                const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1, st1 = (i + 1) % KV_STAGES, ph1 = (i + 1) / KV_STAGES & 1;
+                const bool more = i + 1 < steps;
+                if (!wait(&bars.v_full[st], ph)) break;
+                for (uint32_t t = 0; t < tiles; t++) {
+                    if (!wait(&bars.p_full[t], i & 1)) break;
+                    values(t, i);
+                    if (t + 1 == tiles) umma_commit(&bars.v_empty[st]);
+                    if (!more) {
+                        umma_commit(&bars.o_full[t]);
+                    } else {
+                        if (t == 0 && !wait(&bars.k_full[st1], ph1)) break;
+                        scores(t, i + 1);
+                        if (t + 1 == tiles) umma_commit(&bars.k_empty[st1]);
+                    }
+                }
+            }
+            if (!ok) {
+                gave_up = 1;
+                atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                // what this thread issued finishes before TMEM is freed
+                umma_commit(&bars.drain);
+                mbar_drain(&bars.drain, 0, a.timeout);
+            }
+        }
+    } else if (warp >= SOFT_WARPS) {
+        // codes to values: a warp a unit of each half step
+        const uint32_t w = warp - SOFT_WARPS;
+        for (uint32_t i = 0; i < steps; i++) {
+            const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1;
+            const uint32_t halves = min(2u, (units - 8 * i + 3) / 4);
+            uint8_t* kt = k_tile + st * row_tile<NB>();
+            uint8_t* vt = v_tiles + st * v_tile<NB>();
+            bool ok = warp_wait(&bars.k_empty[st], ph ^ 1, &gave_up, a.timeout);
+            for (uint32_t half = 0; ok && half < halves; half++) {
+                const uint32_t ri = 2 * i + half;
+                ok = warp_wait(&bars.raw_full[ri % RAW_STAGES], ri / RAW_STAGES & 1, &gave_up, a.timeout);
+                if (ok) write_k<NB>(raw + ri % RAW_STAGES * raw_bytes<NB>() + w * 18 * DK, kt, 64 * half + 16 * w);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&bars.k_full[st]);
+            ok = ok && warp_wait(&bars.v_empty[st], ph ^ 1, &gave_up, a.timeout);
+            for (uint32_t half = 0; ok && half < 2; half++) {
+                const uint32_t ri = 2 * i + half;
+                // a half step past the last unit is zeros too: any codes will do
+                write_v<NB>(raw + ri % RAW_STAGES * raw_bytes<NB>() + w * 18 * DK, vt + half * (DK * 128), w,
+                            key_base + static_cast<int32_t>(i * KEYS + 64 * half + 16 * w), half < halves ? static_cast<int32_t>(hi) : INT_MIN);
+                __syncwarp();
+                if (half < halves && lane == 0) mbar_arrive(&bars.raw_empty[ri % RAW_STAGES]);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&bars.v_full[st]);
+            if (!ok) {
+                gave_up = 1;
+                if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                break;
+            }
+        }
+    } else if (warp / 4 < tiles) {
+        // the rows: thread i of a tile's four warps has row i
+        const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
+        const Span span = row < all ? span_of(a, e, tok) : Span{0, 0};
+        const uint32_t at = tmem + ((warp % 4) * 32 << 16), s_at = at + S_COL + 128 * t, o_at = at + O_COL + 128 * t;
+        const float scale = fmaxf(fabsf(a.scale), 1e-37f);  // of a scale 0 too
+        float m = NEG_INF, l = 0.0f;
+        bool ok = true;
+        for (uint32_t i = 0; i < steps; i++) {
+            ok = warp_wait(&bars.s_full[t], i & 1, &gave_up, a.timeout);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t key0 = static_cast<int64_t>(key_base) + i * KEYS;
+            const int32_t first = static_cast<int32_t>(max(min(span.lo - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
+            const int32_t end = static_cast<int32_t>(max(min(span.hi - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
+            const bool mask = __any_sync(FULL, first > 0 || end < KEYS);
+            float top = NEG_INF;
+            uint32_t s[32];
+#pragma unroll
+            for (int c = 0; c < KEYS / 32; c++) {
+                tmem_ld_32x32b_x32(s_at + 32 * c, s);
+                tmem_ld_wait(s);
+                if (mask) {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) top = fmaxf(top, 32 * c + x >= first && 32 * c + x < end ? __uint_as_float(s[x]) : NEG_INF);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(s[x]));
+                }
+            }
+            top = __fmul_rn(top, scale);
+            if (__any_sync(FULL, top > m + 8.0f)) {
+                const float raised = fmaxf(m, top), f = rescale(m, raised);
+                m = raised;
+                l *= f;
+                // the values of the step before are in O: its scores' commit covers them
+                for (int c = 0; i && c < NB; c++) {
+                    uint32_t y[32];
+                    tmem_ld_32x32b_x32(o_at + 32 * c, y);
+                    tmem_ld_wait(y);
+                    uint32_t z[16];
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++) z[x] = __float_as_uint(__fmul_rn(__uint_as_float(y[16 * half + x]), f));
+                        tmem_st_x16(o_at + 32 * c + 16 * half, z);
+                    }
+                }
+                tmem_st_wait();
+            }
+            const float minus = m == NEG_INF ? 0.0f : -m;
+#pragma unroll
+            for (int c = 0; c < KEYS / 32; c++) {
+                tmem_ld_32x32b_x32(s_at + 32 * c, s);
+                tmem_ld_wait(s);
+                float p[32];
+#pragma unroll
+                for (int x = 0; x < 32; x++) p[x] = exp2_fast(__fmaf_rn(__uint_as_float(s[x]), scale, minus));
+                if (mask) {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) p[x] = 32 * c + x >= first && 32 * c + x < end ? p[x] : 0.0f;
+                }
+                uint32_t z[16];
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < 32; x++) sum[x & 3] += p[x];
+#pragma unroll
+                for (int x = 0; x < 16; x++) z[x] = bf16_pair(p[2 * x], p[2 * x + 1]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_x16(s_at + 16 * c, z);  // P's place: columns of S that have been read
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_full[t]);
+        }
+        if (steps && ok) {
+            ok = warp_wait(&bars.o_full[t], 0, &gave_up, a.timeout);
+            tc_fence_after();
+        }
+        if (!ok) {
+            gave_up = 1;
+            if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+        } else {
+            // a row that sees nothing has sum 0 and is zeros; a NaN sum gives NaNs
+            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + static_cast<size_t>(e.r0 + tok) * a.os +
+                                 static_cast<size_t>(h * a.G + row - tok * a.G) * DK;
+#pragma unroll
+            for (int c = 0; c < NB; c++) {
+                uint32_t y[32];
+                if (steps) {
+                    tmem_ld_32x32b_x32(o_at + 32 * c, y);
+                    tmem_ld_wait(y);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) y[x] = 0;
+                }
+                alignas(16) uint32_t z[16];
+#pragma unroll
+                for (int x = 0; x < 16; x++) z[x] = bf16_pair(__fmul_rn(__uint_as_float(y[2 * x]), inv), __fmul_rn(__uint_as_float(y[2 * x + 1]), inv));
+                if (row < all) {
+                    if (a.vec_o) {
+#pragma unroll
+                        for (int x = 0; x < 4; x++) reinterpret_cast<uint4*>(out + 32 * c)[x] = make_uint4(z[4 * x], z[4 * x + 1], z[4 * x + 2], z[4 * x + 3]);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            out[32 * c + x] = __ushort_as_bfloat16(static_cast<unsigned short>(x & 1 ? z[x / 2] >> 16 : z[x / 2] & 0xFFFFu));
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+template <int NB>
+cudaError_t launch_one(const Attn4Args& a, cudaStream_t s) {
+    const dim3 grid((a.max_rows * a.G + ROWS - 1) / ROWS, a.c.heads, a.n);
+    return c4_launch(prompt_kernel<NB>, grid, THREADS, smem_bytes<NB>(), s, a);
+}
+
+}  // namespace
+
+bool attention4_tc_takes(const Attn4Args& a, int type) { return type == PKB_BF16 && a.c.dk <= 128; }
+
+cudaError_t prepare_attention4_tc() {
+    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<1>());
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prompt_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<2>());
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prompt_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<3>());
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prompt_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<4>());
+    return e;
+}
+
+cudaError_t launch_attention4_tc(const Attn4Args& a, cudaStream_t stream) {
+    const cudaError_t e = a.c.dk == 32   ? launch_one<1>(a, stream)
+                          : a.c.dk == 64 ? launch_one<2>(a, stream)
+                          : a.c.dk == 96 ? launch_one<3>(a, stream)
+                                         : launch_one<4>(a, stream);
+    if (e == cudaSuccess) count_launch();
+    return e;
+}
+
+}  // namespace pkb
