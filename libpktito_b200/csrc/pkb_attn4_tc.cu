@@ -32,7 +32,10 @@ namespace {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int SOFT_WARPS = 8, CODE_WARPS = 4, MMA_WARP = SOFT_WARPS + CODE_WARPS, FETCH_WARP = MMA_WARP + 1;
-constexpr int THREADS = (FETCH_WARP + 1) * 32;
+constexpr int THREADS = 512;    // four warpgroups; the last one's two spare warps wait for the end
+// A thread's registers: 65,536 / 512 at launch, then the rows' warps take
+// what the others leave: 256 x 168 + 128 x 104 + 128 x 64 = 64,512.
+constexpr int SOFT_REGS = 168, CODE_REGS = 104, ISSUE_REGS = 64;
 constexpr int ROWS = 256;       // of a block, two tiles of 128
 constexpr int KEYS = 128;       // of a step
 constexpr int RAW_STAGES = 3;   // half steps of codes: 64 keys, four units
@@ -85,31 +88,57 @@ __device__ __forceinline__ Span span_of(const Attn4Args& a, const Entry& e, uint
     return {lo < 0 ? 0 : lo, hi < 0 ? 0 : hi > e.len ? e.len : hi};
 }
 
-// K of a unit (16 keys) into rows row0 .. of a tile. A lane has the words of
-// keys g and g + 8: eight values of a block, a 16-byte chunk. Lanes of odd g
-// take a pair of blocks the other way round, so that the eight lanes of a
-// store's quarter meet eight different banks.
+// NB words from shared memory, as wide as they lie
+template <int N>
+__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+
+// K of a unit (16 keys) into 16 rows of a tile from `rows` on. A lane has the
+// words of keys g and g + 8: eight values of a block, a 16-byte chunk. Lanes
+// of odd g take a pair of blocks the other way round, so that the eight
+// lanes of a store's quarter meet eight different banks.
 template <int NB>
-__device__ __forceinline__ void write_k(const uint8_t* unit, uint8_t* tile, uint32_t row0) {
-    constexpr int DK = NB * 32;
-    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+__device__ __forceinline__ void write_k(const uint8_t* unit, uint8_t* rows) {
+    constexpr int DK = NB * 32, PAIRED = NB / 2 * 2;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3, odd = g & 1;
+    uint8_t* const even_at = rows + g * 128 + (((4 * odd + t) ^ g) << 4);        // of the pair's block taken first
+    uint8_t* const odd_at = rows + g * 128 + (((4 * (odd ^ 1) + t) ^ g) << 4);   // and second
+    uint8_t* const last_at = rows + g * 128 + ((t ^ g) << 4);                    // of a block without a pair
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-        const uint32_t row = row0 + g + 8 * r;
-        uint32_t w[NB], s[NB];
+        uint32_t w[NB], sc[(NB + 1) / 2];
+        lds<NB>(unit + ((g + 8 * r) * 4 + t) * NB * 4, w);
+        if constexpr (NB % 2 == 0) {
+            lds<NB / 2>(unit + 16 * DK + (g + 8 * r) * NB * 2, sc);
+        } else {
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            w[b] = reinterpret_cast<const uint32_t*>(unit)[((g + 8 * r) * 4 + t) * NB + b];
-            s[b] = reinterpret_cast<const uint16_t*>(unit + 16 * DK)[(g + 8 * r) * NB + b];
+            for (int b = 0; b < NB; b += 2) {
+                const uint16_t* at = reinterpret_cast<const uint16_t*>(unit + 16 * DK + (g + 8 * r) * NB * 2) + b;
+                sc[b / 2] = at[0];
+                if (b + 1 < NB) sc[b / 2] |= static_cast<uint32_t>(at[1]) << 16;
+            }
         }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            constexpr int PAIRED = NB / 2 * 2;
-            const bool odd = b < PAIRED && (g & 1);
-            const uint32_t x = odd ? w[b < PAIRED ? b ^ 1 : b] : w[b], sc = odd ? s[b < PAIRED ? b ^ 1 : b] : s[b];
-            const uint32_t block = odd ? b ^ 1 : b, s2 = sc | sc << 16, ms = c4_m24(s2), chunk = 4 * block + t;
+            const bool pair = b < PAIRED;
+            const uint32_t x = pair && odd ? w[pair ? b ^ 1 : b] : w[b];
+            // the block's scale in both halves: the low or the high one of its pair's word
+            const uint32_t s2 = __byte_perm(sc[b / 2], 0, pair && odd ? (b % 2 ? 0x1010 : 0x3232) : (b % 2 ? 0x3232 : 0x1010)), ms = c4_m24(s2);
             const uint4 v = make_uint4(c4_pair<0>(x, s2, ms), c4_pair<1>(x, s2, ms), c4_pair<2>(x, s2, ms), c4_pair<3>(x, s2, ms));
-            *reinterpret_cast<uint4*>(tile + (chunk / 8) * 16384 + swizzled(row, chunk & 7)) = v;
+            *reinterpret_cast<uint4*>((!pair ? last_at : b % 2 ? odd_at : even_at) + b / 2 * 16384 + r * 1024) = v;
         }
     }
 }
@@ -122,6 +151,8 @@ __device__ __forceinline__ void write_v(const uint8_t* unit, uint8_t* slab, uint
     constexpr int DK = NB * 32;
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     const bool edge = key0 + C4_UNIT > limit;
+    uint8_t* const lo_at = slab + g * 128 + 4 * t + (((2 * quarter) ^ g) << 4);       // keys 2t, 2t + 1
+    uint8_t* const hi_at = slab + g * 128 + 4 * t + (((2 * quarter + 1) ^ g) << 4);   // keys 8 + 2t, 9 + 2t
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * DK + ((b * 8 + g) * 4 + t) * 8);
@@ -138,14 +169,117 @@ __device__ __forceinline__ void write_v(const uint8_t* unit, uint8_t* slab, uint
         }
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const uint32_t x = j ? w.y : w.x, dim = 32 * b + 16 * j + g;
-            uint8_t* at = slab + 4 * t;
-            *reinterpret_cast<uint32_t*>(at + swizzled(dim, 2 * quarter)) = c4_pair<0>(x, s2[0], ms[0]);
-            *reinterpret_cast<uint32_t*>(at + swizzled(dim + 8, 2 * quarter)) = c4_pair<1>(x, s2[0], ms[0]);
-            *reinterpret_cast<uint32_t*>(at + swizzled(dim, 2 * quarter + 1)) = c4_pair<2>(x, s2[1], ms[1]);
-            *reinterpret_cast<uint32_t*>(at + swizzled(dim + 8, 2 * quarter + 1)) = c4_pair<3>(x, s2[1], ms[1]);
+            const uint32_t x = j ? w.y : w.x;
+            const int at = (32 * b + 16 * j) * 128;  // dimensions 32 b + 16 j + g, and 8 on
+            *reinterpret_cast<uint32_t*>(lo_at + at) = c4_pair<0>(x, s2[0], ms[0]);
+            *reinterpret_cast<uint32_t*>(lo_at + at + 1024) = c4_pair<1>(x, s2[0], ms[0]);
+            *reinterpret_cast<uint32_t*>(hi_at + at) = c4_pair<2>(x, s2[1], ms[1]);
+            *reinterpret_cast<uint32_t*>(hi_at + at + 1024) = c4_pair<3>(x, s2[1], ms[1]);
         }
     }
+}
+
+// The largest of three
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// P of 32 columns: 2^(s scale + minus), its sum into two running ones, rounded
+// to bf16 and put into 16 TMEM columns. Columns outside [first, end) are 0.
+template <bool MASK>
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t minus2, int32_t first, int32_t end, uint64_t (&sum)[2],
+                                        uint32_t to) {
+    uint32_t z[16];
+#pragma unroll
+    for (int x = 0; x < 16; x++) {
+        float p0, p1;
+        unpack2(fma2_r<0>(pack2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), scale2, minus2), p0, p1);
+        p0 = exp2_fast(p0);
+        p1 = exp2_fast(p1);
+        if constexpr (MASK) {
+            p0 = 2 * x >= first && 2 * x < end ? p0 : 0.0f;
+            p1 = 2 * x + 1 >= first && 2 * x + 1 < end ? p1 : 0.0f;
+        }
+        sum[x & 1] = add2_rn(sum[x & 1], pack2(p0, p1));
+        z[x] = bf16_pair(p0, p1);
+    }
+    tmem_st_x16(to, z);
+}
+
+// The largest of 32 columns of S and `top`
+template <bool MASK>
+__device__ __forceinline__ float largest(const uint32_t (&s)[32], int32_t first, int32_t end, float top) {
+    float other = NEG_INF;
+#pragma unroll
+    for (int x = 0; x < 32; x += 4) {
+        float v[4];
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            v[y] = __uint_as_float(s[x + y]);
+            if constexpr (MASK) v[y] = x + y >= first && x + y < end ? v[y] : NEG_INF;
+        }
+        top = max3(top, v[0], v[1]);
+        other = max3(other, v[2], v[3]);
+    }
+    return fmaxf(top, other);
+}
+
+// A step of a row: its 128 scores at s_at become P in the upper half of their
+// place. Half of the scores are kept from the search for the maximum, the
+// other half is read again.
+template <int NB, bool MASK>
+__device__ __forceinline__ void softmax_step(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l) {
+    uint32_t a[32], b[32], c[32];
+    tmem_ld_32x32b_x32(s_at, a);
+    tmem_ld_wait(a);
+    tmem_ld_32x32b_x32(s_at + 32, b);
+    float top = largest<MASK>(a, first, end, NEG_INF);
+    tmem_ld_wait(b);
+    tmem_ld_32x32b_x32(s_at + 64, a);
+    tmem_ld_32x32b_x32(s_at + 96, c);
+    top = largest<MASK>(b, first - 32, end - 32, top);
+    tmem_ld_wait(a);
+    tmem_ld_settled(c);
+    top = largest<MASK>(a, first - 64, end - 64, top);
+    top = __fmul_rn(largest<MASK>(c, first - 96, end - 96, top), scale);
+    if (__any_sync(FULL, top > m + 8.0f)) {
+        const float raised = fmaxf(m, top), f = rescale(m, raised);
+        m = raised;
+        l *= f;
+        // the values of the step before are in O: its scores' commit covers them
+        for (int d = 0; begun && d < 2 * NB; d++) {
+            uint32_t y[16];
+            tmem_ld_32x32b_x16(o_at + 16 * d, y);
+            tmem_ld_wait(y);
+#pragma unroll
+            for (int x = 0; x < 16; x++) y[x] = __float_as_uint(__fmul_rn(__uint_as_float(y[x]), f));
+            tmem_st_x16(o_at + 16 * d, y);
+        }
+    }
+    const float minus = m == NEG_INF ? 0.0f : -m;
+    const uint64_t scale2 = pack2(scale, scale), minus2 = pack2(minus, minus);
+    uint64_t sum[2] = {0, 0};
+    tmem_ld_32x32b_x32(s_at, b);
+    weights<MASK>(a, scale2, minus2, first - 64, end - 64, sum, s_at + 96);
+    weights<MASK>(c, scale2, minus2, first - 96, end - 96, sum, s_at + 112);
+    tmem_ld_wait(b);
+    tmem_ld_32x32b_x32(s_at + 32, a);
+    weights<MASK>(b, scale2, minus2, first, end, sum, s_at + 64);
+    tmem_ld_wait(a);
+    weights<MASK>(a, scale2, minus2, first - 32, end - 32, sum, s_at + 80);
+    float s0, s1, s2, s3;
+    unpack2(sum[0], s0, s1);
+    unpack2(sum[1], s2, s3);
+    l += (s0 + s1) + (s2 + s3);
+    tmem_st_wait();
+}
+
+template <int REGS, bool MORE>
+__device__ __forceinline__ void set_registers() {
+    if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 template <int NB>
@@ -174,12 +308,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     }
     pdl_trigger();
     pdl_wait();
-    const uint32_t h = blockIdx.y;
-    const Entry e = load_entry(a, blockIdx.z);
+    // the last rows of all entries and heads, which see most, begin first
+    const uint32_t rank = blockIdx.x / (a.n * a.c.heads), h = blockIdx.x % a.c.heads;
+    const Entry e = load_entry(a, blockIdx.x / a.c.heads % a.n);
     const uint32_t all = e.rows * a.G, groups = (all + ROWS - 1) / ROWS;
-    if (blockIdx.x >= groups) return;  // the whole block
-    // the last rows, which see most, begin first
-    const uint32_t group = groups - 1 - blockIdx.x, row0 = group * ROWS, tiles = all - row0 > 128 ? 2 : 1;
+    if (rank >= groups) return;  // the whole block
+    const uint32_t group = groups - 1 - rank, row0 = group * ROWS, tiles = all - row0 > 128 ? 2 : 1;
     const uint32_t last = min(row0 + ROWS, all) - 1;
     const int64_t lo = span_of(a, e, row0 / a.G).lo, hi = span_of(a, e, last / a.G).hi;
     const uint32_t unit0 = static_cast<uint32_t>(lo / C4_UNIT);
@@ -217,6 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     const uint32_t tmem = tmem_slot;
 
     if (warp == FETCH_WARP) {
+        set_registers<ISSUE_REGS, false>();
         // a lane a unit of the half step
         const uint32_t per = a.c.pshift - 4, halves = (units + 3) / 4;
         const int32_t* table = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
@@ -246,7 +381,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         // whatever the others did, the copies in flight land before the block leaves its memory
         for (uint32_t i = issued < RAW_STAGES ? 0 : issued - RAW_STAGES; i < issued; i++)
             mbar_drain(&bars.raw_full[i % RAW_STAGES], i / RAW_STAGES & 1, a.timeout);
+    } else if (warp > FETCH_WARP) {
+        set_registers<ISSUE_REGS, false>();
     } else if (warp == MMA_WARP) {
+        set_registers<ISSUE_REGS, false>();
         if (lane == 0 && steps) {
             const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_tile), v_at = smem_u32(v_tiles);
             constexpr uint32_t QK = bf16_instr_desc(128, KEYS), PV = bf16_instr_desc(128, DK);
@@ -268,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
                 const uint32_t va = v_at + i % KV_STAGES * v_tile<NB>();
 #pragma unroll
                 for (int k = 0; k < KEYS / 16; k++)
-                    umma_bf16_ts(tmem + O_COL + 128 * t, tmem + S_COL + 128 * t + 8 * k, sw128_kmajor_desc(va + k / 4 * (DK * 128) + k % 4 * 32), PV,
+                    umma_bf16_ts(tmem + O_COL + 128 * t, tmem + S_COL + 128 * t + 64 + 8 * k, sw128_kmajor_desc(va + k / 4 * (DK * 128) + k % 4 * 32), PV,
                                  i > 0 || k > 0);
             };
             if (wait(&bars.k_full[0], 0)) {
@@ -302,8 +440,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
                 mbar_drain(&bars.drain, 0, a.timeout);
             }
         }
-    } else if (warp >= SOFT_WARPS) {
+    } else if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         // codes to values: a warp a unit of each half step
+        set_registers<CODE_REGS, false>();
         const uint32_t w = warp - SOFT_WARPS;
         for (uint32_t i = 0; i < steps; i++) {
             const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1;
@@ -314,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             for (uint32_t half = 0; ok && half < halves; half++) {
                 const uint32_t ri = 2 * i + half;
                 ok = warp_wait(&bars.raw_full[ri % RAW_STAGES], ri / RAW_STAGES & 1, &gave_up, a.timeout);
-                if (ok) write_k<NB>(raw + ri % RAW_STAGES * raw_bytes<NB>() + w * 18 * DK, kt, 64 * half + 16 * w);
+                if (ok) write_k<NB>(raw + ri % RAW_STAGES * raw_bytes<NB>() + w * 18 * DK, kt + (64 * half + 16 * w) * 128);
             }
             fence_async_smem();
             __syncwarp();
@@ -337,8 +476,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
                 break;
             }
         }
-    } else if (warp / 4 < tiles) {
+    } else if (warp < SOFT_WARPS && warp / 4 < tiles) {
         // the rows: thread i of a tile's four warps has row i
+        set_registers<SOFT_REGS, true>();
         const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
         const Span span = row < all ? span_of(a, e, tok) : Span{0, 0};
         const uint32_t at = tmem + ((warp % 4) * 32 << 16), s_at = at + S_COL + 128 * t, o_at = at + O_COL + 128 * t;
@@ -353,62 +493,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             const int32_t first = static_cast<int32_t>(max(min(span.lo - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
             const int32_t end = static_cast<int32_t>(max(min(span.hi - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
             const bool mask = __any_sync(FULL, first > 0 || end < KEYS);
-            float top = NEG_INF;
-            uint32_t s[32];
-#pragma unroll
-            for (int c = 0; c < KEYS / 32; c++) {
-                tmem_ld_32x32b_x32(s_at + 32 * c, s);
-                tmem_ld_wait(s);
-                if (mask) {
-#pragma unroll
-                    for (int x = 0; x < 32; x++) top = fmaxf(top, 32 * c + x >= first && 32 * c + x < end ? __uint_as_float(s[x]) : NEG_INF);
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(s[x]));
-                }
-            }
-            top = __fmul_rn(top, scale);
-            if (__any_sync(FULL, top > m + 8.0f)) {
-                const float raised = fmaxf(m, top), f = rescale(m, raised);
-                m = raised;
-                l *= f;
-                // the values of the step before are in O: its scores' commit covers them
-                for (int c = 0; i && c < NB; c++) {
-                    uint32_t y[32];
-                    tmem_ld_32x32b_x32(o_at + 32 * c, y);
-                    tmem_ld_wait(y);
-                    uint32_t z[16];
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {
-#pragma unroll
-                        for (int x = 0; x < 16; x++) z[x] = __float_as_uint(__fmul_rn(__uint_as_float(y[16 * half + x]), f));
-                        tmem_st_x16(o_at + 32 * c + 16 * half, z);
-                    }
-                }
-                tmem_st_wait();
-            }
-            const float minus = m == NEG_INF ? 0.0f : -m;
-#pragma unroll
-            for (int c = 0; c < KEYS / 32; c++) {
-                tmem_ld_32x32b_x32(s_at + 32 * c, s);
-                tmem_ld_wait(s);
-                float p[32];
-#pragma unroll
-                for (int x = 0; x < 32; x++) p[x] = exp2_fast(__fmaf_rn(__uint_as_float(s[x]), scale, minus));
-                if (mask) {
-#pragma unroll
-                    for (int x = 0; x < 32; x++) p[x] = 32 * c + x >= first && 32 * c + x < end ? p[x] : 0.0f;
-                }
-                uint32_t z[16];
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int x = 0; x < 32; x++) sum[x & 3] += p[x];
-#pragma unroll
-                for (int x = 0; x < 16; x++) z[x] = bf16_pair(p[2 * x], p[2 * x + 1]);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_x16(s_at + 16 * c, z);  // P's place: columns of S that have been read
-            }
-            tmem_st_wait();
+            if (mask) softmax_step<NB, true>(s_at, o_at, i > 0, scale, first, end, m, l);
+            else softmax_step<NB, false>(s_at, o_at, i > 0, scale, 0, KEYS, m, l);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.p_full[t]);
@@ -461,8 +547,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
 
 template <int NB>
 cudaError_t launch_one(const Attn4Args& a, cudaStream_t s) {
-    const dim3 grid((a.max_rows * a.G + ROWS - 1) / ROWS, a.c.heads, a.n);
-    return c4_launch(prompt_kernel<NB>, grid, THREADS, smem_bytes<NB>(), s, a);
+    const uint64_t grid = (static_cast<uint64_t>(a.max_rows) * a.G + ROWS - 1) / ROWS * a.c.heads * a.n;
+    if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
+    return c4_launch(prompt_kernel<NB>, static_cast<uint32_t>(grid), THREADS, smem_bytes<NB>(), s, a);
 }
 
 }  // namespace
