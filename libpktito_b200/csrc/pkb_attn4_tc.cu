@@ -13,8 +13,10 @@
 // Four warps turn K's and V's codes into the bf16 values that they stand for
 // (exactly: pkb_cache4.cuh) in the 128-byte swizzled tiles that the tensor
 // cores read: K as [keys][dk], V as [dk][keys], which is how a lane's codes
-// lie in the cache, in stores without bank conflicts. One warp fetches whole
-// units (bulk copies) three half tiles ahead, one thread issues the products,
+// lie in the cache, in stores without bank conflicts. They load the codes a
+// step ahead into registers (with the bf16 tiles of two steps and Q, shared
+// memory has no room for a ring that covers a load's latency: 1.37 ms with
+// one of 96 keys' codes ahead, [TIME] so). One thread issues the products,
 // eight warps have the rows.
 //
 // The maximum of a row is raised only where a score passes it by 8 (a factor
@@ -31,38 +33,62 @@ namespace pkb {
 namespace {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
-constexpr int SOFT_WARPS = 8, CODE_WARPS = 4, MMA_WARP = SOFT_WARPS + CODE_WARPS, FETCH_WARP = MMA_WARP + 1;
-constexpr int THREADS = 512;    // four warpgroups; the last one's two spare warps wait for the end
+constexpr int SOFT_WARPS = 8, CODE_WARPS = 4, MMA_WARP = SOFT_WARPS + CODE_WARPS;
+constexpr int THREADS = 512;    // four warpgroups; the last one's three spare warps wait for the end
 // A thread's registers: 65,536 / 512 at launch, then the rows' warps take
-// what the others leave: 256 x 168 + 128 x 104 + 128 x 64 = 64,512.
-constexpr int SOFT_REGS = 168, CODE_REGS = 104, ISSUE_REGS = 64;
+// what the others leave: 256 x 168 + 128 x 120 + 128 x 48 = 64,512.
+constexpr int SOFT_REGS = 168, CODE_REGS = 120, ISSUE_REGS = 48;
 constexpr int ROWS = 256;       // of a block, two tiles of 128
 constexpr int KEYS = 128;       // of a step
-constexpr int RAW_STAGES = 3;   // half steps of codes: 64 keys, four units
 constexpr int KV_STAGES = 2;    // steps of K and of V as bf16
 constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;  // S (and P) of the tiles at 0 and 128, O at 256 and 384
 
 template <int NB> constexpr int slabs() { return (NB + 1) / 2; }             // of 64 dimensions, 128 rows of 128 bytes each
 template <int NB> constexpr int row_tile() { return slabs<NB>() * 16384; }    // 128 rows of Q or of K
 template <int NB> constexpr int v_tile() { return NB * 32 * 256; }            // dk rows of 128 keys, two slabs of 64 keys
-template <int NB> constexpr int raw_bytes() { return 4 * 18 * 32 * NB; }
 template <int NB> constexpr int smem_bytes() {
-    return 2 * row_tile<NB>() + KV_STAGES * (row_tile<NB>() + v_tile<NB>()) + RAW_STAGES * raw_bytes<NB>() + 1024;
+    return 2 * row_tile<NB>() + KV_STAGES * (row_tile<NB>() + v_tile<NB>()) + 1024;
 }
 
 struct Bars {
-    uint64_t raw_full[RAW_STAGES], raw_empty[RAW_STAGES];
     uint64_t k_full[KV_STAGES], k_empty[KV_STAGES], v_full[KV_STAGES], v_empty[KV_STAGES];
     uint64_t s_full[2], p_full[2], o_full[2], drain;
 };
 
-// D[tmem] (+)= A[tmem] B[smem]^T, a K step of 16, issued by one thread
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp. The issuing warp runs its loop as a whole
+// and only the products and commits are this lane's: what they take then
+// stays in uniform registers ([ISSUE] a step where a single thread ran it).
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(is));
+    return is;
+}
+
+// D[tmem] (+)= A B[smem]^T, a K step of 16: A in shared memory (a descriptor) or in TMEM
+__device__ __forceinline__ void mma_ss(uint32_t me, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(me)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t me, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(me)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t me, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(me)
         : "memory");
 }
 
@@ -88,9 +114,9 @@ __device__ __forceinline__ Span span_of(const Attn4Args& a, const Entry& e, uint
     return {lo < 0 ? 0 : lo, hi < 0 ? 0 : hi > e.len ? e.len : hi};
 }
 
-// NB words from shared memory, as wide as they lie
+// N words of memory, as wide as they lie
 template <int N>
-__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
@@ -106,78 +132,97 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
     }
 }
 
-// K of a unit (16 keys) into 16 rows of a tile from `rows` on. A lane has the
-// words of keys g and g + 8: eight values of a block, a 16-byte chunk. Lanes
-// of odd g take a pair of blocks the other way round, so that the eight
-// lanes of a store's quarter meet eight different banks.
+// A lane's codes and scales of a unit's K: keys g and g + 8
 template <int NB>
-__device__ __forceinline__ void write_k(const uint8_t* unit, uint8_t* rows) {
-    constexpr int DK = NB * 32, PAIRED = NB / 2 * 2;
-    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3, odd = g & 1;
-    uint8_t* const even_at = rows + g * 128 + (((4 * odd + t) ^ g) << 4);        // of the pair's block taken first
-    uint8_t* const odd_at = rows + g * 128 + (((4 * (odd ^ 1) + t) ^ g) << 4);   // and second
-    uint8_t* const last_at = rows + g * 128 + ((t ^ g) << 4);                    // of a block without a pair
+struct KCodes {
+    uint32_t w[2][NB], s[2][(NB + 1) / 2];
+    __device__ __forceinline__ void load(const uint8_t* unit) {
+        const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-        uint32_t w[NB], sc[(NB + 1) / 2];
-        lds<NB>(unit + ((g + 8 * r) * 4 + t) * NB * 4, w);
-        if constexpr (NB % 2 == 0) {
-            lds<NB / 2>(unit + 16 * DK + (g + 8 * r) * NB * 2, sc);
-        } else {
+        for (int r = 0; r < 2; r++) {
+            load_words<NB>(unit + ((g + 8 * r) * 4 + t) * NB * 4, w[r]);
+            const uint8_t* at = unit + 16 * 32 * NB + (g + 8 * r) * NB * 2;
+            if constexpr (NB % 2 == 0) {
+                load_words<NB / 2>(at, s[r]);
+            } else {
 #pragma unroll
-            for (int b = 0; b < NB; b += 2) {
-                const uint16_t* at = reinterpret_cast<const uint16_t*>(unit + 16 * DK + (g + 8 * r) * NB * 2) + b;
-                sc[b / 2] = at[0];
-                if (b + 1 < NB) sc[b / 2] |= static_cast<uint32_t>(at[1]) << 16;
+                for (int b = 0; b < NB; b += 2) {
+                    s[r][b / 2] = reinterpret_cast<const uint16_t*>(at)[b];
+                    if (b + 1 < NB) s[r][b / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(at)[b + 1]) << 16;
+                }
             }
         }
+    }
+    // Into 16 rows of a tile from `rows` on: eight values of a block are a
+    // 16-byte chunk. Lanes of odd g take a pair of blocks the other way
+    // round, so that the eight lanes of a store's quarter meet eight
+    // different banks.
+    __device__ __forceinline__ void store(uint8_t* rows) const {
+        constexpr int PAIRED = NB / 2 * 2;
+        const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3, odd = g & 1;
+        uint8_t* const first_at = rows + g * 128 + (((4 * odd + t) ^ g) << 4);         // of the pair's block taken first
+        uint8_t* const second_at = rows + g * 128 + (((4 * (odd ^ 1) + t) ^ g) << 4);  // and second
+        uint8_t* const last_at = rows + g * 128 + ((t ^ g) << 4);                      // of a block without a pair
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const bool pair = b < PAIRED;
+                const uint32_t x = pair && odd ? w[r][pair ? b ^ 1 : b] : w[r][b];
+                // the block's scale in both halves: the low or the high one of its pair's word
+                const uint32_t s2 = __byte_perm(s[r][b / 2], 0, pair && odd ? (b % 2 ? 0x1010 : 0x3232) : (b % 2 ? 0x3232 : 0x1010)), ms = c4_m24(s2);
+                const uint4 v = make_uint4(c4_pair<0>(x, s2, ms), c4_pair<1>(x, s2, ms), c4_pair<2>(x, s2, ms), c4_pair<3>(x, s2, ms));
+                *reinterpret_cast<uint4*>((!pair ? last_at : b % 2 ? second_at : first_at) + b / 2 * 16384 + r * 1024) = v;
+            }
+    }
+};
+
+// The same of its V: dimensions g, g + 8, .. of keys 2t, 2t + 1, 8 + 2t, 9 + 2t
+template <int NB>
+struct VCodes {
+    uint2 w[NB];
+    uint32_t s[NB][2];
+    __device__ __forceinline__ void load(const uint8_t* unit) {
+        constexpr int DK = NB * 32;
+        const uint32_t lane = threadIdx.x & 31, t = lane & 3;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const bool pair = b < PAIRED;
-            const uint32_t x = pair && odd ? w[pair ? b ^ 1 : b] : w[b];
-            // the block's scale in both halves: the low or the high one of its pair's word
-            const uint32_t s2 = __byte_perm(sc[b / 2], 0, pair && odd ? (b % 2 ? 0x1010 : 0x3232) : (b % 2 ? 0x3232 : 0x1010)), ms = c4_m24(s2);
-            const uint4 v = make_uint4(c4_pair<0>(x, s2, ms), c4_pair<1>(x, s2, ms), c4_pair<2>(x, s2, ms), c4_pair<3>(x, s2, ms));
-            *reinterpret_cast<uint4*>((!pair ? last_at : b % 2 ? odd_at : even_at) + b / 2 * 16384 + r * 1024) = v;
+            w[b] = *reinterpret_cast<const uint2*>(unit + 8 * DK + (b * 32 + lane) * 8);
+#pragma unroll
+            for (int c = 0; c < 2; c++) s[b][c] = *reinterpret_cast<const uint32_t*>(unit + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
         }
     }
-}
-
-// V of a unit into 16 columns of a slab of 64 keys (quarter 0 .. 3 of it): a
-// lane's pairs of keys go to rows of dimensions 8 apart. Keys from `limit` on
-// become zeros: what lies there may be anything.
-template <int NB>
-__device__ __forceinline__ void write_v(const uint8_t* unit, uint8_t* slab, uint32_t quarter, int32_t key0, int32_t limit) {
-    constexpr int DK = NB * 32;
-    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
-    const bool edge = key0 + C4_UNIT > limit;
-    uint8_t* const lo_at = slab + g * 128 + 4 * t + (((2 * quarter) ^ g) << 4);       // keys 2t, 2t + 1
-    uint8_t* const hi_at = slab + g * 128 + 4 * t + (((2 * quarter + 1) ^ g) << 4);   // keys 8 + 2t, 9 + 2t
+    // Into 16 columns of a slab of 64 keys (quarter 0 .. 3 of it). Keys from
+    // `left` on become zeros: what lies there may be anything.
+    __device__ __forceinline__ void store(uint8_t* slab, uint32_t quarter, int32_t left) const {
+        const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+        uint8_t* const lo_at = slab + g * 128 + 4 * t + (((2 * quarter) ^ g) << 4);      // keys 2t, 2t + 1
+        uint8_t* const hi_at = slab + g * 128 + 4 * t + (((2 * quarter + 1) ^ g) << 4);  // keys 8 + 2t, 9 + 2t
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-        const uint2 w = *reinterpret_cast<const uint2*>(unit + 8 * DK + ((b * 8 + g) * 4 + t) * 8);
-        uint32_t s2[2], ms[2];
+        for (int b = 0; b < NB; b++) {
+            uint32_t s2[2], ms[2];
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            s2[c] = *reinterpret_cast<const uint32_t*>(unit + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
-            if (edge) {
-                const int32_t key = key0 + 8 * c + 2 * static_cast<int32_t>(t);
-                if (key >= limit) s2[c] = 0;
-                else if (key + 1 >= limit) s2[c] &= 0xFFFFu;
+            for (int c = 0; c < 2; c++) {
+                s2[c] = s[b][c];
+                if (left < C4_UNIT) {
+                    const int32_t key = 8 * c + 2 * static_cast<int32_t>(t);
+                    if (key >= left) s2[c] = 0;
+                    else if (key + 1 >= left) s2[c] &= 0xFFFFu;
+                }
+                ms[c] = c4_m24(s2[c]);
             }
-            ms[c] = c4_m24(s2[c]);
-        }
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const uint32_t x = j ? w.y : w.x;
-            const int at = (32 * b + 16 * j) * 128;  // dimensions 32 b + 16 j + g, and 8 on
-            *reinterpret_cast<uint32_t*>(lo_at + at) = c4_pair<0>(x, s2[0], ms[0]);
-            *reinterpret_cast<uint32_t*>(lo_at + at + 1024) = c4_pair<1>(x, s2[0], ms[0]);
-            *reinterpret_cast<uint32_t*>(hi_at + at) = c4_pair<2>(x, s2[1], ms[1]);
-            *reinterpret_cast<uint32_t*>(hi_at + at + 1024) = c4_pair<3>(x, s2[1], ms[1]);
+            for (int j = 0; j < 2; j++) {
+                const uint32_t x = j ? w[b].y : w[b].x;
+                const int at = (32 * b + 16 * j) * 128;  // dimensions 32 b + 16 j + g, and 8 on
+                *reinterpret_cast<uint32_t*>(lo_at + at) = c4_pair<0>(x, s2[0], ms[0]);
+                *reinterpret_cast<uint32_t*>(lo_at + at + 1024) = c4_pair<1>(x, s2[0], ms[0]);
+                *reinterpret_cast<uint32_t*>(hi_at + at) = c4_pair<2>(x, s2[1], ms[1]);
+                *reinterpret_cast<uint32_t*>(hi_at + at + 1024) = c4_pair<3>(x, s2[1], ms[1]);
+            }
         }
     }
-}
+};
 
 // The largest of three
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -187,8 +232,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // P of 32 columns: 2^(s scale + minus), its sum into two running ones, rounded
-// to bf16 and put into 16 TMEM columns. Columns outside [first, end) are 0.
-template <bool MASK>
+// to bf16 and put into 16 TMEM columns. Columns from `end` on (MASK 1, 2) and
+// those before `first` (2) are 0.
+template <int MASK>
 __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t minus2, int32_t first, int32_t end, uint64_t (&sum)[2],
                                         uint32_t to) {
     uint32_t z[16];
@@ -198,10 +244,8 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t scale2
         unpack2(fma2_r<0>(pack2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), scale2, minus2), p0, p1);
         p0 = exp2_fast(p0);
         p1 = exp2_fast(p1);
-        if constexpr (MASK) {
-            p0 = 2 * x >= first && 2 * x < end ? p0 : 0.0f;
-            p1 = 2 * x + 1 >= first && 2 * x + 1 < end ? p1 : 0.0f;
-        }
+        if constexpr (MASK >= 1) p0 = 2 * x < end ? p0 : 0.0f, p1 = 2 * x + 1 < end ? p1 : 0.0f;
+        if constexpr (MASK == 2) p0 = 2 * x >= first ? p0 : 0.0f, p1 = 2 * x + 1 >= first ? p1 : 0.0f;
         sum[x & 1] = add2_rn(sum[x & 1], pack2(p0, p1));
         z[x] = bf16_pair(p0, p1);
     }
@@ -209,7 +253,7 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t scale2
 }
 
 // The largest of 32 columns of S and `top`
-template <bool MASK>
+template <int MASK>
 __device__ __forceinline__ float largest(const uint32_t (&s)[32], int32_t first, int32_t end, float top) {
     float other = NEG_INF;
 #pragma unroll
@@ -218,7 +262,8 @@ __device__ __forceinline__ float largest(const uint32_t (&s)[32], int32_t first,
 #pragma unroll
         for (int y = 0; y < 4; y++) {
             v[y] = __uint_as_float(s[x + y]);
-            if constexpr (MASK) v[y] = x + y >= first && x + y < end ? v[y] : NEG_INF;
+            if constexpr (MASK >= 1) v[y] = x + y < end ? v[y] : NEG_INF;
+            if constexpr (MASK == 2) v[y] = x + y >= first ? v[y] : NEG_INF;
         }
         top = max3(top, v[0], v[1]);
         other = max3(other, v[2], v[3]);
@@ -229,7 +274,7 @@ __device__ __forceinline__ float largest(const uint32_t (&s)[32], int32_t first,
 // A step of a row: its 128 scores at s_at become P in the upper half of their
 // place. Half of the scores are kept from the search for the maximum, the
 // other half is read again.
-template <int NB, bool MASK>
+template <int NB, int MASK>
 __device__ __forceinline__ void softmax_step(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l) {
     uint32_t a[32], b[32], c[32];
     tmem_ld_32x32b_x32(s_at, a);
@@ -293,10 +338,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     uint8_t* q_tile = smem;
     uint8_t* k_tile = q_tile + 2 * row_tile<NB>();
     uint8_t* v_tiles = k_tile + KV_STAGES * row_tile<NB>();
-    uint8_t* raw = v_tiles + KV_STAGES * v_tile<NB>();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
     if (tid == 0) {
-        for (int i = 0; i < RAW_STAGES; i++) mbar_init(&bars.raw_full[i], 1), mbar_init(&bars.raw_empty[i], CODE_WARPS);
         for (int i = 0; i < KV_STAGES; i++) {
             mbar_init(&bars.k_full[i], CODE_WARPS), mbar_init(&bars.v_full[i], CODE_WARPS);
             mbar_init(&bars.k_empty[i], 1), mbar_init(&bars.v_empty[i], 1);
@@ -333,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(e.r0 + tok) * a.qs +
                                      static_cast<size_t>(h * a.G + row - tok * a.G) * DK + 8 * chunk;
             if (a.vec) {
-                v = __ldg(reinterpret_cast<const uint4*>(p));
+                v = *reinterpret_cast<const uint4*>(p);
             } else {
                 alignas(16) __nv_bfloat16 y[8];
 #pragma unroll
@@ -348,128 +391,135 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    constexpr uint32_t tmem = 0;  // where an allocation of all 512 columns begins
 
-    if (warp == FETCH_WARP) {
-        set_registers<ISSUE_REGS, false>();
-        // a lane a unit of the half step
-        const uint32_t per = a.c.pshift - 4, halves = (units + 3) / 4;
-        const int32_t* table = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
-        const uint8_t* head = a.c.pages + a.layer * a.c.layer_bytes + h * a.c.head_bytes;
-        int32_t page = lane < 4 && lane < units ? table[(unit0 + lane) >> per] : 0;
-        uint32_t issued = 0;
-        for (uint32_t i = 0; i < halves; i++, issued++) {
-            const int st = i % RAW_STAGES;
-            if (!warp_wait(&bars.raw_empty[st], (i / RAW_STAGES & 1) ^ 1, &gave_up, a.timeout)) {
-                gave_up = 1;
-                if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
-                break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&bars.raw_full[st], min(4u, units - 4 * i) * 18 * DK);
-            __syncwarp();
-            const uint32_t u = 4 * i + lane, unit = unit0 + u;
-            if (lane < 4 && u < units) {
-                if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
-                    atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
-                    page = 0;
-                }
-                bulk_load(raw + st * raw_bytes<NB>() + lane * 18 * DK,
-                          head + static_cast<uint32_t>(page) * a.c.page_bytes + (unit & ((1u << per) - 1)) * (18 * DK), 18 * DK, &bars.raw_full[st]);
-                if (u + 4 < units) page = table[(unit + 4) >> per];
-            }
-        }
-        // whatever the others did, the copies in flight land before the block leaves its memory
-        for (uint32_t i = issued < RAW_STAGES ? 0 : issued - RAW_STAGES; i < issued; i++)
-            mbar_drain(&bars.raw_full[i % RAW_STAGES], i / RAW_STAGES & 1, a.timeout);
-    } else if (warp > FETCH_WARP) {
+    if (warp > MMA_WARP) {
         set_registers<ISSUE_REGS, false>();
     } else if (warp == MMA_WARP) {
         set_registers<ISSUE_REGS, false>();
-        if (lane == 0 && steps) {
-            const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_tile), v_at = smem_u32(v_tiles);
-            constexpr uint32_t QK = bf16_instr_desc(128, KEYS), PV = bf16_instr_desc(128, DK);
-            bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity) {
-                ok = ok && mbar_wait(bar, parity, &gave_up, a.timeout);
-                if (ok) tc_fence_after();
-                return ok;
-            };
-            auto scores = [&](uint32_t t, uint32_t i) {
-                const uint32_t qa = q_at + t * row_tile<NB>(), ka = k_at + i % KV_STAGES * row_tile<NB>();
+        // descriptors hold addresses in units of 16 bytes, in their low bits
+        const uint64_t q_at = sw128_kmajor_desc(smem_u32(q_tile)), k_at = sw128_kmajor_desc(smem_u32(k_tile)),
+                       v_at = sw128_kmajor_desc(smem_u32(v_tiles));
+        constexpr uint32_t QK = bf16_instr_desc(128, KEYS), PV = bf16_instr_desc(128, DK);
+        const uint32_t me = elected();
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            ok = ok && warp_wait(bar, parity, &gave_up, a.timeout);
+            if (ok) tc_fence_after();
+            return ok;
+        };
+        auto scores = [&](uint32_t t, uint32_t i) {
+            const uint64_t qd = q_at + t * (row_tile<NB>() / 16), kd = k_at + i % KV_STAGES * (row_tile<NB>() / 16);
 #pragma unroll
-                for (int k = 0; k < DK / 16; k++)
-                    umma_bf16(tmem + S_COL + 128 * t, sw128_kmajor_desc(qa + k / 4 * 16384 + k % 4 * 32),
-                              sw128_kmajor_desc(ka + k / 4 * 16384 + k % 4 * 32), QK, k > 0);
-                umma_commit(&bars.s_full[t]);
-            };
-            auto values = [&](uint32_t t, uint32_t i) {
-                const uint32_t va = v_at + i % KV_STAGES * v_tile<NB>();
+            for (int k = 0; k < DK / 16; k++)
+                mma_ss(me, S_COL + 128 * t, qd + k / 4 * 1024 + k % 4 * 2, kd + k / 4 * 1024 + k % 4 * 2, QK, k > 0);
+            commit(me, &bars.s_full[t]);
+        };
+        auto values = [&](uint32_t t, uint32_t i) {
+            const uint64_t vd = v_at + i % KV_STAGES * (v_tile<NB>() / 16);
 #pragma unroll
-                for (int k = 0; k < KEYS / 16; k++)
-                    umma_bf16_ts(tmem + O_COL + 128 * t, tmem + S_COL + 128 * t + 64 + 8 * k, sw128_kmajor_desc(va + k / 4 * (DK * 128) + k % 4 * 32), PV,
-                                 i > 0 || k > 0);
-            };
-            if (wait(&bars.k_full[0], 0)) {
-                for (uint32_t t = 0; t < tiles; t++) scores(t, 0);
-                umma_commit(&bars.k_empty[0]);
-            }
-            // a tile's next scores follow its values: they take P's place in
-            // TMEM, and products of one thread run in their order
-            for (uint32_t i = 0; ok && i < steps; i++) {
-                const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1, st1 = (i + 1) % KV_STAGES, ph1 = (i + 1) / KV_STAGES & 1;
-                const bool more = i + 1 < steps;
-                if (!wait(&bars.v_full[st], ph)) break;
-                for (uint32_t t = 0; t < tiles; t++) {
-                    if (!wait(&bars.p_full[t], i & 1)) break;
-                    values(t, i);
-                    if (t + 1 == tiles) umma_commit(&bars.v_empty[st]);
-                    if (!more) {
-                        umma_commit(&bars.o_full[t]);
-                    } else {
-                        if (t == 0 && !wait(&bars.k_full[st1], ph1)) break;
-                        scores(t, i + 1);
-                        if (t + 1 == tiles) umma_commit(&bars.k_empty[st1]);
-                    }
+            for (int k = 0; k < KEYS / 16; k++)
+                mma_ts(me, O_COL + 128 * t, S_COL + 128 * t + 64 + 8 * k, vd + k / 4 * (DK * 8) + k % 4 * 2, PV, i > 0 || k > 0);
+        };
+        if (steps && wait(&bars.k_full[0], 0)) {
+            for (uint32_t t = 0; t < tiles; t++) scores(t, 0);
+            commit(me, &bars.k_empty[0]);
+        }
+        // a tile's next scores follow its values: they take P's place in
+        // TMEM, and products of one thread run in their order
+        for (uint32_t i = 0; ok && i < steps; i++) {
+            const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1, st1 = (i + 1) % KV_STAGES, ph1 = (i + 1) / KV_STAGES & 1;
+            const bool more = i + 1 < steps;
+            if (!wait(&bars.v_full[st], ph)) break;
+            for (uint32_t t = 0; t < tiles; t++) {
+                if (!wait(&bars.p_full[t], i & 1)) break;
+                values(t, i);
+                if (t + 1 == tiles) commit(me, &bars.v_empty[st]);
+                if (!more) {
+                    commit(me, &bars.o_full[t]);
+                } else {
+                    if (t == 0 && !wait(&bars.k_full[st1], ph1)) break;
+                    scores(t, i + 1);
+                    if (t + 1 == tiles) commit(me, &bars.k_empty[st1]);
                 }
             }
-            if (!ok) {
-                gave_up = 1;
-                atomicOr(a.err, PKB_DEVERR_TIMEOUT);
-                // what this thread issued finishes before TMEM is freed
-                umma_commit(&bars.drain);
-                mbar_drain(&bars.drain, 0, a.timeout);
-            }
+        }
+        if (!ok) {
+            gave_up = 1;
+            if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+            // what was issued finishes before TMEM is freed
+            commit(me, &bars.drain);
+            if (me) mbar_drain(&bars.drain, 0, a.timeout);
+            __syncwarp();
         }
     } else if (warp >= SOFT_WARPS && warp < MMA_WARP) {
-        // codes to values: a warp a unit of each half step
+        // codes to values: a warp takes units w and w + 4 of each step
         set_registers<CODE_REGS, false>();
-        const uint32_t w = warp - SOFT_WARPS;
+        const uint32_t w = warp - SOFT_WARPS, per = a.c.pshift - 4;
+        const int32_t* table = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
+        const uint8_t* head = a.c.pages + a.layer * a.c.layer_bytes + h * a.c.head_bytes;
+        KCodes<NB> k[2];
+        VCodes<NB> v[2];
+        int32_t page[2];  // of the step that is loaded next
+        auto look = [&](uint32_t i) {
+#pragma unroll
+            for (uint32_t half = 0; half < 2; half++) {
+                const uint32_t u = 8 * i + 4 * half + w;
+                page[half] = u < units ? table[(unit0 + u) >> per] : 0;
+            }
+        };
+        // where a unit lies; past the last one any codes will do, they become zeros or are hidden
+        auto unit_at = [&](uint32_t i, uint32_t half) {
+            uint32_t p = static_cast<uint32_t>(page[half]);
+            if (p >= a.c.n_pages) {
+                if (lane == 0) atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
+                p = 0;
+            }
+            const uint32_t u = unit0 + 8 * i + 4 * half + w;
+            return head + p * a.c.page_bytes + (u & ((1u << per) - 1)) * (18 * DK);
+        };
+        const uint8_t* at[2] = {nullptr, nullptr};
+        if (steps) {
+            look(0);
+            for (uint32_t half = 0; half < 2; half++) {
+                at[half] = unit_at(0, half);
+                k[half].load(at[half]);
+                v[half].load(at[half]);
+            }
+            look(1);
+        }
         for (uint32_t i = 0; i < steps; i++) {
             const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1;
-            const uint32_t halves = min(2u, (units - 8 * i + 3) / 4);
-            uint8_t* kt = k_tile + st * row_tile<NB>();
+            uint8_t* kt = k_tile + st * row_tile<NB>() + 16 * w * 128;
             uint8_t* vt = v_tiles + st * v_tile<NB>();
+            const bool more = i + 1 < steps;
             bool ok = warp_wait(&bars.k_empty[st], ph ^ 1, &gave_up, a.timeout);
-            for (uint32_t half = 0; ok && half < halves; half++) {
-                const uint32_t ri = 2 * i + half;
-                ok = warp_wait(&bars.raw_full[ri % RAW_STAGES], ri / RAW_STAGES & 1, &gave_up, a.timeout);
-                if (ok) write_k<NB>(raw + ri % RAW_STAGES * raw_bytes<NB>() + w * 18 * DK, kt + (64 * half + 16 * w) * 128);
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(&bars.k_full[st]);
-            ok = ok && warp_wait(&bars.v_empty[st], ph ^ 1, &gave_up, a.timeout);
-            for (uint32_t half = 0; ok && half < 2; half++) {
-                const uint32_t ri = 2 * i + half;
-                // a half step past the last unit is zeros too: any codes will do
-                write_v<NB>(raw + ri % RAW_STAGES * raw_bytes<NB>() + w * 18 * DK, vt + half * (DK * 128), w,
-                            key_base + static_cast<int32_t>(i * KEYS + 64 * half + 16 * w), half < halves ? static_cast<int32_t>(hi) : INT_MIN);
+            if (ok) {
+#pragma unroll
+                for (uint32_t half = 0; half < 2; half++) {
+                    k[half].store(kt + half * (64 * 128));
+                    if (more) {
+                        at[half] = unit_at(i + 1, half);
+                        k[half].load(at[half]);
+                    }
+                }
+                if (more) look(i + 2);
+                fence_async_smem();
                 __syncwarp();
-                if (half < halves && lane == 0) mbar_arrive(&bars.raw_empty[ri % RAW_STAGES]);
+                if (lane == 0) mbar_arrive(&bars.k_full[st]);
+                ok = warp_wait(&bars.v_empty[st], ph ^ 1, &gave_up, a.timeout);
             }
-            fence_async_smem();
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(&bars.v_full[st]);
+            if (ok) {
+#pragma unroll
+                for (uint32_t half = 0; half < 2; half++) {
+                    const int64_t left = hi - key_base - static_cast<int64_t>(i * KEYS + 64 * half + 16 * w);
+                    v[half].store(vt + half * (DK * 128), w, static_cast<int32_t>(left < 0 ? 0 : left < C4_UNIT ? left : C4_UNIT));
+                    if (more) v[half].load(at[half]);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.v_full[st]);
+            }
             if (!ok) {
                 gave_up = 1;
                 if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
@@ -480,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         // the rows: thread i of a tile's four warps has row i
         set_registers<SOFT_REGS, true>();
         const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
-        const Span span = row < all ? span_of(a, e, tok) : Span{0, 0};
+        const Span span = span_of(a, e, min(tok, e.rows - 1));  // rows there are none of see what the last one does
         const uint32_t at = tmem + ((warp % 4) * 32 << 16), s_at = at + S_COL + 128 * t, o_at = at + O_COL + 128 * t;
         const float scale = fmaxf(fabsf(a.scale), 1e-37f);  // of a scale 0 too
         float m = NEG_INF, l = 0.0f;
@@ -492,9 +542,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             const int64_t key0 = static_cast<int64_t>(key_base) + i * KEYS;
             const int32_t first = static_cast<int32_t>(max(min(span.lo - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
             const int32_t end = static_cast<int32_t>(max(min(span.hi - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
-            const bool mask = __any_sync(FULL, first > 0 || end < KEYS);
-            if (mask) softmax_step<NB, true>(s_at, o_at, i > 0, scale, first, end, m, l);
-            else softmax_step<NB, false>(s_at, o_at, i > 0, scale, 0, KEYS, m, l);
+            const bool before = __any_sync(FULL, first > 0), behind = __any_sync(FULL, end < KEYS);
+            if (before) softmax_step<NB, 2>(s_at, o_at, i > 0, scale, first, end, m, l);
+            else if (behind) softmax_step<NB, 1>(s_at, o_at, i > 0, scale, 0, end, m, l);
+            else softmax_step<NB, 0>(s_at, o_at, i > 0, scale, 0, KEYS, m, l);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.p_full[t]);
@@ -541,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     __syncthreads();
     if (warp == MMA_WARP) {
         tc_fence_after();
-        tmem_dealloc(tmem, TMEM_COLS);
+        tmem_dealloc(tmem_slot, TMEM_COLS);
     }
 }
 

@@ -104,7 +104,7 @@ __device__ __forceinline__ void c4_load8(const T* p, float (&x)[8]) {
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; i++)
-            reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = p[i];
