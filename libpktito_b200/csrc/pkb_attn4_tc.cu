@@ -10,7 +10,7 @@
 // runs: 2 x (128 x 128 x dk) products each for S and O against 2 x 16,384
 // powers of two a step, some 2,048 cycles of either at dk 128.
 //
-// Four warps turn K's and V's codes into the bf16 values that they stand for
+// Eight warps turn K's and V's codes into the bf16 values that they stand for
 // (exactly: pkb_cache4.cuh) in the 128-byte swizzled tiles that the tensor
 // cores read: K as [keys][dk], V as [dk][keys], which is how a lane's codes
 // lie in the cache, in stores without bank conflicts. They load the codes a
@@ -33,11 +33,12 @@ namespace pkb {
 namespace {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
-constexpr int SOFT_WARPS = 8, CODE_WARPS = 4, MMA_WARP = SOFT_WARPS + CODE_WARPS;
-constexpr int THREADS = 512;    // four warpgroups; the last one's three spare warps wait for the end
-// A thread's registers: 65,536 / 512 at launch, then the rows' warps take
-// what the others leave: 256 x 168 + 128 x 120 + 128 x 48 = 64,512.
-constexpr int SOFT_REGS = 168, CODE_REGS = 120, ISSUE_REGS = 48;
+constexpr int SOFT_WARPS = 8, CODE_WARPS = 8, MMA_WARP = SOFT_WARPS + CODE_WARPS;
+constexpr int THREADS = 640;    // five warpgroups; the last one's three spare warps wait for the end
+// A thread's registers: 96 at launch (61,440 of the SM's 65,536), then the
+// rows' warps take what the others leave: 256 x 152 + 256 x 64 + 128 x 40 =
+// 60,416.
+constexpr int SOFT_REGS = 152, CODE_REGS = 64, ISSUE_REGS = 40;
 constexpr int ROWS = 256;       // of a block, two tiles of 128
 constexpr int KEYS = 128;       // of a step
 constexpr int KV_STAGES = 2;    // steps of K and of V as bf16
@@ -57,7 +58,8 @@ struct Bars {
 
 // One lane of a converged warp. The issuing warp runs its loop as a whole
 // and only the products and commits are this lane's: what they take then
-// stays in uniform registers ([ISSUE] a step where a single thread ran it).
+// stays in uniform registers (1.42 -> 1.25 ms for two prompts of 8,191
+// tokens, a single thread's loop against this one).
 __device__ __forceinline__ uint32_t elected() {
     uint32_t is;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(is));
@@ -232,15 +234,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // P of 32 columns: 2^(s scale + minus), its sum into two running ones, rounded
-// to bf16 and put into 16 TMEM columns. Columns from `end` on (MASK 1, 2) and
-// those before `first` (2) are 0.
+// to bf16, and the largest score beside it. Columns from `end` on (MASK 1, 2) and those before `first` (2) are 0.
 template <int MASK>
 __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t minus2, int32_t first, int32_t end, uint64_t (&sum)[2],
-                                        uint32_t to) {
-    uint32_t z[16];
+                                        uint32_t (&z)[16], float& top) {
 #pragma unroll
     for (int x = 0; x < 16; x++) {
-        float p0, p1;
+        float p0, p1, s0 = __uint_as_float(s[2 * x]), s1 = __uint_as_float(s[2 * x + 1]);
+        if constexpr (MASK >= 1) s0 = 2 * x < end ? s0 : NEG_INF, s1 = 2 * x + 1 < end ? s1 : NEG_INF;
+        if constexpr (MASK == 2) s0 = 2 * x >= first ? s0 : NEG_INF, s1 = 2 * x + 1 >= first ? s1 : NEG_INF;
+        top = max3(top, s0, s1);
         unpack2(fma2_r<0>(pack2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), scale2, minus2), p0, p1);
         p0 = exp2_fast(p0);
         p1 = exp2_fast(p1);
@@ -249,7 +252,6 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t scale2
         sum[x & 1] = add2_rn(sum[x & 1], pack2(p0, p1));
         z[x] = bf16_pair(p0, p1);
     }
-    tmem_st_x16(to, z);
 }
 
 // The largest of 32 columns of S and `top`
@@ -271,54 +273,78 @@ __device__ __forceinline__ float largest(const uint32_t (&s)[32], int32_t first,
     return fmaxf(top, other);
 }
 
+// Raises a row's maximum to that of its 128 scores at s_at, and rescales its
+// sum and its values (those of the steps before: the scores' commit covers
+// them).
+template <int NB, int MASK>
+__device__ __noinline__ void raise(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l) {
+    float top = NEG_INF;
+#pragma unroll 1
+    for (int c = 0; c < 4; c++) {
+        uint32_t a[32];
+        tmem_ld_32x32b_x32(s_at + 32 * c, a);
+        tmem_ld_wait(a);
+        top = largest<MASK>(a, first - 32 * c, end - 32 * c, top);
+    }
+    const float raised = fmaxf(m, __fmul_rn(top, scale)), f = rescale(m, raised);
+    m = raised;
+    l *= f;
+#pragma unroll 1
+    for (int d = 0; begun && d < 2 * NB; d++) {
+        uint32_t y[16];
+        tmem_ld_32x32b_x16(o_at + 16 * d, y);
+        tmem_ld_wait(y);
+#pragma unroll
+        for (int x = 0; x < 16; x++) y[x] = __float_as_uint(__fmul_rn(__uint_as_float(y[x]), f));
+        tmem_st_x16(o_at + 16 * d, y);
+    }
+    tmem_st_wait();
+}
+
 // A step of a row: its 128 scores at s_at become P in the upper half of their
-// place. Half of the scores are kept from the search for the maximum, the
-// other half is read again.
+// place. The weights are taken with the maximum there is, while the scores'
+// own is looked for; where that passes it by 8 (the first step, and few
+// others) the maximum is raised and they are taken again: nothing of S is
+// overwritten before its last columns have been seen.
 template <int NB, int MASK>
 __device__ __forceinline__ void softmax_step(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l) {
-    uint32_t a[32], b[32], c[32];
-    tmem_ld_32x32b_x32(s_at, a);
-    tmem_ld_wait(a);
-    tmem_ld_32x32b_x32(s_at + 32, b);
-    float top = largest<MASK>(a, first, end, NEG_INF);
-    tmem_ld_wait(b);
-    tmem_ld_32x32b_x32(s_at + 64, a);
-    tmem_ld_32x32b_x32(s_at + 96, c);
-    top = largest<MASK>(b, first - 32, end - 32, top);
-    tmem_ld_wait(a);
-    tmem_ld_settled(c);
-    top = largest<MASK>(a, first - 64, end - 64, top);
-    top = __fmul_rn(largest<MASK>(c, first - 96, end - 96, top), scale);
-    if (__any_sync(FULL, top > m + 8.0f)) {
-        const float raised = fmaxf(m, top), f = rescale(m, raised);
-        m = raised;
-        l *= f;
-        // the values of the step before are in O: its scores' commit covers them
-        for (int d = 0; begun && d < 2 * NB; d++) {
-            uint32_t y[16];
-            tmem_ld_32x32b_x16(o_at + 16 * d, y);
-            tmem_ld_wait(y);
-#pragma unroll
-            for (int x = 0; x < 16; x++) y[x] = __float_as_uint(__fmul_rn(__uint_as_float(y[x]), f));
-            tmem_st_x16(o_at + 16 * d, y);
+    const uint64_t scale2 = pack2(scale, scale);
+    if (!begun) raise<NB, MASK>(s_at, o_at, begun, scale, first, end, m, l);
+    for (;;) {
+        uint32_t a[32], b[32], z0[16], z1[16], z2[16];
+        const float minus = m == NEG_INF ? 0.0f : -m;
+        const uint64_t minus2 = pack2(minus, minus);
+        uint64_t sum[2] = {0, 0};
+        tmem_ld_32x32b_x32(s_at, a);
+        tmem_ld_wait(a);
+        tmem_ld_32x32b_x32(s_at + 32, b);
+        float top = NEG_INF;
+        weights<MASK>(a, scale2, minus2, first, end, sum, z0, top);
+        tmem_ld_wait(b);
+        tmem_ld_32x32b_x32(s_at + 64, a);
+        weights<MASK>(b, scale2, minus2, first - 32, end - 32, sum, z1, top);
+        tmem_ld_wait(a);
+        tmem_ld_32x32b_x32(s_at + 96, b);
+        weights<MASK>(a, scale2, minus2, first - 64, end - 64, sum, z2, top);
+        tmem_ld_wait(b);
+        top = largest<MASK>(b, first - 96, end - 96, top);
+        if (__any_sync(FULL, __fmul_rn(top, scale) > m + 8.0f)) {
+            raise<NB, MASK>(s_at, o_at, begun, scale, first, end, m, l);
+            continue;
         }
+        tmem_st_x16(s_at + 64, z0);
+        tmem_st_x16(s_at + 80, z1);
+        tmem_st_x16(s_at + 96, z2);
+        float seen = top;
+        weights<MASK>(b, scale2, minus2, first - 96, end - 96, sum, z0, seen);
+        tmem_st_x16(s_at + 112, z0);
+        float s0, s1, s2, s3;
+        unpack2(sum[0], s0, s1);
+        unpack2(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
+        tmem_st_wait();
+        break;
     }
-    const float minus = m == NEG_INF ? 0.0f : -m;
-    const uint64_t scale2 = pack2(scale, scale), minus2 = pack2(minus, minus);
-    uint64_t sum[2] = {0, 0};
-    tmem_ld_32x32b_x32(s_at, b);
-    weights<MASK>(a, scale2, minus2, first - 64, end - 64, sum, s_at + 96);
-    weights<MASK>(c, scale2, minus2, first - 96, end - 96, sum, s_at + 112);
-    tmem_ld_wait(b);
-    tmem_ld_32x32b_x32(s_at + 32, a);
-    weights<MASK>(b, scale2, minus2, first, end, sum, s_at + 64);
-    tmem_ld_wait(a);
-    weights<MASK>(a, scale2, minus2, first - 32, end - 32, sum, s_at + 80);
-    float s0, s1, s2, s3;
-    unpack2(sum[0], s0, s1);
-    unpack2(sum[1], s2, s3);
-    l += (s0 + s1) + (s2 + s3);
-    tmem_st_wait();
 }
 
 template <int REGS, bool MORE>
@@ -369,23 +395,32 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     }
     // Q, zeros for rows there are none of; a negative scale's sign goes with it
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-    for (uint32_t x = tid; x < tiles * 128 * (DK / 8); x += THREADS) {
-        const uint32_t r = x / (DK / 8), chunk = x % (DK / 8), row = row0 + r, tok = row / a.G;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < all) {
+    constexpr int CHUNKS = (ROWS * (DK / 8) + THREADS - 1) / THREADS;
+    uint4 chunk_of[CHUNKS];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {  // all loads before the first store
+        const uint32_t x = tid + i * THREADS, chunk = x % (DK / 8), row = row0 + x / (DK / 8), tok = row / a.G;
+        chunk_of[i] = make_uint4(0, 0, 0, 0);
+        if (x < ROWS * (DK / 8) && row < all) {
             const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(e.r0 + tok) * a.qs +
                                      static_cast<size_t>(h * a.G + row - tok * a.G) * DK + 8 * chunk;
             if (a.vec) {
-                v = *reinterpret_cast<const uint4*>(p);
+                chunk_of[i] = *reinterpret_cast<const uint4*>(p);
             } else {
                 alignas(16) __nv_bfloat16 y[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = p[i];
-                v = *reinterpret_cast<const uint4*>(y);
+                for (int j = 0; j < 8; j++) y[j] = p[j];
+                chunk_of[i] = *reinterpret_cast<const uint4*>(y);
             }
-            v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
         }
-        *reinterpret_cast<uint4*>(q_tile + (r / 128) * row_tile<NB>() + (chunk / 8) * 16384 + swizzled(r % 128, chunk & 7)) = v;
+    }
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+        const uint32_t x = tid + i * THREADS, chunk = x % (DK / 8), r = x / (DK / 8);
+        const uint4 v = chunk_of[i];
+        if (x < ROWS * (DK / 8))
+            *reinterpret_cast<uint4*>(q_tile + (r / 128) * row_tile<NB>() + (chunk / 8) * 16384 + swizzled(r % 128, chunk & 7)) =
+                make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
     }
     fence_async_smem();
     tc_fence_before();
@@ -453,72 +488,58 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             __syncwarp();
         }
     } else if (warp >= SOFT_WARPS && warp < MMA_WARP) {
-        // codes to values: a warp takes units w and w + 4 of each step
+        // codes to values: a warp a unit of each step
         set_registers<CODE_REGS, false>();
         const uint32_t w = warp - SOFT_WARPS, per = a.c.pshift - 4;
         const int32_t* table = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
         const uint8_t* head = a.c.pages + a.layer * a.c.layer_bytes + h * a.c.head_bytes;
-        KCodes<NB> k[2];
-        VCodes<NB> v[2];
-        int32_t page[2];  // of the step that is loaded next
+        KCodes<NB> k;
+        VCodes<NB> v;
+        int32_t page = 0;  // of the step that is loaded next
         auto look = [&](uint32_t i) {
-#pragma unroll
-            for (uint32_t half = 0; half < 2; half++) {
-                const uint32_t u = 8 * i + 4 * half + w;
-                page[half] = u < units ? table[(unit0 + u) >> per] : 0;
-            }
+            const uint32_t u = 8 * i + w;
+            page = u < units ? table[(unit0 + u) >> per] : 0;
         };
         // where a unit lies; past the last one any codes will do, they become zeros or are hidden
-        auto unit_at = [&](uint32_t i, uint32_t half) {
-            uint32_t p = static_cast<uint32_t>(page[half]);
+        auto unit_at = [&](uint32_t i) {
+            uint32_t p = static_cast<uint32_t>(page);
             if (p >= a.c.n_pages) {
                 if (lane == 0) atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
                 p = 0;
             }
-            const uint32_t u = unit0 + 8 * i + 4 * half + w;
-            return head + p * a.c.page_bytes + (u & ((1u << per) - 1)) * (18 * DK);
+            return head + p * a.c.page_bytes + ((unit0 + 8 * i + w) & ((1u << per) - 1)) * (18 * DK);
         };
-        const uint8_t* at[2] = {nullptr, nullptr};
+        const uint8_t* at = nullptr;
         if (steps) {
             look(0);
-            for (uint32_t half = 0; half < 2; half++) {
-                at[half] = unit_at(0, half);
-                k[half].load(at[half]);
-                v[half].load(at[half]);
-            }
+            at = unit_at(0);
+            k.load(at);
+            v.load(at);
             look(1);
         }
         for (uint32_t i = 0; i < steps; i++) {
             const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1;
-            uint8_t* kt = k_tile + st * row_tile<NB>() + 16 * w * 128;
-            uint8_t* vt = v_tiles + st * v_tile<NB>();
             const bool more = i + 1 < steps;
             bool ok = warp_wait(&bars.k_empty[st], ph ^ 1, &gave_up, a.timeout);
             if (ok) {
-#pragma unroll
-                for (uint32_t half = 0; half < 2; half++) {
-                    k[half].store(kt + half * (64 * 128));
-                    if (more) {
-                        at[half] = unit_at(i + 1, half);
-                        k[half].load(at[half]);
-                    }
-                }
-                if (more) look(i + 2);
+                k.store(k_tile + st * row_tile<NB>() + 16 * w * 128);
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.k_full[st]);
+                if (more) {
+                    at = unit_at(i + 1);
+                    k.load(at);
+                    look(i + 2);
+                }
                 ok = warp_wait(&bars.v_empty[st], ph ^ 1, &gave_up, a.timeout);
             }
             if (ok) {
-#pragma unroll
-                for (uint32_t half = 0; half < 2; half++) {
-                    const int64_t left = hi - key_base - static_cast<int64_t>(i * KEYS + 64 * half + 16 * w);
-                    v[half].store(vt + half * (DK * 128), w, static_cast<int32_t>(left < 0 ? 0 : left < C4_UNIT ? left : C4_UNIT));
-                    if (more) v[half].load(at[half]);
-                }
+                const int64_t left = hi - key_base - static_cast<int64_t>(i * KEYS + 16 * w);
+                v.store(v_tiles + st * v_tile<NB>() + w / 4 * (DK * 128), w % 4, static_cast<int32_t>(left < 0 ? 0 : left < C4_UNIT ? left : C4_UNIT));
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.v_full[st]);
+                if (more) v.load(at);
             }
             if (!ok) {
                 gave_up = 1;
