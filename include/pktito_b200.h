@@ -363,7 +363,7 @@ typedef struct {
     int32_t *table;       /* [max_seqs][max_pages] pages, -1 for none */
     int32_t *lens;        /* [max_seqs] tokens held */
     int32_t *refs;        /* [n_pages] sequences that hold the page */
-    uint32_t n_layers, n_pages, max_seqs, max_pages;
+    uint32_t n_layers, n_pages, max_seqs, max_pages; /* max_pages page_tokens at most 2^30 */
     uint32_t page_tokens; /* 16, 32, 64, 128 or 256 */
     uint32_t n_heads;     /* K/V heads */
     uint32_t head_dim;    /* dk: 32, 64, 96, 128 or 256 */

@@ -18,9 +18,9 @@
 // fetch lies together in a page. All (sequence, team, block of rows) items'
 // tiles are laid end to end and divided evenly over all teams of warps on the
 // GPU, whatever the sequences' lengths: a share begins and ends inside
-// items. One warp a block fetches for the others (bulk copies of whole
-// units, 18 dk bytes, into a ring of each warp's own), so warps never wait
-// for one another. An item that one share has whole is written at once; of
+// items. Each warp fetches for itself (bulk copies of whole units, 18 dk
+// bytes, into a ring of its own, some tiles ahead), so warps never wait for
+// one another. An item that one share has whole is written at once; of
 // the others each share leaves its part (m, l, O) in the work area, and a
 // second kernel joins an item's parts in a fixed order.
 
@@ -36,16 +36,16 @@ namespace {
 constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int JOIN_WARPS = 8;
 constexpr int TILE = 32;            // keys of a tile: two units
-constexpr uint32_t MAX_ENTRIES = 512;  // sequences of one launch
+constexpr uint32_t MAX_ENTRIES = 1024;  // sequences of one launch
 constexpr uint32_t MAX_TEAM = 16;
 constexpr uint32_t SPLIT_ROWS = 128;   // rows of an entry and cached head that are split along the keys; more are many
 constexpr int MAX_GRID = 160;
-constexpr int MAX_WORKERS = 15;
+constexpr int MAX_WORKERS = 16;
 
-// Warps of a block that compute, beside one that fetches; one block an SM.
-// Fifteen leave a thread 128 registers, seven 255.
-template <int NB, int NT> __host__ __device__ constexpr int workers() { return NB * NT <= 4 ? 15 : 7; }
-template <int NB, int NT> __host__ __device__ constexpr int stages() { return workers<NB, NT>() == 15 ? (NB <= 2 ? 4 : 3) : NB == 8 ? 3 : 4; }
+// Warps of a block, one block an SM. Sixteen leave a thread 128 registers,
+// eight 255.
+template <int NB, int NT> __host__ __device__ constexpr int workers() { return NB * NT <= 4 ? 16 : 8; }
+template <int NB, int NT> __host__ __device__ constexpr int stages() { return NB <= 2 ? 4 : NB * NT == 4 || NB == 8 ? 2 : 3; }
 template <int NB> __host__ __device__ constexpr int tile_bytes() { return 2 * 18 * 32 * NB; }
 template <int NB, int NT> __host__ __device__ constexpr int part_regs() { return NT * (NB * 8 + 4); }  // a lane's of one part
 
@@ -79,10 +79,9 @@ __device__ __forceinline__ Column column(const Attn4Args& a, const Entry& e, uin
     c.r = block * (8 * NT) + i / 2 * 8 + 2 * (threadIdx.x & 3) + i % 2;
     c.tok = c.r / a.G;
     c.valid = c.tok < e.rows;
-    const int64_t pos = static_cast<int64_t>(e.len) - e.rows + c.tok;
-    const int64_t hi = a.causal ? pos + 1 : e.len, lo = a.window ? pos - a.window + 1 : 0;
-    c.hi = c.valid ? static_cast<int32_t>(hi < 0 ? 0 : hi > e.len ? e.len : hi) : 0;
-    c.lo = static_cast<int32_t>(lo < 0 ? 0 : lo > INT_MAX ? INT_MAX : lo);
+    const Keys k = keys_of(a, e, c.tok);
+    c.lo = k.lo;
+    c.hi = c.valid ? k.hi : 0;
     return c;
 }
 
@@ -254,11 +253,21 @@ __device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB,
 // mask: some key of it is hidden from some row, or lies past the last one
 // that was fetched (limit).
 template <int NB, int NT, int PARTS>
-__device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, const Entry& e, uint32_t block, const uint8_t* buf,
+__device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, const Entry& e, uint32_t block, uint8_t* buf,
                                           const Query<NB, NT, PARTS>& q, int32_t key0, int32_t limit,
                                           float (&o)[2 * NB][NT][4], float (&m)[2 * NT], float (&l)[2 * NT]) {
     constexpr int DK = NB * 32;
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+    if (mask && key0 + TILE > limit) {
+        // V's scales past the limit may be anything, and 0 times a NaN is one: they become zeros where they lie
+        for (uint32_t x = lane; x < 2 * NB * C4_UNIT; x += 32) {
+            const uint32_t u = x / (NB * C4_UNIT), at = x % (NB * C4_UNIT);
+            if (key0 + static_cast<int32_t>(C4_UNIT * u + at % C4_UNIT) >= limit)
+                *reinterpret_cast<uint16_t*>(buf + u * 18 * DK + 17 * DK + 2 * at) = 0;
+        }
+        fence_async_smem();  // before a later copy into this place
+        __syncwarp();
+    }
     float s[2][NT][4];
     unit_scores<NB, NT, PARTS>(buf, q, s[0]);
     unit_scores<NB, NT, PARTS>(buf + 18 * DK, q, s[1]);
@@ -345,11 +354,6 @@ __device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, cons
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 s2[c] = *reinterpret_cast<const uint32_t*>(unit + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
-                if (mask) {  // scales past the limit may be anything, and 0 times a NaN is one
-                    const int32_t key = key0 + 16 * u + 8 * c + 2 * static_cast<int32_t>(t);
-                    if (key >= limit) s2[c] = 0;
-                    else if (key + 1 >= limit) s2[c] &= 0xFFFFu;
-                }
                 ms[c] = c4_m24(s2[c]);
             }
 #pragma unroll
@@ -379,21 +383,18 @@ __device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, cons
 }
 
 template <typename T, int NB, int NT, int PARTS>
-__global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(Attn4Args a) {
-    constexpr int DK = NB * 32, WORKERS = workers<NB, NT>(), THREADS = (WORKERS + 1) * 32, STAGES = stages<NB, NT>(), BYTES = tile_bytes<NB>();
+__global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4Args a) {
+    constexpr int DK = NB * 32, WORKERS = workers<NB, NT>(), THREADS = WORKERS * 32, STAGES = stages<NB, NT>(), BYTES = tile_bytes<NB>();
     constexpr int EACH = (MAX_ENTRIES + THREADS - 1) / THREADS;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t full[WORKERS][STAGES], empty[WORKERS][STAGES];
-    __shared__ uint32_t sums[WORKERS + 1];
+    __shared__ uint64_t full[WORKERS][STAGES];
+    __shared__ uint32_t sums[WORKERS];
     __shared__ volatile int gave_up;
     Entry* entries = reinterpret_cast<Entry*>(smem + WORKERS * STAGES * BYTES);
     uint32_t* base = reinterpret_cast<uint32_t*>(entries + a.n);  // each entry's first place
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
-    if (lane == 0 && warp < WORKERS) {
-        for (int i = 0; i < STAGES; i++) {
-            mbar_init(&full[warp][i], 1);
-            mbar_init(&empty[warp][i], 1);
-        }
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; i++) mbar_init(&full[warp][i], 1);
         fence_mbar_init();
     }
     if (tid == 0) gave_up = 0;
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(
             const Entry e = load_entry(a, i);
             entries[i] = e;
             base[i] = own;
-            own += e.places(a) * a.teams * e.blocks<NT>(a);
+            own += e.places * a.teams * e.blocks<NT>(a);
         }
     }
     uint32_t scan = own;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(
     __syncthreads();
     uint32_t total = 0;
 #pragma unroll
-    for (uint32_t w = 0; w <= WORKERS; w++) {
+    for (uint32_t w = 0; w < WORKERS; w++) {
         if (w == warp) scan += total - own;
         total += sums[w];
     }
@@ -438,104 +439,81 @@ __global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(
     };
     auto item_at = [&](uint32_t x) {
         Item it;
-        uint32_t lo = 0, hi = a.n;
+        uint32_t lo = 0, hi = a.n;  // thirty-two probes a step
         while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (base[mid] <= x) lo = mid; else hi = mid;
+            const uint32_t step = (hi - lo + 31) / 32, i = lo + lane * step;
+            const uint32_t last = 31 - __clz(__ballot_sync(FULL, i < hi && base[i] <= x) | 1u);
+            lo += last * step;
+            hi = min(lo + step, hi);
         }
         it.entry = lo;
         const Entry& e = entries[lo];
-        it.places = e.places(a);
-        const uint32_t at = x - base[lo], i = at / it.places, blocks = e.blocks<NT>(a), t = i / blocks;
-        it.place = at - i * it.places;
-        it.block = i - t * blocks;
-        it.head0 = t * a.team;
+        it.places = e.places;
+        it.place = x - base[lo];
+        it.block = it.head0 = 0;
+        if (it.place >= it.places) {
+            const uint32_t i = it.place / it.places, blocks = e.blocks<NT>(a), t = i / blocks;
+            it.place -= i * it.places;
+            it.block = i - t * blocks;
+            it.head0 = t * a.team;
+        }
         return it;
     };
 
-    if (warp == WORKERS) {
-        // the producer: lanes 2 w and 2 w + 1 fetch the units of worker w's tiles
-        const uint32_t mate = lane & 1, to = lane / 2, v = to * gridDim.x + blockIdx.x;
-        const uint32_t share = v / a.team, member = v - share * a.team;
-        const bool mine = to < WORKERS && share < split.n;
-        uint32_t x = mine ? split.begin(share) : 0;
-        const uint32_t end = mine ? split.begin(share + 1) : 0;
-        uint64_t* bars = full[mine ? to : 0];
-        uint8_t* ring = smem + ((mine ? to : 0) * STAGES * 2 + mate) * 18 * DK;
-        uint32_t left = 0, unit = 0, stop = 0;  // tiles of the item that are left in the share; this lane's next unit, and the item's end
-        const uint8_t* head = nullptr;          // the head's first unit in page 0
-        const int32_t* row = nullptr;           // the sequence's table
-        int32_t page = 0;                       // of this lane's next unit, asked for a tile ahead
-        const uint32_t per = a.c.pshift - 4;
-        // the first tile from place x on
-        auto enter = [&]() {
-            while (x < end) {
-                const Item it = item_at(x);
-                const Entry e = entries[it.entry];
-                const uint32_t skip = it.place < START ? START - it.place : 0, here = min(it.places - it.place, end - x);
-                x += here;
-                if (here <= skip || it.head0 + member >= a.c.heads) continue;
-                left = here - skip;
-                unit = e.unit0(a) + 2 * (it.place + skip - START) + mate;
-                stop = e.unit0(a) + e.units(a);
-                row = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
-                head = a.c.pages + a.layer * a.c.layer_bytes + (it.head0 + member) * a.c.head_bytes;
-                break;
-            }
-            if (left && unit < stop) page = row[unit >> per];
-        };
-        enter();
-        int stage = 0;
-        uint32_t phase = 0, issued = 0;
-        long long since = clock64();
-        while (__any_sync(FULL, left)) {
-            bool go = left && mbar_test_wait(&empty[to][stage], phase ^ 1);
-            go = __shfl_sync(FULL, go, static_cast<int>(lane & ~1u));
-            const bool has = unit < stop, both = __shfl_down_sync(FULL, has, 1);
-            if (go && !mate) mbar_arrive_expect_tx(&bars[stage], (both ? 2 : 1) * 18 * DK);
-            __syncwarp();
-            if (go) {
-                if (has) {
-                    if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
-                        atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
-                        page = 0;
-                    }
-                    bulk_load(ring + stage * BYTES, head + static_cast<uint32_t>(page) * a.c.page_bytes + (unit & ((1u << per) - 1)) * (18 * DK),
-                              18 * DK, &bars[stage]);
-                }
-                issued++;
-                if (++stage == STAGES) stage = 0, phase ^= 1;
-                if (--left) {
-                    unit += 2;
-                    if (unit < stop) page = row[unit >> per];
-                } else {
-                    enter();
-                }
-            }
-            if (__any_sync(FULL, go)) since = clock64();
-            else if (gave_up || clock64() - since > a.timeout) break;
-            else __nanosleep(64);  // the rings are full
-        }
-        if (left) {
-            gave_up = 1;
-            atomicOr(a.err, PKB_DEVERR_TIMEOUT);
-        }
-        // whatever the workers did, the copies in flight land before the block leaves its memory
-        for (int i = 0; i < STAGES && i < static_cast<int>(issued); i++) {
-            if (--stage < 0) stage = STAGES - 1, phase ^= 1;
-            mbar_drain(&bars[stage], phase, a.timeout);
-        }
-        return;
-    }
-
     // a team's warps lie on neighbouring SMs, and so do shares
     const uint32_t v = warp * gridDim.x + blockIdx.x, share = v / a.team, member = v - share * a.team;
-    const uint8_t* ring = smem + warp * STAGES * BYTES;
-    int stage = 0;
-    uint32_t phase = 0;
+    uint8_t* ring = smem + warp * STAGES * BYTES;
     if (share < split.n) {
         uint32_t x = split.begin(share);
         const uint32_t end = split.begin(share + 1);
+        // What is fetched next, STAGES tiles ahead of what is computed: lanes
+        // 0 and 1 take a tile's two units. A tile's pages are asked for a tile
+        // before they are needed.
+        uint32_t ahead = x, left = 0, unit = 0, stop_unit = 0;  // the next item's place; tiles left of this one, this lane's unit, the end
+        const uint8_t* head = nullptr;  // the head's first unit in page 0
+        const int32_t* row = nullptr;   // the sequence's table
+        int32_t page = 0;
+        const uint32_t per = a.c.pshift - 4;
+        auto look = [&]() {
+            if (lane < 2 && unit < stop_unit) page = row[unit >> per];
+        };
+        auto enter = [&]() {  // the first tile from place `ahead` on
+            while (ahead < end) {
+                const Item it = item_at(ahead);
+                const Entry e = entries[it.entry];
+                const uint32_t skip = it.place < START ? START - it.place : 0, here = min(it.places - it.place, end - ahead);
+                ahead += here;
+                if (here <= skip || it.head0 + member >= a.c.heads) continue;
+                left = here - skip;
+                unit = e.unit0 + 2 * (it.place + skip - START) + lane;
+                stop_unit = e.unit0 + e.units;
+                row = a.c.table + static_cast<size_t>(e.seq) * a.c.max_pages;
+                head = a.c.pages + a.layer * a.c.layer_bytes + (it.head0 + member) * a.c.head_bytes;
+                look();
+                break;
+            }
+        };
+        auto fetch = [&](int stage) {
+            if (!left) return;
+            // of two units, the second may lie past the sequence's end (lane 0 knows)
+            if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], (unit + 1 < stop_unit ? 2 : 1) * 18 * DK);
+            __syncwarp();
+            if (lane < 2 && unit < stop_unit) {
+                if (page < 0 || static_cast<uint32_t>(page) >= a.c.n_pages) {
+                    atomicOr(a.err, PKB_DEVERR_ARGS);  // any page will do, the rows are not defined
+                    page = 0;
+                }
+                bulk_load(ring + (2 * stage + lane) * 18 * DK, head + static_cast<uint32_t>(page) * a.c.page_bytes + (unit & ((1u << per) - 1)) * (18 * DK),
+                          18 * DK, &full[warp][stage]);
+            }
+            unit += 2;
+            if (--left) look();
+            else enter();
+        };
+        enter();
+        int stage = 0, flying = 0;
+        uint32_t phase = 0;
+        for (; flying < STAGES && left; flying++) fetch(flying);
         while (x < end) {
             // one item, or the part of it in this share
             const Item it = item_at(x);
@@ -567,19 +545,25 @@ __global__ void __launch_bounds__((workers<NB, NT>() + 1) * 32, 1) split_kernel(
                     for (int y = 0; y < 4; y++) o[d][j][y] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
-            int32_t key0 = static_cast<int32_t>((e.unit0(a) + 2 * first) * C4_UNIT);
+            int32_t key0 = static_cast<int32_t>((e.unit0 + 2 * first) * C4_UNIT);
             for (uint32_t left = stop - START - first; left; left--) {
                 if (!warp_wait(&full[warp][stage], phase, &gave_up, a.timeout)) {
-                    gave_up = 1;  // the producer lets what is in flight land
+                    // a copy that does not come: say so, let those in flight land, leave
+                    gave_up = 1;
                     if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                    for (; flying; flying--) {
+                        mbar_drain(&full[warp][stage], phase, a.timeout);
+                        if (++stage == STAGES) stage = 0, phase ^= 1;
+                    }
                     return;
                 }
-                const uint8_t* buf = ring + stage * BYTES;
+                uint8_t* buf = ring + stage * BYTES;
                 // warp-uniform: tiles at the window's start, the causal edge and the last token
-                const bool mask = key0 < all_lo || static_cast<int64_t>(key0) + TILE > all_hi;
+                const bool mask = key0 < all_lo || key0 + TILE > all_hi;
                 tile_step<NB, NT, PARTS>(mask, a, e, block, buf, q, key0, static_cast<int32_t>(e.len), o, m, l);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[warp][stage]);
+                if (left) fetch(stage);
+                else flying--;
                 key0 += TILE;
                 if (++stage == STAGES) stage = 0, phase ^= 1;
             }
@@ -696,7 +680,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint
         }
     }
     if (z >= QUADS) return;
-    const Entry e = {0, item.r0, item.rows, 0};
+    const Entry e = {0, item.r0, item.rows, 0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const Column c = column<NT>(a, e, block, 2 * j + i);
@@ -746,9 +730,7 @@ __global__ void __launch_bounds__((ROW_WARPS + 1) * 32, 1) rows_kernel(Attn4Args
     const uint32_t group = groups - 1 - blockIdx.x, block = group * ROW_WARPS + warp;
     // the units that the block's rows can see
     const uint32_t tok0 = group * ROW_WARPS * 8 * NT / a.G, tok1 = min((group + 1) * ROW_WARPS * 8 * NT - 1, e.rows * a.G - 1) / a.G;
-    const int64_t pos0 = static_cast<int64_t>(e.len) - e.rows + tok0, pos1 = static_cast<int64_t>(e.len) - e.rows + tok1;
-    const int64_t lo = a.window && pos0 - a.window + 1 > 0 ? pos0 - a.window + 1 : 0;
-    const int64_t hi = a.causal ? (pos1 + 1 < e.len ? pos1 + 1 : e.len) : e.len;
+    const int32_t lo = keys_of(a, e, tok0).lo, hi = keys_of(a, e, tok1).hi;
     const uint32_t unit0 = static_cast<uint32_t>(lo / C4_UNIT);
     const uint32_t units = hi > lo ? static_cast<uint32_t>((hi + C4_UNIT - 1) / C4_UNIT) - unit0 : 0, tiles = (units + 1) / 2;
 
@@ -818,9 +800,9 @@ __global__ void __launch_bounds__((ROW_WARPS + 1) * 32, 1) rows_kernel(Attn4Args
             if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
             return;
         }
-        if (key0 < any_hi && static_cast<int64_t>(key0) + TILE > any_lo) {
-            const bool mask = key0 < all_lo || static_cast<int64_t>(key0) + TILE > all_hi;
-            tile_step<NB, NT, PARTS>(mask, a, e, block, smem + stage * BYTES, q, key0, static_cast<int32_t>(hi), o, m, l);
+        if (key0 < any_hi && key0 + TILE > any_lo) {
+            const bool mask = key0 < all_lo || key0 + TILE > all_hi;
+            tile_step<NB, NT, PARTS>(mask, a, e, block, smem + stage * BYTES, q, key0, hi, o, m, l);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
@@ -866,7 +848,7 @@ cudaError_t launch_one(Attn4Args a, int sms, cudaStream_t s) {
     }
     const uint32_t grid = static_cast<uint32_t>(sms < MAX_GRID ? sms : MAX_GRID);
     a.max_blocks = (a.max_rows * a.G + 8 * NT - 1) / (8 * NT);
-    cudaError_t e = c4_launch(split_kernel<T, NB, NT, PARTS>, grid, (workers<NB, NT>() + 1) * 32, split_smem<NB, NT>(a.n), s, a);
+    cudaError_t e = c4_launch(split_kernel<T, NB, NT, PARTS>, grid, workers<NB, NT>() * 32, split_smem<NB, NT>(a.n), s, a);
     if (e != cudaSuccess) return e;
     count_launch();
     // parts an item has about, if all have as many: more than four go two ways and so on
@@ -958,6 +940,8 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     if (!H || H % c->n_heads) return set_error(PKB_EINVAL, "%s: H = %u, a multiple of the cache's %u heads", who, H, c->n_heads);
     if (!(scale - scale == 0.0f)) return set_error(PKB_EINVAL, "%s: scale is not finite", who);
     if (window > INT_MAX) return set_error(PKB_EINVAL, "%s: window = %u", who, window);
+    // one that reaches past every sequence's first token from its last row on is none
+    if (window >= static_cast<uint64_t>(c->max_pages) * c->page_tokens + max_rows) window = 0;
     if (!n || !rows) return PKB_OK;
     if (!o || !q || !seqs || !starts || !work) return set_error(PKB_EINVAL, "%s: null pointer", who);
     if (!max_rows || max_rows > rows) return set_error(PKB_EINVAL, "%s: max_rows = %u of %u rows", who, max_rows, rows);

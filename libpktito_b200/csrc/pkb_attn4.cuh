@@ -127,19 +127,15 @@ __device__ __forceinline__ float rescale(float from, float to) { return from == 
 // tiles.
 constexpr uint32_t START = 2;
 
-// One entry's rows and tokens, and of what its rows can see the units and
-// the places (START and the tiles, 0 where nothing is seen).
+// One entry's rows and tokens, and of what its rows can see the first unit,
+// how many, and the places (START and the tiles, 0 where nothing is seen).
+// Positions fit an int: a cache's sequences are below 2^30 tokens, and a
+// window that reaches past one is none.
 struct Entry {
-    uint32_t seq, r0, rows, len;
-    __device__ __forceinline__ uint32_t unit0(const Attn4Args& a) const {
-        // the first row's window begins furthest back; the last row's causal end is len
-        const int64_t lo = a.window ? static_cast<int64_t>(len) - rows - a.window + 1 : 0;
-        return lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
-    }
-    __device__ __forceinline__ uint32_t units(const Attn4Args& a) const { return (len + C4_UNIT - 1) / C4_UNIT - unit0(a); }
-    __device__ __forceinline__ uint32_t places(const Attn4Args& a) const { return len ? START + (units(a) + 1) / 2 : 0; }
+    uint32_t seq, r0, rows, len, unit0, units, places;
     template <int NT>
     __device__ __forceinline__ uint32_t blocks(const Attn4Args& a) const { return (rows * a.G + 8 * NT - 1) / (8 * NT); }
+    __device__ __forceinline__ int32_t position(uint32_t tok) const { return static_cast<int32_t>(len - rows + tok); }
 };
 
 __device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
@@ -150,7 +146,21 @@ __device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
         e.rows = 0;
     }
     e.len = e.rows ? c4_len(a.c, e.seq, a.err) : 0;
+    // the first row's window begins furthest back; the last row's causal end is len
+    const int32_t lo = a.window ? e.position(0) - static_cast<int32_t>(a.window) + 1 : 0;
+    e.unit0 = lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
+    e.units = (e.len + C4_UNIT - 1) / C4_UNIT - e.unit0;
+    e.places = e.len ? START + (e.units + 1) / 2 : 0;
     return e;
+}
+
+// The keys [lo, hi) that the row of an entry's token sees.
+struct Keys {
+    int32_t lo, hi;
+};
+__device__ __forceinline__ Keys keys_of(const Attn4Args& a, const Entry& e, uint32_t tok) {
+    const int32_t pos = e.position(tok), len = static_cast<int32_t>(e.len);
+    return {a.window ? max(pos - static_cast<int32_t>(a.window) + 1, 0) : 0, a.causal ? max(min(pos + 1, len), 0) : len};
 }
 
 // Many bf16 rows on the fifth-generation tensor cores (pkb_attn4_tc.cu): whether

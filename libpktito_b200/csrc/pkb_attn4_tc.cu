@@ -106,16 +106,6 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t at, const uint32_t (&r)[16]
 // byte offset of a 16-byte chunk of a row in a slab of 128-byte swizzled rows
 __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
-// What the rows of a block may see: keys [lo, hi)
-struct Span {
-    int64_t lo, hi;
-};
-__device__ __forceinline__ Span span_of(const Attn4Args& a, const Entry& e, uint32_t tok) {
-    const int64_t pos = static_cast<int64_t>(e.len) - e.rows + tok;
-    const int64_t hi = a.causal ? pos + 1 : e.len, lo = a.window ? pos - a.window + 1 : 0;
-    return {lo < 0 ? 0 : lo, hi < 0 ? 0 : hi > e.len ? e.len : hi};
-}
-
 // N words of memory, as wide as they lie
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
@@ -384,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     if (rank >= groups) return;  // the whole block
     const uint32_t group = groups - 1 - rank, row0 = group * ROWS, tiles = all - row0 > 128 ? 2 : 1;
     const uint32_t last = min(row0 + ROWS, all) - 1;
-    const int64_t lo = span_of(a, e, row0 / a.G).lo, hi = span_of(a, e, last / a.G).hi;
+    const int32_t lo = keys_of(a, e, row0 / a.G).lo, hi = keys_of(a, e, last / a.G).hi;
     const uint32_t unit0 = static_cast<uint32_t>(lo / C4_UNIT);
     const uint32_t units = hi > lo ? static_cast<uint32_t>((hi + C4_UNIT - 1) / C4_UNIT) - unit0 : 0;
     const uint32_t steps = (units * C4_UNIT + KEYS - 1) / KEYS;
@@ -534,8 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
                 ok = warp_wait(&bars.v_empty[st], ph ^ 1, &gave_up, a.timeout);
             }
             if (ok) {
-                const int64_t left = hi - key_base - static_cast<int64_t>(i * KEYS + 16 * w);
-                v.store(v_tiles + st * v_tile<NB>() + w / 4 * (DK * 128), w % 4, static_cast<int32_t>(left < 0 ? 0 : left < C4_UNIT ? left : C4_UNIT));
+                v.store(v_tiles + st * v_tile<NB>() + w / 4 * (DK * 128), w % 4, hi - key_base - static_cast<int32_t>(i * KEYS + 16 * w));
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.v_full[st]);
@@ -551,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         // the rows: thread i of a tile's four warps has row i
         set_registers<SOFT_REGS, true>();
         const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
-        const Span span = span_of(a, e, min(tok, e.rows - 1));  // rows there are none of see what the last one does
+        const Keys span = keys_of(a, e, min(tok, e.rows - 1));  // rows there are none of see what the last one does
         const uint32_t at = tmem + ((warp % 4) * 32 << 16), s_at = at + S_COL + 128 * t, o_at = at + O_COL + 128 * t;
         const float scale = fmaxf(fabsf(a.scale), 1e-37f);  // of a scale 0 too
         float m = NEG_INF, l = 0.0f;
@@ -560,9 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             ok = warp_wait(&bars.s_full[t], i & 1, &gave_up, a.timeout);
             if (!ok) break;
             tc_fence_after();
-            const int64_t key0 = static_cast<int64_t>(key_base) + i * KEYS;
-            const int32_t first = static_cast<int32_t>(max(min(span.lo - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
-            const int32_t end = static_cast<int32_t>(max(min(span.hi - key0, static_cast<int64_t>(KEYS)), static_cast<int64_t>(0)));
+            const int32_t key0 = key_base + static_cast<int32_t>(i * KEYS), first = span.lo - key0, end = span.hi - key0;
             const bool before = __any_sync(FULL, first > 0), behind = __any_sync(FULL, end < KEYS);
             if (before) softmax_step<NB, 2>(s_at, o_at, i > 0, scale, first, end, m, l);
             else if (behind) softmax_step<NB, 1>(s_at, o_at, i > 0, scale, 0, end, m, l);

@@ -708,7 +708,7 @@ int c4_view(const pkb_cache4* c, const char* who, Cache4* v) {
         return set_error(PKB_EINVAL, "%s: pages of %u tokens, %u heads of %u: 16 to 256 tokens, a power of two; heads of 32, 64, 96, 128 or 256",
                          who, c->page_tokens, c->n_heads, c->head_dim);
     if (!c->n_layers || !c->n_pages || !c->max_seqs || !c->max_pages || c->n_pages > INT_MAX || c->max_seqs > INT_MAX ||
-        static_cast<uint64_t>(c->max_pages) * c->page_tokens > INT_MAX)
+        static_cast<uint64_t>(c->max_pages) * c->page_tokens > 1u << 30)
         return set_error(PKB_EINVAL, "%s: %u layers, %u pages, %u sequences of up to %u pages", who, c->n_layers, c->n_pages,
                          c->max_seqs, c->max_pages);
     if (!c->pages || !c->table || !c->lens || !c->refs) return set_error(PKB_EINVAL, "%s: null pointer in the cache", who);
