@@ -388,10 +388,11 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
     constexpr int EACH = (MAX_ENTRIES + THREADS - 1) / THREADS;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[WORKERS][STAGES];
-    __shared__ uint32_t sums[WORKERS];
+    __shared__ uint64_t sums[WORKERS];
+    __shared__ uint32_t most[WORKERS];
     __shared__ volatile int gave_up;
     Entry* entries = reinterpret_cast<Entry*>(smem + WORKERS * STAGES * BYTES);
-    uint32_t* base = reinterpret_cast<uint32_t*>(entries + a.n);  // each entry's first place
+    uint32_t* base = reinterpret_cast<uint32_t*>(entries + a.n);  // each entry's first place, or item where shares take whole ones
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
     if (lane == 0) {
         for (int i = 0; i < STAGES; i++) mbar_init(&full[warp][i], 1);
@@ -400,44 +401,55 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
     if (tid == 0) gave_up = 0;
     pdl_trigger();
     pdl_wait();
-    uint32_t own = 0;
+    // places and items (in the upper half) before each entry, and the longest item's places
+    uint64_t before[EACH], own = 0;
+    uint32_t longest = 0;
 #pragma unroll
     for (int x = 0; x < EACH; x++) {
         const uint32_t i = tid * EACH + x;
+        before[x] = own;
         if (i < a.n) {
             const Entry e = load_entry(a, i);
             entries[i] = e;
-            base[i] = own;
-            own += e.places * a.teams * e.blocks<NT>(a);
+            const uint64_t items = e.places ? a.teams * e.blocks<NT>(a) : 0;
+            own += items * e.places + (items << 32);
+            longest = max(longest, e.places);
         }
     }
-    uint32_t scan = own;
+    uint64_t scan = own;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const uint32_t y = __shfl_up_sync(FULL, scan, d);
+        const uint64_t y = __shfl_up_sync(FULL, scan, d);
         if (lane >= static_cast<uint32_t>(d)) scan += y;
     }
-    if (lane == 31) sums[warp] = scan;
+    longest = __reduce_max_sync(FULL, longest);
+    if (lane == 31) sums[warp] = scan, most[warp] = longest;
     __syncthreads();
-    uint32_t total = 0;
+    uint64_t total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < WORKERS; w++) {
         if (w == warp) scan += total - own;
         total += sums[w];
+        longest = max(longest, most[w]);
     }
+    // Where no item is longer than one and a half shares, shares take whole
+    // items: there is nothing to join then.
+    const uint32_t room = min(gridDim.x * WORKERS / a.team, a.max_shares), places = static_cast<uint32_t>(total);
+    const bool whole = 2ull * longest * room <= 3ull * places;
 #pragma unroll
     for (int x = 0; x < EACH; x++) {
         const uint32_t i = tid * EACH + x;
-        if (i < a.n) base[i] += scan;
+        if (i < a.n) base[i] = static_cast<uint32_t>(whole ? (scan + before[x]) >> 32 : scan + before[x]);
     }
-    if (tid == 0) base[a.n] = total;
+    if (tid == 0) base[a.n] = whole ? static_cast<uint32_t>(total >> 32) : places;
     __syncthreads();
-    const Split split(total, min(gridDim.x * WORKERS / a.team, a.max_shares));
+    const Split split(whole ? static_cast<uint32_t>(total >> 32) : places, room);
     // where a place lies: its entry, its item of that, and its place in the item
     struct Item {
         uint32_t entry, head0, block, place, places;
+        uint32_t stop, next;  // the share's last place of it and one, and where its next item begins
     };
-    auto item_at = [&](uint32_t x) {
+    auto item_at = [&](uint32_t x, uint32_t end) {
         Item it;
         uint32_t lo = 0, hi = a.n;  // thirty-two probes a step
         while (hi - lo > 1) {
@@ -451,12 +463,15 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
         it.places = e.places;
         it.place = x - base[lo];
         it.block = it.head0 = 0;
-        if (it.place >= it.places) {
-            const uint32_t i = it.place / it.places, blocks = e.blocks<NT>(a), t = i / blocks;
-            it.place -= i * it.places;
+        const uint32_t each = whole ? 1 : it.places;
+        if (it.place >= each) {
+            const uint32_t i = it.place / each, blocks = e.blocks<NT>(a), t = i / blocks;
+            it.place -= i * each;
             it.block = i - t * blocks;
             it.head0 = t * a.team;
         }
+        it.stop = whole ? it.places : min(it.places, it.place + (end - x));
+        it.next = x + (whole ? 1 : it.stop - it.place);
         return it;
     };
 
@@ -479,10 +494,10 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
         };
         auto enter = [&]() {  // the first tile from place `ahead` on
             while (ahead < end) {
-                const Item it = item_at(ahead);
-                const Entry e = entries[it.entry];
-                const uint32_t skip = it.place < START ? START - it.place : 0, here = min(it.places - it.place, end - ahead);
-                ahead += here;
+                const Item it = item_at(ahead, end);
+                const Entry& e = entries[it.entry];
+                const uint32_t skip = it.place < START ? START - it.place : 0, here = it.stop - it.place;
+                ahead = it.next;
                 if (here <= skip || it.head0 + member >= a.c.heads) continue;
                 left = here - skip;
                 unit = e.unit0 + 2 * (it.place + skip - START) + lane;
@@ -516,9 +531,9 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
         for (; flying < STAGES && left; flying++) fetch(flying);
         while (x < end) {
             // one item, or the part of it in this share
-            const Item it = item_at(x);
-            const uint32_t x0 = x - it.place, here = min(it.places - it.place, end - x), stop = it.place + here;
-            x += here;
+            const Item it = item_at(x, end);
+            const uint32_t x0 = x - it.place, stop = it.stop;
+            x = it.next;
             const uint32_t h = it.head0 + member;
             if (stop <= START || h >= a.c.heads) continue;
             const Entry e = entries[it.entry];
@@ -569,8 +584,8 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
             }
 #pragma unroll
             for (int i = 0; i < 2 * NT; i++) l[i] = column_sum(l[i]);
-            const bool whole = first == 0 && stop == it.places;
-            if (whole) {
+            const bool entire = first == 0 && stop == it.places;
+            if (entire) {
                 write_rows<T, NB, NT>(a, e, h, block, o, l);
             } else {
                 float4* part = reinterpret_cast<float4*>(a.part) + static_cast<size_t>(2 * v + (first == 0)) * (part_regs<NB, NT>() / 4) * 32 + lane;
@@ -585,7 +600,7 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
             if (stop == it.places && lane == 0) {
                 const uint32_t team = it.head0 / a.team;
                 a.joins[((static_cast<size_t>(it.entry) * a.teams + team) * a.max_blocks + block) * a.team + member] =
-                    Attn4Join{whole ? Attn4Join::NONE : split.of(x0 + START), share, e.r0, e.rows};
+                    Attn4Join{entire ? Attn4Join::NONE : split.of(x0 + START), share, e.r0, e.rows};
             }
         }
     }
@@ -609,7 +624,7 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 // items have few parts each and take one way, a few long ones take up to
 // eight, so that no warp reads many parts one after another.
 template <typename T, int NB, int NT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint32_t ways) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32, 4) join_kernel(Attn4Args a, uint32_t ways) {
     constexpr int QUADS = 2 * NB * NT, STRIDE = part_regs<NB, NT>() / 4;  // float4s of a lane: [dims 16][eight rows], then m and l
     __shared__ float4 sm[2][JOIN_WARPS][32];
     pdl_trigger();
@@ -626,11 +641,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint
     const uint32_t all = item.last - item.first + 1, count = all > way ? (all - way + ways - 1) / ways : 0;
     if (z < QUADS) {
         const float4* part = reinterpret_cast<const float4*>(a.part) + lane;
-        // eight parts at a time, all of their loads before the first use
-        for (uint32_t i0 = 0; i0 < count; i0 += 8) {
-            float4 v[8], x[8];
+        // four parts at a time, all of their loads before the first use
+        for (uint32_t i0 = 0; i0 < count; i0 += 4) {
+            float4 v[4], x[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
+            for (uint32_t i = 0; i < 4; i++) {
                 v[i] = make_float4(NEG_INF, NEG_INF, 0.0f, 0.0f);
                 x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (i0 + i < count) {
@@ -642,7 +657,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint
             }
             float t0 = m0, t1 = m1;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
+            for (uint32_t i = 0; i < 4; i++) {
                 t0 = fmaxf(t0, v[i].x);
                 t1 = fmaxf(t1, v[i].y);
             }
@@ -650,7 +665,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Attn4Args a, uint
             m0 = t0, m1 = t1;
             l0 *= k0, l1 *= k1, o[0] *= k0, o[1] *= k1, o[2] *= k0, o[3] *= k1;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
+            for (uint32_t i = 0; i < 4; i++) {
                 const float f0 = rescale(v[i].x, m0), f1 = rescale(v[i].y, m1);
                 l0 = __fmaf_rn(v[i].z, f0, l0);
                 l1 = __fmaf_rn(v[i].w, f1, l1);
