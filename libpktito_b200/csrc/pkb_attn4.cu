@@ -623,8 +623,10 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 // item's parts; `ways` warps then join theirs, always in the same order. Many
 // items have few parts each and take one way, a few long ones take up to
 // eight, so that no warp reads many parts one after another.
-template <typename T, int NB, int NT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32, 4) join_kernel(Attn4Args a, uint32_t ways) {
+// BATCH parts are loaded together: four (and 64 registers, so that four blocks
+// share an SM) for many items, eight for a few long ones.
+template <typename T, int NB, int NT, int BATCH>
+__global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kernel(Attn4Args a, uint32_t ways) {
     constexpr int QUADS = 2 * NB * NT, STRIDE = part_regs<NB, NT>() / 4;  // float4s of a lane: [dims 16][eight rows], then m and l
     __shared__ float4 sm[2][JOIN_WARPS][32];
     pdl_trigger();
@@ -641,11 +643,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) join_kernel(Attn4Args a, u
     const uint32_t all = item.last - item.first + 1, count = all > way ? (all - way + ways - 1) / ways : 0;
     if (z < QUADS) {
         const float4* part = reinterpret_cast<const float4*>(a.part) + lane;
-        // four parts at a time, all of their loads before the first use
-        for (uint32_t i0 = 0; i0 < count; i0 += 4) {
-            float4 v[4], x[4];
+        // all of a batch's loads before the first use
+        for (uint32_t i0 = 0; i0 < count; i0 += BATCH) {
+            float4 v[BATCH], x[BATCH];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
+            for (uint32_t i = 0; i < BATCH; i++) {
                 v[i] = make_float4(NEG_INF, NEG_INF, 0.0f, 0.0f);
                 x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (i0 + i < count) {
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) join_kernel(Attn4Args a, u
             }
             float t0 = m0, t1 = m1;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
+            for (uint32_t i = 0; i < BATCH; i++) {
                 t0 = fmaxf(t0, v[i].x);
                 t1 = fmaxf(t1, v[i].y);
             }
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) join_kernel(Attn4Args a, u
             m0 = t0, m1 = t1;
             l0 *= k0, l1 *= k1, o[0] *= k0, o[1] *= k1, o[2] *= k0, o[3] *= k1;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
+            for (uint32_t i = 0; i < BATCH; i++) {
                 const float f0 = rescale(v[i].x, m0), f1 = rescale(v[i].y, m1);
                 l0 = __fmaf_rn(v[i].z, f0, l0);
                 l1 = __fmaf_rn(v[i].w, f1, l1);
@@ -872,7 +874,7 @@ cudaError_t launch_one(Attn4Args a, int sms, cudaStream_t s) {
     uint32_t ways = 1;
     while (ways < 8 && shares > 4 * ways * items) ways *= 2;
     const uint32_t quads = JOIN_WARPS / ways;
-    e = c4_launch(join_kernel<T, NB, NT>, dim3(static_cast<uint32_t>(items * a.team), (2 * NB * NT + quads - 1) / quads), JOIN_WARPS * 32, 0, s, a, ways);
+    e = c4_launch(ways > 1 ? join_kernel<T, NB, NT, 8> : join_kernel<T, NB, NT, 4>, dim3(static_cast<uint32_t>(items * a.team), (2 * NB * NT + quads - 1) / quads), JOIN_WARPS * 32, 0, s, a, ways);
     if (e == cudaSuccess) count_launch();
     return e;
 }
