@@ -34,6 +34,16 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 // no scan over the entries is needed. Thirty-two probes a step.
 __device__ __forceinline__ uint32_t slot_entry(const int32_t* starts, uint32_t n, uint32_t x) {
     const uint32_t lane = threadIdx.x & 31;
+    if (n <= 256) {  // eight entries a lane, all asked for at once
+        uint32_t below = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            const uint32_t i = j * 32 + lane;
+            below += i < n && static_cast<uint32_t>(starts[i]) / C4_UNIT + 2 * i <= x;
+        }
+        below = __reduce_add_sync(FULL, below);
+        return below ? below - 1 : 0;
+    }
     uint32_t lo = 0, hi = n;  // the answer is in [lo, hi)
     while (hi - lo > 1) {
         const uint32_t step = (hi - lo + 31) / 32, i = lo + lane * step;
@@ -84,13 +94,58 @@ __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, u
 
 template <int NB> __host__ __device__ constexpr int v_row() { return NB * 16 + 8; }  // a token's V bytes, and 8 against bank conflicts
 
+// A block's scale and its codes + 8, from four lanes' eight values each.
+//
+// The scale is the largest s of 5 significant bits with 7 s <= amax: amax / 7
+// cut to 5 bits, or the one before where the product rounded up (7 s has 8
+// bits, so the comparison is exact). A code is rint(x / s), ties to even:
+// from x times an approximate 1 / s, whose remainder x - c s is exact in
+// one FMA and says whether c is the nearest. It is not, or may be a tie, in
+// few warps: the others skip the correction. No division: with a correctly
+// rounded one a value the kernel took 49 us for 28.8 M float values, 30 so.
+__device__ __forceinline__ float quantize_block(float (&f)[8], uint32_t (&nib)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, abs_bits(f[i]));
+    m = max(m, __shfl_xor_sync(FULL, m, 1));
+    m = max(m, __shfl_xor_sync(FULL, m, 2));
+    const bool scaled = block_scaled(m);
+    float s = __uint_as_float(__float_as_uint(__fmul_rn(__uint_as_float(m), 0.14285714924335479736f)) & 0xFFF80000u);
+    if (__fmul_rn(s, 7.0f) > __uint_as_float(m)) s = __uint_as_float(__float_as_uint(s) - 0x80000u);
+    if (__any_sync(FULL, !scaled)) {  // zeros, with a scale that divides
+        s = scaled ? s : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = scaled ? f[i] : 0.0f;
+    }
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    float left[8], worst = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        // 8 + c in the low bits of 1.5 2^23 + 8 + x / s (8 is even, so ties stay ties)
+        const float sum = __fadd_rn(__fmul_rn(f[i], inv), 12582920.0f);
+        nib[i] = __float_as_uint(sum);
+        left[i] = __fmaf_rn(__fsub_rn(12582920.0f, sum), s, f[i]);
+        worst = fmaxf(worst, fabsf(left[i]));
+    }
+    const float half = 0.5f * s;
+    if (__any_sync(FULL, worst >= half)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (fabsf(left[i]) > half || (fabsf(left[i]) == half && (nib[i] & 1))) nib[i] += left[i] > 0.0f ? 1 : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) nib[i] &= 15u;
+    return scaled ? s : 0.0f;
+}
+
 template <typename T, int NB, bool VEC>
-__global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* __restrict__ k, const T* __restrict__ v, RowArgs a) {
+__global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* k, const T* v, RowArgs a) {
     constexpr int DK = NB * 32;
     __shared__ alignas(16) uint8_t stage[ROW_WARPS][C4_UNIT * v_row<NB>()];
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane / 4, t = lane & 3;
     const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + warp;
     const bool is_v = item & 1;
     const uint32_t h = static_cast<uint32_t>((item >> 1) % a.c.heads);
@@ -98,53 +153,54 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* __restr
     if (slot >= a.slots) return;
     const UnitRows u = warp_unit(a, static_cast<uint32_t>(slot), h);
     if (!u.bytes) return;
-    const T* x = is_v ? v : k;
     const size_t xs = is_v ? a.vs : a.ks;
+    const T* x = (is_v ? v : k) + h * DK + 8 * t;
     uint8_t* codes = u.bytes + (is_v ? 8 * DK : 0);
     __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(u.bytes + (is_v ? 17 * DK : 16 * DK));
     uint8_t* vb = stage[warp];
-#pragma unroll 4
-    for (int pass = 0; pass < 2 * NB; pass++) {
-        const int b = pass * 8 + lane / 4, token = b / NB, blk = b % NB, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        // lanes 4 g .. 4 g + 3 have token g or g + 8, eight values of each block
+        const int token = static_cast<int>(g) + 8 * r;
         const bool valid = token >= u.first && token < u.last;
         if (!__any_sync(FULL, valid)) continue;
-        float f[8];
+        float f[NB][8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = 0.0f;
-        if (valid) c4_load8<T, VEC>(x + (u.row0 + token) * xs + h * DK + blk * 32 + t * 8, f);
-        uint32_t m = 0;
+        for (int b = 0; b < NB; b++) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = max(m, abs_bits(f[i]));
-        m = max(m, __shfl_xor_sync(FULL, m, 1));
-        m = max(m, __shfl_xor_sync(FULL, m, 2));
-        // 5 significant bits of amax / 7, cut: 7 s is at most amax (no
-        // overflow) and amax / s below 7.47, so every code is within 7. The
-        // correctly rounded quotients round to an integer as the exact ones
-        // do: with s of 5 bits x / s is never so near a half, or amax / 7 a
-        // number of 5 bits, that the float quotient would meet it.
-        const bool scaled = block_scaled(m);
-        const float s = scaled ? __uint_as_float(__float_as_uint(__fdiv_rn(__uint_as_float(m), 7.0f)) & 0xFFF80000u) : 1.0f;
-        uint32_t nib[8];
+            for (int i = 0; i < 8; i++) f[b][i] = 0.0f;
+            if (valid) c4_load8<T, VEC>(x + (u.row0 + token) * xs + b * 32, f[b]);
+        }
+        uint32_t words[NB];
 #pragma unroll
-        for (int i = 0; i < 8; i++)  // 8 + rint(x / s) in the low bits of 1.5 * 2^23 + 8 + x / s
-            nib[i] = scaled ? __float_as_uint(__fadd_rn(__fdiv_rn(f[i], s), 12582920.0f)) & 15u : 8u;
-        const __nv_bfloat16 sb = __float2bfloat16_rn(scaled ? s : 0.0f);  // exact: 5 bits
-        if (!is_v) {
-            uint32_t w = 0;
+        for (int b = 0; b < NB; b++) {
+            uint32_t nib[8];
+            const __nv_bfloat16 s = __float2bfloat16_rn(quantize_block(f[b], nib));  // exact: 5 bits
+            if (!is_v) {
+                uint32_t w = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) w |= nib[i] << (4 * (i / 2) + 16 * (i % 2));
-            if (valid) {
-                reinterpret_cast<uint32_t*>(codes)[(token * 4 + t) * NB + blk] = w;
-                if (t == 0) scales[token * NB + blk] = sb;
+                for (int i = 0; i < 8; i++) w |= nib[i] << (4 * (i / 2) + 16 * (i % 2));
+                words[b] = w;
+                if (valid && t == 0) scales[token * NB + b] = s;
+            } else {
+                const uint32_t lo = nib[0] | nib[1] << 8 | nib[2] << 16 | nib[3] << 24;
+                const uint32_t hi = nib[4] | nib[5] << 8 | nib[6] << 16 | nib[7] << 24;
+                // values 8 apart share a byte: the even lane of a pair makes the first four bytes, the odd one the others
+                const uint32_t got = __shfl_xor_sync(FULL, t & 1 ? lo : hi, 1);
+                const uint32_t w = t & 1 ? got | hi << 4 : lo | got << 4;
+                *reinterpret_cast<uint32_t*>(vb + token * v_row<NB>() + (b * 2 + t / 2) * 8 + (t & 1) * 4) = w;
+                if (valid && t == 0) scales[b * C4_UNIT + token] = s;
             }
-        } else {
-            const uint32_t lo = nib[0] | nib[1] << 8 | nib[2] << 16 | nib[3] << 24;
-            const uint32_t hi = nib[4] | nib[5] << 8 | nib[6] << 16 | nib[7] << 24;
-            // values 8 apart share a byte: the even lane of a pair makes the first four bytes, the odd one the others
-            const uint32_t got = __shfl_xor_sync(FULL, t & 1 ? lo : hi, 1);
-            const uint32_t w = t & 1 ? got | hi << 4 : lo | got << 4;
-            *reinterpret_cast<uint32_t*>(vb + token * v_row<NB>() + (blk * 2 + t / 2) * 8 + (t & 1) * 4) = w;
-            if (valid && t == 0) scales[blk * C4_UNIT + token] = sb;
+        }
+        if (!is_v && valid) {
+            uint32_t* at = reinterpret_cast<uint32_t*>(codes) + (token * 4 + t) * NB;
+            if constexpr (NB % 4 == 0) {
+#pragma unroll
+                for (int b = 0; b < NB; b += 4) *reinterpret_cast<uint4*>(at + b) = make_uint4(words[b], words[b + 1], words[b + 2], words[b + 3]);
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; b++) at[b] = words[b];
+            }
         }
     }
     if (!is_v) return;
@@ -152,16 +208,17 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* __restr
     const uint32_t have = (0xFFFFu >> (C4_UNIT - u.last)) & (0xFFFFu << u.first);
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) {
-        const int wi = i * 32 + lane, blk = wi / 64, g = wi / 8 % 8, t = wi / 2 % 4, j = wi % 2;
-        const uint8_t* at = vb + (blk * 2 + j) * 8 + g;
-        // byte 2 e + c of a word is token 8 c + 2 t + e
-        const uint32_t mine = have >> (2 * t);
+        const int wi = i * 32 + lane, blk = wi / 64, j = wi % 2;
+        const uint8_t* at = vb + (blk * 2 + j) * 8 + wi / 8 % 8;
+        const int pair = wi / 2 % 4;
+        // byte 2 e + c of a word is token 8 c + 2 pair + e
+        const uint32_t mine = have >> (2 * pair);
         if ((mine & 0x0303u) == 0) continue;
         uint8_t y[4];
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) y[2 * e + c] = at[(8 * c + 2 * t + e) * v_row<NB>()];
+            for (int c = 0; c < 2; c++) y[2 * e + c] = at[(8 * c + 2 * pair + e) * v_row<NB>()];
         if ((mine & 0x0303u) == 0x0303u) {
             reinterpret_cast<uint32_t*>(codes)[wi] = y[0] | y[1] << 8 | y[2] << 16 | static_cast<uint32_t>(y[3]) << 24;
         } else {
@@ -174,13 +231,27 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* __restr
     }
 }
 
+// a bf16 pair's two values at p (8-byte, or 4-byte aligned for 16-bit types, where VEC)
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_pair(T* p, uint32_t pair) {
+    const float lo = __uint_as_float(pair << 16), hi = __uint_as_float(pair & 0xFFFF0000u);
+    if constexpr (!VEC) {
+        p[0] = c4_round<T>(lo);
+        p[1] = c4_round<T>(hi);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2*>(p) = make_float2(lo, hi);
+    } else {
+        alignas(4) T y[2] = {c4_round<T>(lo), c4_round<T>(hi)};
+        *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(y);
+    }
+}
+
 template <typename T, int NB, bool VEC>
-__global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* __restrict__ k, T* __restrict__ v, RowArgs a) {
+__global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* k, T* v, RowArgs a) {
     constexpr int DK = NB * 32;
-    __shared__ uint32_t stage[ROW_WARPS][NB * 72];  // 64 words a block of V, and 8 against bank conflicts
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane / 4, t = lane & 3;
     const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + warp;
     const bool is_v = item & 1;
     const uint32_t h = static_cast<uint32_t>((item >> 1) % a.c.heads);
@@ -188,36 +259,61 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* __restrict__ k,
     if (slot >= a.slots) return;
     const UnitRows u = warp_unit(a, static_cast<uint32_t>(slot), h);
     if (!u.bytes) return;
-    T* x = is_v ? v : k;
-    const size_t xs = is_v ? a.vs : a.ks;
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(u.bytes + (is_v ? 8 * DK : 0));
-    const uint16_t* scales = reinterpret_cast<const uint16_t*>(u.bytes + (is_v ? 17 * DK : 16 * DK));
-    uint32_t* vw = stage[warp];
-    if (is_v) {
+    if (!is_v) {
+        // a lane's words of tokens g and g + 8: eight values of each block
+        uint32_t w[2][NB];
+        uint16_t s[2][NB];
 #pragma unroll
-        for (int i = 0; i < 2 * NB; i++) vw[i / 2 * 72 + i % 2 * 32 + lane] = codes[i * 32 + lane];
-        __syncwarp();
-    }
-#pragma unroll 4
-    for (int pass = 0; pass < 2 * NB; pass++) {
-        const int b = pass * 8 + lane / 4, token = b / NB, blk = b % NB, t = lane & 3;
-        if (token < u.first || token >= u.last) continue;
-        float f[8];
-        if (!is_v) {
-            const uint32_t w = codes[(token * 4 + t) * NB + blk];
-            const float s = c4_bf16(scales[token * NB + blk]);
+        for (int r = 0; r < 2; r++)
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                f[i] = __fmul_rn(static_cast<float>(static_cast<int>(w >> (4 * (i / 2) + 16 * (i % 2)) & 15u) - 8), s);
-        } else {
-            const float s = c4_bf16(scales[blk * C4_UNIT + token]);
-            const int shift = 8 * (2 * (token & 1) + token / 8) + 4 * (t & 1);
+            for (int b = 0; b < NB; b++) {
+                w[r][b] = reinterpret_cast<const uint32_t*>(u.bytes)[((g + 8 * r) * 4 + t) * NB + b];
+                s[r][b] = reinterpret_cast<const uint16_t*>(u.bytes + 16 * DK)[(g + 8 * r) * NB + b];
+            }
 #pragma unroll
-            for (int g = 0; g < 8; g++)
-                f[g] = __fmul_rn(
-                    static_cast<float>(static_cast<int>(vw[blk * 72 + g * 8 + token % 8 / 2 * 2 + t / 2] >> shift & 15u) - 8), s);
+        for (int r = 0; r < 2; r++) {
+            const int token = static_cast<int>(g) + 8 * r;
+            if (token < u.first || token >= u.last) continue;
+            T* to = k + (u.row0 + token) * a.ks + h * DK + 8 * t;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint32_t s2 = s[r][b] | static_cast<uint32_t>(s[r][b]) << 16;
+                const uint32_t p[4] = {c4_pair_any<0>(w[r][b], s2), c4_pair_any<1>(w[r][b], s2), c4_pair_any<2>(w[r][b], s2), c4_pair_any<3>(w[r][b], s2)};
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    f[2 * i] = __uint_as_float(p[i] << 16);
+                    f[2 * i + 1] = __uint_as_float(p[i] & 0xFFFF0000u);
+                }
+                c4_store8<T, VEC>(to + b * 32, f);
+            }
         }
-        c4_store8<T, VEC>(x + (u.row0 + token) * xs + h * DK + blk * 32 + t * 8, f);
+        return;
+    }
+    // A lane's words have pairs of tokens of dimensions g, g + 8, ..: eight by
+    // eight transposes make them pairs of dimensions of token g
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const uint2 w = *reinterpret_cast<const uint2*>(u.bytes + 8 * DK + (b * 32 + lane) * 8);
+        uint32_t s2[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) s2[c] = *reinterpret_cast<const uint32_t*>(u.bytes + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t x = j ? w.y : w.x;
+            uint32_t p[2][2] = {{c4_pair_any<0>(x, s2[0]), c4_pair_any<1>(x, s2[0])}, {c4_pair_any<2>(x, s2[1]), c4_pair_any<3>(x, s2[1])}};
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int token = static_cast<int>(g) + 8 * c;
+                const bool valid = token >= u.first && token < u.last;
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    uint32_t y;
+                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(p[c][r]));
+                    if (valid) store_pair<T, VEC>(v + (u.row0 + token) * a.vs + h * DK + 32 * b + 16 * j + 8 * r + 2 * t, y);
+                }
+            }
+        }
     }
 }
 

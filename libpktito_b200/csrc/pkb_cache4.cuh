@@ -68,13 +68,28 @@ __device__ __forceinline__ uint32_t c4_rows(const Cache4& c, const int32_t* seqs
 // The four pairs of a word's eight codes as bf16 pairs: a nibble n in the
 // top four mantissa bits of 16.0 is 16 + n, and the one fused (16 + n) s
 // - 24 s is c s exactly (24 s has 7 significant bits, c s 8), so neither
-// the conversion nor the scale rounds. Three instructions a pair.
+// the conversion nor the scale rounds. Three instructions a pair. For scales
+// below 2^123 (24 s is finite).
 template <int J>
-__device__ __forceinline__ uint32_t c4_pair(uint32_t w, uint32_t s2, uint32_t m24s2) {
+__device__ __forceinline__ uint32_t c4_sixteens(uint32_t w) {
     const uint32_t at = J == 0 ? w << 3 : w >> (4 * J - 3);
     uint32_t r;
     asm("lop3.b32 %0, %1, 0x00780078, 0x41804180, 0xEA;" : "=r"(r) : "r"(at));  // (at & mask) | 16.0
+    return r;
+}
+template <int J>
+__device__ __forceinline__ uint32_t c4_pair(uint32_t w, uint32_t s2, uint32_t m24s2) {
+    uint32_t r = c4_sixteens<J>(w);
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(r), "r"(s2), "r"(m24s2));
+    return r;
+}
+
+// The same for any scale: 16 + n less 24 first.
+template <int J>
+__device__ __forceinline__ uint32_t c4_pair_any(uint32_t w, uint32_t s2) {
+    uint32_t r;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(c4_sixteens<J>(w)), "r"(0xC1C0C1C0u));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(s2));
     return r;
 }
 
