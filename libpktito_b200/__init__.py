@@ -415,6 +415,7 @@ class Cache4(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "table", "lens", "refs")] + \
                [(n, ctypes.c_uint32) for n in ("n_layers", "n_pages", "max_seqs", "max_pages", "page_tokens", "n_heads",
                                                "head_dim")]
+    device = int32 = None  # of a descriptor made from addresses: nothing to compare a tensor with
 
     @classmethod
     def of(cls, pages, table, lens, refs, page_tokens: int, n_heads: int, head_dim: int) -> "Cache4":
@@ -434,6 +435,7 @@ class Cache4(ctypes.Structure):
         c = cls(_ptr(pages), _ptr(table), _ptr(lens), _ptr(refs), pages.shape[0], refs.shape[0], *table.shape,
                 page_tokens, n_heads, head_dim)
         c.tensors = (pages, table, lens, refs)
+        c.device, c.int32 = pages.get_device(), torch.int32
         return c
 
     @classmethod
@@ -456,8 +458,41 @@ def _type(a) -> int:
     return kind
 
 
-def _bytes(work) -> int:
-    return work.numel() * work.element_size()
+def _work(cache: "Cache4", t) -> tuple:
+    """A work area's address and bytes."""
+    if cache.int32 is not None and (t.get_device() != cache.device or not t.is_contiguous()):
+        raise PkbError(1, f"a work area on {t.device}: in one piece on the cache's device expected")
+    return t.data_ptr(), t.nbytes
+
+
+def _ints(cache: Cache4, t, n: int) -> int:
+    """The address of a list of at least n int32 on the cache's device."""
+    if t is None:
+        return 0
+    if cache.int32 is not None and (t.dtype != cache.int32 or t.numel() < n or t.get_device() != cache.device or
+                                    not t.is_contiguous()):
+        raise PkbError(1, f"a list of {t.numel()} {t.dtype} on {t.device}: {n} int32 in one piece on the cache's device "
+                          f"expected")
+    return t.data_ptr()
+
+
+def _stream_of(cache: Cache4, stream) -> int:
+    """The stream, by default the current one of the cache's device, which has to be the current device."""
+    if stream is not None:
+        return int(stream)
+    import torch
+    at = torch.cuda.current_device()
+    if cache.device not in (None, at):
+        raise PkbError(1, f"a cache on device {cache.device}, the current one is {at}")
+    return torch._C._cuda_getCurrentRawStream(at)
+
+
+def _rows_type(cache: Cache4, a, b) -> int:
+    if a.dtype != b.dtype:
+        raise PkbError(1, f"tensors of {a.dtype} and {b.dtype}")
+    if cache.int32 is not None and not a.get_device() == b.get_device() == cache.device:
+        raise PkbError(1, f"tensors on {a.device} and {b.device}: not the cache's device")
+    return _type(a)
 
 
 def cache4_page_bytes(page_tokens: int, n_heads: int, head_dim: int) -> int:
@@ -469,57 +504,55 @@ def cache4_work_bytes(cache: Cache4) -> int:
 
 
 def cache4_reset_dev(cache: Cache4, stream=None) -> None:
-    _check(lib().pkb_cache4_reset_dev(_stream(stream), ctypes.byref(cache)))
+    _check(lib().pkb_cache4_reset_dev(_stream_of(cache, stream), ctypes.byref(cache)))
 
 
 def cache4_grow_dev(cache: Cache4, seqs, add, n: int, status, work, stream=None) -> None:
     """Room for add[i] more tokens of sequence seqs[i]; status (device int32) as CACHE4_*."""
-    _check(lib().pkb_cache4_grow_dev(_stream(stream), ctypes.byref(cache), _ptr(seqs), _ptr(add), n, _ptr(status),
-                                     _ptr(work), _bytes(work)))
+    _check(lib().pkb_cache4_grow_dev(_stream_of(cache, stream), ctypes.byref(cache), _ints(cache, seqs, n),
+                                     _ints(cache, add, n), n, _ints(cache, status, 1), *_work(cache, work)))
 
 
 def cache4_fork_dev(cache: Cache4, src, dst, lens, n: int, status, work, stream=None) -> None:
     """The empty sequences dst take the first lens tokens of src, sharing their pages."""
-    _check(lib().pkb_cache4_fork_dev(_stream(stream), ctypes.byref(cache), _ptr(src), _ptr(dst), _ptr(lens), n,
-                                     _ptr(status), _ptr(work), _bytes(work)))
+    _check(lib().pkb_cache4_fork_dev(_stream_of(cache, stream), ctypes.byref(cache), _ints(cache, src, n),
+                                     _ints(cache, dst, n), _ints(cache, lens, n), n, _ints(cache, status, 1),
+                                     *_work(cache, work)))
 
 
 def cache4_copy_dev(to: Cache4, cache: Cache4, src, dst, lens, n: int, status, work, stream=None) -> None:
     """The empty sequences dst of `to` take the first lens tokens of src in pages of their own."""
-    _check(lib().pkb_cache4_copy_dev(_stream(stream), ctypes.byref(to), ctypes.byref(cache), _ptr(src), _ptr(dst),
-                                     _ptr(lens), n, _ptr(status), _ptr(work), _bytes(work)))
+    _check(lib().pkb_cache4_copy_dev(_stream_of(cache, stream), ctypes.byref(to), ctypes.byref(cache),
+                                     _ints(cache, src, n), _ints(to, dst, n), _ints(cache, lens, n), n,
+                                     _ints(cache, status, 1), *_work(cache, work)))
 
 
 def cache4_free_dev(cache: Cache4, seqs, n: int, status, work, stream=None) -> None:
-    _check(lib().pkb_cache4_free_dev(_stream(stream), ctypes.byref(cache), _ptr(seqs), n, _ptr(status), _ptr(work),
-                                     _bytes(work)))
+    _check(lib().pkb_cache4_free_dev(_stream_of(cache, stream), ctypes.byref(cache), _ints(cache, seqs, n), n,
+                                     _ints(cache, status, 1), *_work(cache, work)))
 
 
 def cache4_compact_dev(cache: Cache4, used, status, work, stream=None) -> None:
     """Pages in use move to the lowest places; used (device int32 or None): how many there are."""
-    _check(lib().pkb_cache4_compact_dev(_stream(stream), ctypes.byref(cache), _ptr(used), _ptr(status), _ptr(work),
-                                        _bytes(work)))
-
-
-def _same_type(a, b) -> int:
-    if a.dtype != b.dtype:
-        raise PkbError(1, f"tensors of {a.dtype} and {b.dtype}")
-    return _type(a)
+    _check(lib().pkb_cache4_compact_dev(_stream_of(cache, stream), ctypes.byref(cache), _ints(cache, used, 1),
+                                        _ints(cache, status, 1), *_work(cache, work)))
 
 
 def cache4_append_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
                       stream=None) -> None:
     """K and V rows, ks and vs values apart, into the layer: rows starts[i] .. starts[i+1] - 1 are the last
     tokens of sequence seqs[i]."""
-    _check(lib().pkb_cache4_append_dev(_stream(stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
-                                       _same_type(k, v), _ptr(seqs), _ptr(starts), n, rows))
+    _check(lib().pkb_cache4_append_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
+                                       _rows_type(cache, k, v), _ints(cache, seqs, n),
+                                       _ints(cache, starts, n + 1 if n else 0), n, rows))
 
 
 def cache4_read_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
                     stream=None) -> None:
     """What the last tokens of the sequences stand for, into rows of k and v."""
-    _check(lib().pkb_cache4_read_dev(_stream(stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
-                                     _same_type(k, v), _ptr(seqs), _ptr(starts), n, rows))
+    _check(lib().pkb_cache4_read_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
+                                     _rows_type(cache, k, v), _ints(cache, seqs, n),
+                                     _ints(cache, starts, n + 1 if n else 0), n, rows))
 
 
 def attention_cache4_work_bytes(cache: Cache4, H: int, rows: int, n: int) -> int:
@@ -530,6 +563,7 @@ def attention_cache4_dev(o, os_: int, q, qs: int, H: int, cache: Cache4, layer: 
                          max_rows: int, scale: float, causal: bool, window: int, work, stream=None) -> None:
     """Attention of q's rows (H heads) over the cache's layer: rows starts[i] .. starts[i+1] - 1 are the last
     positions of sequence seqs[i]; window 0: the whole history."""
-    _check(lib().pkb_attention_cache4_dev(_stream(stream), _ptr(o), os_, _ptr(q), qs, _same_type(o, q), H,
-                                          ctypes.byref(cache), layer, _ptr(seqs), _ptr(starts), n, rows, max_rows, scale,
-                                          int(causal), window, _ptr(work), _bytes(work)))
+    _check(lib().pkb_attention_cache4_dev(_stream_of(cache, stream), _ptr(o), os_, _ptr(q), qs, _rows_type(cache, o, q),
+                                          H, ctypes.byref(cache), layer, _ints(cache, seqs, n),
+                                          _ints(cache, starts, n + 1 if n else 0), n, rows, max_rows, scale,
+                                          int(causal), window, *_work(cache, work)))

@@ -955,7 +955,8 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     if ((rc = c4_check_type(type, who))) return rc;
     if (layer >= c->n_layers) return set_error(PKB_EINVAL, "%s: layer %u of %u", who, layer, c->n_layers);
     if (!H || H % c->n_heads) return set_error(PKB_EINVAL, "%s: H = %u, a multiple of the cache's %u heads", who, H, c->n_heads);
-    if (!(scale - scale == 0.0f)) return set_error(PKB_EINVAL, "%s: scale is not finite", who);
+    a.scale = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074);  // log2 e
+    if (!(a.scale - a.scale == 0.0f)) return set_error(PKB_EINVAL, "%s: scale log2 e is not finite", who);
     if (window > INT_MAX) return set_error(PKB_EINVAL, "%s: window = %u", who, window);
     // one that reaches past every sequence's first token from its last row on is none
     if (window >= static_cast<uint64_t>(c->max_pages) * c->page_tokens + max_rows) window = 0;
@@ -988,7 +989,6 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     a.G = H / c->n_heads;
     a.vec = is_aligned(q, 16) && qs * size % 16 == 0;
     a.vec_o = is_aligned(o, 16) && os * size % 16 == 0;
-    a.scale = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074);  // log2 e
     a.causal = causal ? 1 : 0;
     a.window = window;
     a.timeout = wait_cycles();

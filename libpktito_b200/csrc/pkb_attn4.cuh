@@ -138,6 +138,12 @@ struct Entry {
     __device__ __forceinline__ int32_t position(uint32_t tok) const { return static_cast<int32_t>(len - rows + tok); }
 };
 
+// The first key that a row at `pos` (below 0 before the first token) sees.
+__device__ __forceinline__ int32_t window_begin(const Attn4Args& a, int32_t pos) {
+    const int32_t window = static_cast<int32_t>(a.window);
+    return window && pos >= window ? pos - window + 1 : 0;
+}
+
 __device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
     Entry e;
     e.rows = c4_rows(a.c, a.seqs, a.starts, i, a.rows, &e.seq, &e.r0, a.err);
@@ -147,8 +153,7 @@ __device__ __forceinline__ Entry load_entry(const Attn4Args& a, uint32_t i) {
     }
     e.len = e.rows ? c4_len(a.c, e.seq, a.err) : 0;
     // the first row's window begins furthest back; the last row's causal end is len
-    const int32_t lo = a.window ? e.position(0) - static_cast<int32_t>(a.window) + 1 : 0;
-    e.unit0 = lo > 0 ? static_cast<uint32_t>(lo) / C4_UNIT : 0;
+    e.unit0 = static_cast<uint32_t>(window_begin(a, e.position(0))) / C4_UNIT;
     e.units = (e.len + C4_UNIT - 1) / C4_UNIT - e.unit0;
     e.places = e.len ? START + (e.units + 1) / 2 : 0;
     return e;
@@ -160,7 +165,7 @@ struct Keys {
 };
 __device__ __forceinline__ Keys keys_of(const Attn4Args& a, const Entry& e, uint32_t tok) {
     const int32_t pos = e.position(tok), len = static_cast<int32_t>(e.len);
-    return {a.window ? max(pos - static_cast<int32_t>(a.window) + 1, 0) : 0, a.causal ? max(min(pos + 1, len), 0) : len};
+    return {window_begin(a, pos), a.causal ? max(min(pos + 1, len), 0) : len};
 }
 
 // Many bf16 rows on the fifth-generation tensor cores (pkb_attn4_tc.cu): whether

@@ -135,6 +135,39 @@ def test_descriptor_checks_its_tensors():
         P.Cache4.of(pages, table, lens, refs, 16, 2, 48)
 
 
+def test_calls_check_their_tensors():
+    import torch
+    c = P.Cache4.of(torch.zeros((1, 5, P.cache4_page_bytes(16, 2, 32)), dtype=torch.uint8), torch.zeros((3, 4), dtype=torch.int32),
+                    torch.zeros(3, dtype=torch.int32), torch.zeros(5, dtype=torch.int32), 16, 2, 32)
+    good, work, rows = torch.zeros(4, dtype=torch.int32), torch.zeros(1 << 16, dtype=torch.uint8), torch.zeros((4, 64))
+    bad = [good.long(), good[:1], torch.zeros(8, dtype=torch.int32)[::2], good.float(), good.to("meta")]
+    for x in bad:
+        calls = [lambda: P.cache4_grow_dev(c, x, good, 2, good, work, 0), lambda: P.cache4_grow_dev(c, good, x, 2, good, work, 0),
+                 lambda: P.cache4_free_dev(c, x, 2, good, work, 0)]
+        calls += [lambda i=i: P.cache4_fork_dev(c, *[x if i == j else good for j in range(3)], 2, good, work, 0) for i in range(3)]
+        calls += [lambda i=i: P.cache4_copy_dev(c, c, *[x if i == j else good for j in range(3)], 2, good, work, 0) for i in range(3)]
+        calls += [lambda i=i: P.cache4_append_dev(c, 0, rows, 64, rows, 64, *[x if i == j else good for j in range(2)], 2, 4, 0)
+                  for i in range(2)]
+        calls += [lambda i=i: P.attention_cache4_dev(rows, 64, rows, 64, 2, c, 0, *[x if i == j else good for j in range(2)], 2, 4, 4,
+                                                     0.1, True, 0, work, 0) for i in range(2)]
+        for call in calls:
+            with pytest.raises(P.PkbError):
+                call()
+    for k, v in ((rows, rows.half()), (rows.int(), rows.int()), (rows.to("meta"), rows), (rows, rows.to("meta"))):
+        with pytest.raises(P.PkbError):
+            P.cache4_read_dev(c, 0, k, 64, v, 64, good, good, 2, 4, 0)
+    for area in (work.to("meta"), work[::2]):
+        with pytest.raises(P.PkbError):
+            P.cache4_compact_dev(c, None, good, area, 0)
+    with pytest.raises(P.PkbError):
+        P.cache4_compact_dev(c, None, good.long(), work, 0)
+
+
+def test_a_scale_that_overflows_is_refused():
+    assert attend(scale=3.0e38) == EINVAL  # times log2 e
+    assert attend(scale=-3.0e38) == EINVAL
+
+
 @pytest.mark.parametrize("dk", [32, 64, 96, 128, 256])
 def test_every_nibble_is_one_values(dk):
     for at in R.nibble_places(dk):

@@ -162,7 +162,7 @@ def filled(lens, page, heads, dk, seed, layers=1, spread=1.0, **kw):
 def check_attention(c, lens, rows, seqs, G, kind, causal, window, layer=0, scale=None, seed=1, pad=0, tail=0, q=None, max_rows=None):
     heads, dk, page = c.n_heads, c.head_dim, c.page_tokens
     H, n, starts = heads * G, sum(rows), np.concatenate([[0], np.cumsum(rows)])
-    scale = scale or dk ** -0.5
+    scale = dk ** -0.5 if scale is None else scale
     g = torch.Generator("cuda").manual_seed(seed)
     if q is None:
         q = torch.randn((n + tail, H * dk), generator=g, device="cuda").to(KIND[kind])
@@ -300,6 +300,106 @@ def test_bad_tables_and_sequences_do_not_reach_memory():
     c.tensors[2][1] = 40
     c.tensors[1][0, 1], c.tensors[1][1, 0] = -7, 1 << 30
     assert run([0, 1], [0, 1, 2]) == 2
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,G,dk", [(17, 1, 32), (20, 3, 64), (33, 2, 32), (40, 1, 128)])
+def test_more_heads_than_a_team(kind, heads, G, dk):
+    lens = [1, 900, 33, 0, 250]
+    c = filled(lens, 16, heads, dk, seed=heads)
+    check_attention(c, lens, [1] * 5, [4, 1, 3, 0, 2], G, kind, True, 0)
+    check_attention(c, lens, [1, 5, 2, 1, 3], [4, 1, 3, 0, 2], G, kind, True, 70)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 3, 150])  # one part, some rows, a prompt
+def test_padded_entries_and_a_sequence_listed_twice(kind, rows):
+    lens = [160, 400, 151]
+    c = filled(lens, 32, 2, 64, seed=13)
+    r = [0, rows, 0, 1, rows, 0, rows]
+    check_attention(c, lens + [0], r, [-1, 1, 2, 0, 1, 99, 2], 1, kind, True, 0, tail=5)
+    check_attention(c, lens, [rows, rows], [2, 0], 2, kind, False, 2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 200])
+def test_a_scale_of_zero_is_the_mean(kind, rows):
+    lens = [333, 201]
+    c = filled(lens, 32, 2, 64, seed=9)
+    check_attention(c, lens, [rows, rows], [0, 1], 1, kind, True, 0, scale=0.0)
+
+
+@pytest.mark.parametrize("most,rows", [(1, 2), (4, 5), (140, 141)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_more_rows_than_said_set_the_error_word(kind, most, rows):
+    lens = [300, 300]
+    c = filled(lens, 16, 1, 32, seed=6)
+    n = rows + most
+    q = torch.randn((n, 32), device="cuda").to(KIND[kind])
+    o, work = torch.empty_like(q), torch.empty(P.attention_cache4_work_bytes(c, 1, n, 2), dtype=torch.uint8, device="cuda")
+    P.attention_cache4_dev(o, 32, q, 32, 1, c, 0, ints([0, 1]), ints([0, most, n]), 2, n, most, 0.1, True, 0, work)
+    torch.cuda.synchronize()
+    assert P.device_errors(0) == 2
+    alone = torch.empty_like(q)
+    P.attention_cache4_dev(alone, 32, q, 32, 1, c, 0, ints([0]), ints([0, most]), 1, n, most, 0.1, True, 0, work)
+    no_errors()
+    assert torch.allclose(o[:most].float(), alone[:most].float(), rtol=2 * HALF[kind] + 1e-5, atol=1e-5)  # the other entry's rows
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("rows", [3, 260])
+def test_a_row_that_is_not_finite_stays_its_own(kind, value, rows):
+    lens, H, dk = [300], 2, 64
+    c = filled(lens, 16, 1, dk, seed=4)
+    q = torch.randn((rows, H * dk), generator=torch.Generator("cuda").manual_seed(3), device="cuda").to(KIND[kind])
+    o, work = torch.empty_like(q), torch.empty(P.attention_cache4_work_bytes(c, H, rows, 1), dtype=torch.uint8, device="cuda")
+    args = (H, c, 0, ints([0]), ints([0, rows]), 1, rows, rows, 0.1, True, 0, work)
+    P.attention_cache4_dev(o, H * dk, q, H * dk, *args)
+    clean = o.clone()
+    q[1, dk:] = value
+    P.attention_cache4_dev(o, H * dk, q, H * dk, *args)
+    no_errors()
+    assert o[1, dk:].isnan().all()
+    o[1, dk:] = clean[1, dk:]
+    assert torch.equal(o, clean)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_offsets_past_32_bits(kind):
+    """The last pages of a layer's 2.2 GB, in the second layer: the same bits as from a small cache, and page copies."""
+    heads, dk, page, n_pages = 8, 256, 256, 3700
+    lens, rows = [700, 300], [300, 1]
+    small = P.Cache4.empty(1, 5, 3, 4, page, heads, dk)
+    large = P.Cache4.empty(2, n_pages, 3, 4, page, heads, dk)
+    assert large.tensors[0].numel() > 2 ** 32
+    k, v = torch.randn((2, 1000, heads * dk), generator=torch.Generator("cuda").manual_seed(2), device="cuda").to(KIND[kind])
+    q = torch.randn((301, heads * dk), generator=torch.Generator("cuda").manual_seed(3), device="cuda").to(KIND[kind])
+    got = []
+    for c, layer, last in ((small, 0, 4), (large, 1, n_pages - 1)):
+        c.tensors[1][0, :3], c.tensors[1][1, :2] = ints([last, last - 2, last - 1]), ints([last - 4, last - 3])
+        c.tensors[2][:2] = ints(lens)
+        c.tensors[3][last - 4:last + 1] = 1
+        append(c, layer, k, v, [0, 1], lens)
+        out = []
+        for r, most in ((rows, 300), ([1, 1], 1)):
+            n = sum(r)
+            o, work = torch.empty_like(q[:n]), torch.empty(P.attention_cache4_work_bytes(c, heads, n, 2), dtype=torch.uint8, device="cuda")
+            P.attention_cache4_dev(o, heads * dk, q, heads * dk, heads, c, layer, ints([0, 1]), ints([0, r[0], n]), 2, n, most, 0.06,
+                                   True, 0, work)
+            out.append(o)
+        ko, vo = torch.empty_like(k), torch.empty_like(v)
+        P.cache4_read_dev(c, layer, ko, heads * dk, vo, heads * dk, ints([0, 1]), ints([0, *np.cumsum(lens)]), 2, 1000)
+        no_errors()
+        got.append(out + [ko, vo])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    status, work = ints([9]), torch.empty(P.cache4_work_bytes(large), dtype=torch.uint8, device="cuda")
+    P.cache4_copy_dev(large, large, ints([0]), ints([2]), ints([700]), 1, status, work)  # to the first pages
+    P.cache4_read_dev(large, 1, ko, heads * dk, vo, heads * dk, ints([2]), ints([0, 700]), 1, 1000)
+    no_errors()
+    assert int(status) == 0 and large.tensors[1][2].tolist() == [0, 1, 2, -1]
+    assert torch.equal(ko, got[0][2]) and torch.equal(vo, got[0][3])
 
 
 # ------------------------------------------------------------- page operations --
@@ -526,6 +626,44 @@ def test_steps_in_a_graph():
             y, size, score = R.attention(q[s:s + 1].double().cpu().numpy().reshape(1, heads, dk), kk, vv, kk.shape[1], 0.125, True, 0)
             assert np.array_equal(kk[:, -1], R.held(k[s].double().cpu().numpy().reshape(heads, dk)))
             assert np.abs(o[s].double().cpu().numpy().reshape(y.shape) - y).max() <= 1e-5 * (1 + score.max()) * size.max()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_chunked_prompt_in_a_graph(kind):
+    """A chunk of 160 rows a replay: pages taken, rows appended and attended, lengths and pages moving on the device."""
+    heads, dk, G, page, n = 2, 64, 2, 16, 160
+    x = Both(80, 2, 40, page, heads, dk, 1)
+    g = torch.Generator("cuda").manual_seed(4)
+    k, v = torch.empty((2, n, heads * dk), device="cuda").to(KIND[kind])
+    q = torch.empty((n, G * heads * dk), device="cuda").to(KIND[kind])
+    o = torch.empty_like(q)
+    seqs, starts, add = ints([1]), ints([0, n]), ints([n])
+    work = torch.empty(P.attention_cache4_work_bytes(x.c, G * heads, n, 1), dtype=torch.uint8, device="cuda")
+
+    def step(to):
+        P.attention_cache4_dev(to, G * heads * dk, q, G * heads * dk, G * heads, x.c, 0, seqs, starts, 1, n, n, 0.125, True, 200, work)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        P.cache4_grow_dev(x.c, seqs, add, 1, x.status, x.work)
+        P.cache4_append_dev(x.c, 0, k, heads * dk, v, heads * dk, seqs, starts, 1, n)
+        step(o)
+    for i in range(4):
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert x.b.grow([1], [n]) == 0
+        x.raw = x.c.tensors[0].cpu().numpy().copy()
+        x.same(0)
+        again = torch.empty_like(o)
+        step(again)
+        no_errors()
+        assert torch.equal(o, again)
+        assert check_attention(x.c, x.b.lens, [n], [1], G, kind, True, 200, scale=0.125, q=q) <= 1
+    graph.replay()  # 640 tokens are all that a table row has room for
+    torch.cuda.synchronize()
+    assert int(x.status) == P.CACHE4_LONG and P.device_errors(0) == 0
 
 
 def test_two_streams_with_work_areas_of_their_own():
