@@ -38,7 +38,7 @@ constexpr int JOIN_WARPS = 8;
 constexpr int TILE = 32;            // keys of a tile: two units
 constexpr uint32_t MAX_ENTRIES = 1024;  // sequences of one launch
 constexpr uint32_t MAX_TEAM = 16;
-constexpr uint32_t SPLIT_ROWS = 128;   // rows of an entry and cached head that are split along the keys; more are many
+constexpr uint32_t SPLIT_ROWS = 1024;   // rows of an entry and cached head that may be split along the keys
 constexpr int MAX_GRID = 160;
 constexpr int MAX_WORKERS = 16;
 
@@ -433,7 +433,9 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
         longest = max(longest, most[w]);
     }
     // Where no item is longer than one and a half shares, shares take whole
-    // items: there is nothing to join then.
+    // items: there is nothing to join then (200 sequences of 512 tokens, 8
+    // heads of 64, 4 rows each: 29.3 us in equal shares, 28.1 in whole items;
+    // 40 of 700 tokens, one row each: 15.5 and 15.9).
     const uint32_t room = min(gridDim.x * WORKERS / a.team, a.max_shares), places = static_cast<uint32_t>(total);
     const bool whole = 2ull * longest * room <= 3ull * places;
 #pragma unroll
@@ -855,15 +857,16 @@ cudaError_t prepare_type() {
 }
 
 template <typename T, int NB, int NT, int PARTS>
-cudaError_t launch_one(Attn4Args a, int sms, cudaStream_t s) {
-    if (a.max_rows * a.G > SPLIT_ROWS) {
-        const uint32_t most = ROW_WARPS * 8 * NT;
-        const dim3 grid((a.max_rows * a.G + most - 1) / most, a.c.heads, a.n);
-        const cudaError_t e = c4_launch(rows_kernel<T, NB, NT, PARTS>, grid, (ROW_WARPS + 1) * 32, ROW_STAGES * tile_bytes<NB>(), s, a);
-        if (e == cudaSuccess) count_launch();
-        return e;
-    }
-    const uint32_t grid = static_cast<uint32_t>(sms < MAX_GRID ? sms : MAX_GRID);
+cudaError_t launch_rows(const Attn4Args& a, cudaStream_t s) {
+    const uint32_t most = ROW_WARPS * 8 * NT;
+    const dim3 grid((a.max_rows * a.G + most - 1) / most, a.c.heads, a.n);
+    const cudaError_t e = c4_launch(rows_kernel<T, NB, NT, PARTS>, grid, (ROW_WARPS + 1) * 32, ROW_STAGES * tile_bytes<NB>(), s, a);
+    if (e == cudaSuccess) count_launch();
+    return e;
+}
+
+template <typename T, int NB, int NT, int PARTS>
+cudaError_t launch_split(Attn4Args a, uint32_t grid, cudaStream_t s) {
     a.max_blocks = (a.max_rows * a.G + 8 * NT - 1) / (8 * NT);
     cudaError_t e = c4_launch(split_kernel<T, NB, NT, PARTS>, grid, workers<NB, NT>() * 32, split_smem<NB, NT>(a.n), s, a);
     if (e != cudaSuccess) return e;
@@ -874,20 +877,26 @@ cudaError_t launch_one(Attn4Args a, int sms, cudaStream_t s) {
     uint32_t ways = 1;
     while (ways < 8 && shares > 4 * ways * items) ways *= 2;
     const uint32_t quads = JOIN_WARPS / ways;
-    e = c4_launch(ways > 1 ? join_kernel<T, NB, NT, 8> : join_kernel<T, NB, NT, 4>, dim3(static_cast<uint32_t>(items * a.team), (2 * NB * NT + quads - 1) / quads), JOIN_WARPS * 32, 0, s, a, ways);
+    e = c4_launch(ways > 1 ? join_kernel<T, NB, NT, 8> : join_kernel<T, NB, NT, 4>,
+                  dim3(static_cast<uint32_t>(items * a.team), (2 * NB * NT + quads - 1) / quads), JOIN_WARPS * 32, 0, s, a, ways);
     if (e == cudaSuccess) count_launch();
     return e;
 }
 
+template <typename T, int NB, int NT, int PARTS>
+cudaError_t launch_one(const Attn4Args& a, uint32_t grid, bool split, cudaStream_t s) {
+    return split ? launch_split<T, NB, NT, PARTS>(a, grid, s) : launch_rows<T, NB, NT, PARTS>(a, s);
+}
+
 template <typename T, int PARTS>
-cudaError_t launch_type(const Attn4Args& a, int sms, cudaStream_t s) {
+cudaError_t launch_type(const Attn4Args& a, uint32_t grid, bool split, cudaStream_t s) {
     const bool two = static_cast<uint64_t>(a.max_rows) * a.G > 8;  // more than eight rows: two blocks of eight share the codes' conversion
     switch (a.c.dk) {
-        case 32: return two ? launch_one<T, 1, 2, PARTS>(a, sms, s) : launch_one<T, 1, 1, PARTS>(a, sms, s);
-        case 64: return two ? launch_one<T, 2, 2, PARTS>(a, sms, s) : launch_one<T, 2, 1, PARTS>(a, sms, s);
-        case 96: return two ? launch_one<T, 3, 2, PARTS>(a, sms, s) : launch_one<T, 3, 1, PARTS>(a, sms, s);
-        case 128: return two ? launch_one<T, 4, 2, PARTS>(a, sms, s) : launch_one<T, 4, 1, PARTS>(a, sms, s);
-        default: return launch_one<T, 8, 1, PARTS>(a, sms, s);
+        case 32: return two ? launch_one<T, 1, 2, PARTS>(a, grid, split, s) : launch_one<T, 1, 1, PARTS>(a, grid, split, s);
+        case 64: return two ? launch_one<T, 2, 2, PARTS>(a, grid, split, s) : launch_one<T, 2, 1, PARTS>(a, grid, split, s);
+        case 96: return two ? launch_one<T, 3, 2, PARTS>(a, grid, split, s) : launch_one<T, 3, 1, PARTS>(a, grid, split, s);
+        case 128: return two ? launch_one<T, 4, 2, PARTS>(a, grid, split, s) : launch_one<T, 4, 1, PARTS>(a, grid, split, s);
+        default: return launch_one<T, 8, 1, PARTS>(a, grid, split, s);
     }
 }
 
@@ -899,26 +908,49 @@ void teams_of(uint32_t heads, uint32_t* team, uint32_t* teams) {
     *team = (heads + *teams - 1) / *teams;
 }
 
-// A call's bounds, over any lengths that the cache's table has room for: the
-// entries of a launch, its shares, and the bytes of the work area: a join an
-// item (an entry, head and eight rows), two parts a share and head. Only
-// entries of up to SPLIT_ROWS rows are split.
+// Places of a sequence at most, whatever its length: they are counted in 32 bits.
+uint64_t places_of(const pkb_cache4* c) { return static_cast<uint64_t>(c->max_pages) * c->page_tokens / TILE + 1 + START; }
+
+// Whether `rows` rows of each of n entries are split along the keys, or taken
+// by blocks that go over all of an entry's keys. Lengths are not known here,
+// but both ways' times are proportional to them, so only the grids count:
+//  - bf16 on tcgen05: 16 rows of a split take the GPU as long as half an SM
+//    takes to do 256 (8 sequences of 2,048 tokens, 8 heads of 128 with 4 query
+//    heads each: 16 tokens 43 us split and 41 so, 32 tokens 64 and 42; one
+//    sequence of 8,192 tokens: 64 tokens 67 and 160).
+//  - others: rows_kernel's warps are as fast as the split's, and leave out what
+//    a prompt's rows cannot see, half of it at most: it is worth an
+//    SM's eight warps where half of all SMs' have work (float rows of 24
+//    sequences of 600 tokens, 100 tokens each: 53 us split and 61 so; of one
+//    sequence of 8,192, 64 tokens with 4 query heads each: 92 and 728).
+bool splits(const Attn4Args& a, int type, uint32_t n, uint32_t grid) {
+    const uint64_t rows = static_cast<uint64_t>(a.max_rows) * a.G, heads = static_cast<uint64_t>(n) * a.teams * a.team;
+    if (rows > SPLIT_ROWS) return false;
+    const bool tc = attention4_tc_takes(a, type);
+    const uint64_t block = a.c.dk == 256 || rows <= 8 ? 8 : 16, blocks = (rows + block - 1) / block;
+    if (!tc && rows <= 128) return true;
+    const uint64_t many = tc ? 256 : ROW_WARPS * block, waves = (heads * ((rows + many - 1) / many) + grid - 1) / grid;
+    return heads * blocks <= (tc ? 2 : 4) * grid * waves;
+}
+
+// The work area of a call, over any lengths and max_rows: a join an item (an
+// entry, head and block of rows), two parts a share and head. Where more than
+// 128 rows are split, `splits` holds heads times blocks below
+// 4 (16 heads + MAX_GRID) for blocks of eight rows, 4 (8 heads + MAX_GRID) for
+// sixteen.
 struct Bounds {
-    uint64_t entries, shares, join_bytes, bytes;
+    uint64_t shares, join_bytes, bytes;
 };
 
 Bounds bounds_of(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
     uint32_t team, teams;
     teams_of(c->n_heads, &team, &teams);
-    const uint64_t G = H / c->n_heads, tiles = static_cast<uint64_t>(c->max_pages) * c->page_tokens / TILE + 1 + START;
-    const uint64_t blocks = rows * G < SPLIT_ROWS ? (rows * G + 7) / 8 : SPLIT_ROWS / 8;
+    const uint64_t all = static_cast<uint64_t>(rows) * (H / c->n_heads), blocks = all < 512 ? (all + 7) / 8 : 64;
+    const uint64_t items = static_cast<uint64_t>(n < MAX_ENTRIES ? n : MAX_ENTRIES) * teams * team * blocks + (all > 128 ? 4 * MAX_GRID : 0);
+    const uint64_t most = static_cast<uint64_t>(MAX_GRID) * MAX_WORKERS / team, places = items / team * places_of(c);
     Bounds b;
-    b.entries = n < MAX_ENTRIES ? n : MAX_ENTRIES;
-    // places are counted in 32 bits
-    if (b.entries > INT_MAX / (teams * tiles * blocks)) b.entries = INT_MAX / (teams * tiles * blocks);
-    const uint64_t most = static_cast<uint64_t>(MAX_GRID) * MAX_WORKERS / team, places = b.entries * teams * tiles * blocks;
     b.shares = places < most ? places : most;
-    b.join_bytes = (b.entries * teams * team * blocks * sizeof(Attn4Join) + 255) & ~static_cast<uint64_t>(255);
+    b.join_bytes = (items * sizeof(Attn4Join) + 255) & ~static_cast<uint64_t>(255);
     b.bytes = b.join_bytes + 2 * b.shares * team * (c->head_dim == 256 ? 1 : 2) * (c->head_dim / 4 + 4) * 128;
     return b;
 }
@@ -975,8 +1007,6 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     const Bounds bounds = bounds_of(c, H, rows, n);
     if (work_bytes < bounds.bytes || !is_aligned(work, 256))
         return set_error(PKB_EINVAL, "%s: work area of %zu bytes (%zu needed, 256-byte aligned)", who, work_bytes, static_cast<size_t>(bounds.bytes));
-    if (!bounds.entries || (static_cast<uint64_t>(max_rows) * (H / c->n_heads) > SPLIT_ROWS && c->n_heads > 65535))
-        return set_error(PKB_EINVAL, "%s: %u heads of sequences of up to %u pages are too many", who, c->n_heads, c->max_pages);
     int sms;
     if ((rc = current_device_info(&sms, &a.err))) return rc;
     a.q = q;
@@ -998,16 +1028,19 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + bounds.join_bytes);
     a.max_shares = static_cast<uint32_t>(bounds.shares);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const uint32_t step = static_cast<uint32_t>(bounds.entries);
+    const uint32_t grid = static_cast<uint32_t>(sms < MAX_GRID ? sms : MAX_GRID);
+    // entries of a launch: a split's places are counted in 32 bits
+    const uint64_t entry = places_of(c) * a.teams * ((static_cast<uint64_t>(max_rows) * a.G + 7) / 8);
+    const bool split = splits(a, type, n, grid) && entry <= UINT_MAX;
+    const uint32_t step = split && UINT_MAX / entry < MAX_ENTRIES ? static_cast<uint32_t>(UINT_MAX / entry) : MAX_ENTRIES;
     for (uint32_t i = 0; i < n; i += step) {
         a.seqs = seqs + i;
         a.starts = starts + i;
         a.n = n - i < step ? n - i : step;
-        const bool many = a.max_rows * a.G > SPLIT_ROWS;
-        const cudaError_t e = many && attention4_tc_takes(a, type) ? launch_attention4_tc(a, s)
-                              : type == PKB_F32   ? launch_type<float, 3>(a, sms, s)
-                              : type == PKB_F16 ? launch_type<__half, 2>(a, sms, s)
-                                                : launch_type<__nv_bfloat16, 1>(a, sms, s);
+        const cudaError_t e = !split && attention4_tc_takes(a, type) ? launch_attention4_tc(a, s)
+                              : type == PKB_F32 ? launch_type<float, 3>(a, grid, split, s)
+                              : type == PKB_F16 ? launch_type<__half, 2>(a, grid, split, s)
+                                                : launch_type<__nv_bfloat16, 1>(a, grid, split, s);
         if (e != cudaSuccess)
             return set_error(e == cudaErrorMemoryAllocation ? PKB_ENOMEM : PKB_ECUDA, "%s launch: %s", who, cudaGetErrorString(e));
     }
