@@ -40,9 +40,10 @@ constexpr int THREADS = 640;    // five warpgroups; the last one's three spare w
 // 60,416.
 constexpr int SOFT_REGS = 152, CODE_REGS = 64, ISSUE_REGS = 40;
 constexpr int ROWS = 256;       // of a block, two tiles of 128
-constexpr int KEYS = 128;       // of a step
+constexpr int KEYS = 128;       // of a step of K and V
+constexpr int HALF = 64;        // of a product
 constexpr int KV_STAGES = 2;    // steps of K and of V as bf16
-constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;  // S (and P) of the tiles at 0 and 128, O at 256 and 384
+constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;  // S (and P) of two halves of each tile from 0 on, O at 256 and 384
 
 template <int NB> constexpr int slabs() { return (NB + 1) / 2; }             // of 64 dimensions, 128 rows of 128 bytes each
 template <int NB> constexpr int row_tile() { return slabs<NB>() * 16384; }    // 128 rows of Q or of K
@@ -53,7 +54,7 @@ template <int NB> constexpr int smem_bytes() {
 
 struct Bars {
     uint64_t k_full[KV_STAGES], k_empty[KV_STAGES], v_full[KV_STAGES], v_empty[KV_STAGES];
-    uint64_t s_full[2], p_full[2], o_full[2], drain;
+    uint64_t s_full[2][2], p_full[2][2], o_full[2][2], drain;  // of each tile and parity of its half steps
 };
 
 // One lane of a converged warp. The issuing warp runs its loop as a whole
@@ -263,14 +264,13 @@ __device__ __forceinline__ float largest(const uint32_t (&s)[32], int32_t first,
     return fmaxf(top, other);
 }
 
-// Raises a row's maximum to that of its 128 scores at s_at, and rescales its
-// sum and its values (those of the steps before: the scores' commit covers
-// them).
+// Raises a row's maximum to that of its 64 scores at s_at, and rescales its
+// sum and its values, which no product is adding to.
 template <int NB, int MASK>
 __device__ __noinline__ void raise(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l) {
     float top = NEG_INF;
 #pragma unroll 1
-    for (int c = 0; c < 4; c++) {
+    for (int c = 0; c < HALF / 32; c++) {
         uint32_t a[32];
         tmem_ld_32x32b_x32(s_at + 32 * c, a);
         tmem_ld_wait(a);
@@ -291,17 +291,18 @@ __device__ __noinline__ void raise(uint32_t s_at, uint32_t o_at, bool begun, flo
     tmem_st_wait();
 }
 
-// A step of a row: its 128 scores at s_at become P in the upper half of their
-// place. The weights are taken with the maximum there is, while the scores'
-// own is looked for; where that passes it by 8 (the first step, and few
-// others) the maximum is raised and they are taken again: nothing of S is
-// overwritten before its last columns have been seen.
-template <int NB, int MASK>
-__device__ __forceinline__ void softmax_step(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l) {
+// A half step of a row: its 64 scores at s_at become P in the upper half of
+// their place. The weights are taken with the maximum there is, and the
+// scores' own is found beside them; where that passes it by 8 (the first
+// step, and few others) the maximum is raised, once the products of the half
+// step before have ended (`idle`), and they are taken again.
+template <int NB, int MASK, typename Idle>
+__device__ __forceinline__ bool softmax_step(uint32_t s_at, uint32_t o_at, bool begun, float scale, int32_t first, int32_t end, float& m, float& l,
+                                             Idle idle) {
     const uint64_t scale2 = pack2(scale, scale);
     if (!begun) raise<NB, MASK>(s_at, o_at, begun, scale, first, end, m, l);
     for (;;) {
-        uint32_t a[32], b[32], z0[16], z1[16], z2[16];
+        uint32_t a[32], b[32], z0[16], z1[16];
         const float minus = m == NEG_INF ? 0.0f : -m;
         const uint64_t minus2 = pack2(minus, minus);
         uint64_t sum[2] = {0, 0};
@@ -311,29 +312,20 @@ __device__ __forceinline__ void softmax_step(uint32_t s_at, uint32_t o_at, bool 
         float top = NEG_INF;
         weights<MASK>(a, scale2, minus2, first, end, sum, z0, top);
         tmem_ld_wait(b);
-        tmem_ld_32x32b_x32(s_at + 64, a);
         weights<MASK>(b, scale2, minus2, first - 32, end - 32, sum, z1, top);
-        tmem_ld_wait(a);
-        tmem_ld_32x32b_x32(s_at + 96, b);
-        weights<MASK>(a, scale2, minus2, first - 64, end - 64, sum, z2, top);
-        tmem_ld_wait(b);
-        top = largest<MASK>(b, first - 96, end - 96, top);
         if (__any_sync(FULL, __fmul_rn(top, scale) > m + 8.0f)) {
+            if (!idle()) return false;
             raise<NB, MASK>(s_at, o_at, begun, scale, first, end, m, l);
             continue;
         }
-        tmem_st_x16(s_at + 64, z0);
-        tmem_st_x16(s_at + 80, z1);
-        tmem_st_x16(s_at + 96, z2);
-        float seen = top;
-        weights<MASK>(b, scale2, minus2, first - 96, end - 96, sum, z0, seen);
-        tmem_st_x16(s_at + 112, z0);
+        tmem_st_x16(s_at + 32, z0);
+        tmem_st_x16(s_at + 48, z1);
         float s0, s1, s2, s3;
         unpack2(sum[0], s0, s1);
         unpack2(sum[1], s2, s3);
         l += (s0 + s1) + (s2 + s3);
         tmem_st_wait();
-        break;
+        return true;
     }
 }
 
@@ -360,7 +352,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             mbar_init(&bars.k_full[i], CODE_WARPS), mbar_init(&bars.v_full[i], CODE_WARPS);
             mbar_init(&bars.k_empty[i], 1), mbar_init(&bars.v_empty[i], 1);
         }
-        for (int i = 0; i < 2; i++) mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_full[i], 4), mbar_init(&bars.o_full[i], 1);
+        for (int i = 0; i < 4; i++)
+            mbar_init(&bars.s_full[i / 2][i % 2], 1), mbar_init(&bars.p_full[i / 2][i % 2], 4), mbar_init(&bars.o_full[i / 2][i % 2], 1);
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
         gave_up = 0;
@@ -377,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     const int32_t lo = keys_of(a, e, row0 / a.G).lo, hi = keys_of(a, e, last / a.G).hi;
     const uint32_t unit0 = static_cast<uint32_t>(lo / C4_UNIT);
     const uint32_t units = hi > lo ? static_cast<uint32_t>((hi + C4_UNIT - 1) / C4_UNIT) - unit0 : 0;
-    const uint32_t steps = (units * C4_UNIT + KEYS - 1) / KEYS;
+    const uint32_t steps = (units * C4_UNIT + KEYS - 1) / KEYS, halves = (units * C4_UNIT + HALF - 1) / HALF;
     const int32_t key_base = static_cast<int32_t>(unit0 * C4_UNIT);
     if (warp == MMA_WARP) {
         tmem_alloc(&tmem_slot, TMEM_COLS);
@@ -425,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         // descriptors hold addresses in units of 16 bytes, in their low bits
         const uint64_t q_at = sw128_kmajor_desc(smem_u32(q_tile)), k_at = sw128_kmajor_desc(smem_u32(k_tile)),
                        v_at = sw128_kmajor_desc(smem_u32(v_tiles));
-        constexpr uint32_t QK = bf16_instr_desc(128, KEYS), PV = bf16_instr_desc(128, DK);
+        constexpr uint32_t QK = bf16_instr_desc(128, HALF), PV = bf16_instr_desc(128, DK);
         const uint32_t me = elected();
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -434,39 +427,36 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             return ok;
         };
         auto scores = [&](uint32_t t, uint32_t i) {
-            const uint64_t qd = q_at + t * (row_tile<NB>() / 16), kd = k_at + i % KV_STAGES * (row_tile<NB>() / 16);
+            const uint64_t qd = q_at + t * (row_tile<NB>() / 16), kd = k_at + i / 2 % KV_STAGES * (row_tile<NB>() / 16) + i % 2 * (HALF * 8);
+            const uint32_t to = S_COL + 128 * t + HALF * (i % 2);
 #pragma unroll
-            for (int k = 0; k < DK / 16; k++)
-                mma_ss(me, S_COL + 128 * t, qd + k / 4 * 1024 + k % 4 * 2, kd + k / 4 * 1024 + k % 4 * 2, QK, k > 0);
-            commit(me, &bars.s_full[t]);
+            for (int k = 0; k < DK / 16; k++) mma_ss(me, to, qd + k / 4 * 1024 + k % 4 * 2, kd + k / 4 * 1024 + k % 4 * 2, QK, k > 0);
+            commit(me, &bars.s_full[t][i % 2]);
+            if (t + 1 == tiles && i % 2) commit(me, &bars.k_empty[i / 2 % KV_STAGES]);
         };
         auto values = [&](uint32_t t, uint32_t i) {
-            const uint64_t vd = v_at + i % KV_STAGES * (v_tile<NB>() / 16);
+            const uint64_t vd = v_at + i / 2 % KV_STAGES * (v_tile<NB>() / 16) + i % 2 * (DK * 8);
+            const uint32_t from = S_COL + 128 * t + HALF * (i % 2) + 32;
 #pragma unroll
-            for (int k = 0; k < KEYS / 16; k++)
-                mma_ts(me, O_COL + 128 * t, S_COL + 128 * t + 64 + 8 * k, vd + k / 4 * (DK * 8) + k % 4 * 2, PV, i > 0 || k > 0);
+            for (int k = 0; k < HALF / 16; k++) mma_ts(me, O_COL + 128 * t, from + 8 * k, vd + 2 * k, PV, i > 0 || k > 0);
+            commit(me, &bars.o_full[t][i % 2]);
+            if (t + 1 == tiles && i % 2) commit(me, &bars.v_empty[i / 2 % KV_STAGES]);
         };
-        if (steps && wait(&bars.k_full[0], 0)) {
-            for (uint32_t t = 0; t < tiles; t++) scores(t, 0);
-            commit(me, &bars.k_empty[0]);
+        if (halves && wait(&bars.k_full[0], 0)) {
+            for (uint32_t i = 0; i < halves && i < 2; i++)
+                for (uint32_t t = 0; t < tiles; t++) scores(t, i);
         }
-        // a tile's next scores follow its values: they take P's place in
-        // TMEM, and products of one thread run in their order
-        for (uint32_t i = 0; ok && i < steps; i++) {
-            const uint32_t st = i % KV_STAGES, ph = i / KV_STAGES & 1, st1 = (i + 1) % KV_STAGES, ph1 = (i + 1) / KV_STAGES & 1;
-            const bool more = i + 1 < steps;
-            if (!wait(&bars.v_full[st], ph)) break;
+        // a tile's scores of the half step after next follow its values: they
+        // take P's place in TMEM, and products of one thread run in their order
+        for (uint32_t i = 0; ok && i < halves; i++) {
+            const uint32_t j = i / 2, st = j % KV_STAGES, ph = j / KV_STAGES & 1, st1 = (j + 1) % KV_STAGES, ph1 = (j + 1) / KV_STAGES & 1;
+            if (i % 2 == 0 && !wait(&bars.v_full[st], ph)) break;
             for (uint32_t t = 0; t < tiles; t++) {
-                if (!wait(&bars.p_full[t], i & 1)) break;
+                if (!wait(&bars.p_full[t][i % 2], j & 1)) break;
                 values(t, i);
-                if (t + 1 == tiles) commit(me, &bars.v_empty[st]);
-                if (!more) {
-                    commit(me, &bars.o_full[t]);
-                } else {
-                    if (t == 0 && !wait(&bars.k_full[st1], ph1)) break;
-                    scores(t, i + 1);
-                    if (t + 1 == tiles) commit(me, &bars.k_empty[st1]);
-                }
+                if (i + 2 >= halves) continue;
+                if (t == 0 && i % 2 == 0 && !wait(&bars.k_full[st1], ph1)) break;
+                scores(t, i + 2);
             }
         }
         if (!ok) {
@@ -545,23 +535,29 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         const float scale = fmaxf(fabsf(a.scale), 1e-37f);  // of a scale 0 too
         float m = NEG_INF, l = 0.0f;
         bool ok = true;
-        for (uint32_t i = 0; i < steps; i++) {
-            ok = warp_wait(&bars.s_full[t], i & 1, &gave_up, a.timeout);
+        // the values up to half step i are in O
+        auto values_in = [&](uint32_t i) {
+            const bool in = warp_wait(&bars.o_full[t][i % 2], i / 2 & 1, &gave_up, a.timeout);
+            tc_fence_after();
+            return in;
+        };
+        for (uint32_t i = 0; i < halves; i++) {
+            ok = warp_wait(&bars.s_full[t][i % 2], i / 2 & 1, &gave_up, a.timeout);
             if (!ok) break;
             tc_fence_after();
-            const int32_t key0 = key_base + static_cast<int32_t>(i * KEYS), first = span.lo - key0, end = span.hi - key0;
-            const bool before = __any_sync(FULL, first > 0), behind = __any_sync(FULL, end < KEYS);
-            if (before) softmax_step<NB, 2>(s_at, o_at, i > 0, scale, first, end, m, l);
-            else if (behind) softmax_step<NB, 1>(s_at, o_at, i > 0, scale, 0, end, m, l);
-            else softmax_step<NB, 0>(s_at, o_at, i > 0, scale, 0, KEYS, m, l);
+            auto idle = [&]() { return i == 0 || values_in(i - 1); };
+            const uint32_t from = s_at + HALF * (i % 2);
+            const int32_t key0 = key_base + static_cast<int32_t>(i * HALF), first = span.lo - key0, end = span.hi - key0;
+            const bool before = __any_sync(FULL, first > 0), behind = __any_sync(FULL, end < HALF);
+            if (before) ok = softmax_step<NB, 2>(from, o_at, i > 0, scale, first, end, m, l, idle);
+            else if (behind) ok = softmax_step<NB, 1>(from, o_at, i > 0, scale, 0, end, m, l, idle);
+            else ok = softmax_step<NB, 0>(from, o_at, i > 0, scale, 0, HALF, m, l, idle);
+            if (!ok) break;
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.p_full[t]);
+            if (lane == 0) mbar_arrive(&bars.p_full[t][i % 2]);
         }
-        if (steps && ok) {
-            ok = warp_wait(&bars.o_full[t], 0, &gave_up, a.timeout);
-            tc_fence_after();
-        }
+        if (halves && ok) ok = values_in(halves - 1);
         if (!ok) {
             gave_up = 1;
             if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
