@@ -2,26 +2,37 @@
 // fifth-generation tensor cores.
 //
 // A block takes 256 rows (tokens times the query heads of one cached head) as
-// two tiles of 128 and goes over its keys 128 at a time:
+// two tiles of 128 and goes over its keys 64 at a time:
 //     S = Q K^T   (tcgen05, Q and K from shared memory, S in TMEM)
 //     P = 2^(scale log2e S - m), row sums l, a row a thread
 //     O += P V    (tcgen05, P from TMEM, where it takes S's place, V from shared memory)
-// While the tensor cores work on one tile of rows, the other one's softmax
-// runs: 2 x (128 x 128 x dk) products each for S and O against 2 x 16,384
-// powers of two a step, some 2,048 cycles of either at dk 128.
+// Each tile has two places for S, so that the next scores lie there when a
+// softmax ends, and the products of one half step run beside the softmax of
+// the next. With O of both tiles that is all of TMEM. Products of 128 keys at a
+// time, which have one place a tile, wait for the softmax and it for them:
+// 1.18 ms against 1.09 for two prompts of 8,191 tokens, 8 heads of 128 with 4
+// query heads each (1,007 TFLOP/s, of the 1,662 that a library's bf16 product
+// reaches; leaving out the powers of two changes 1%).
+//
+// What bounds it: the products alone take 0.94 ms. Q's 4 KB are read anew for
+// every 64 keys x 16, as many cycles as the product of 128 keys takes; the
+// codes' warps and the softmax, which end in 0.70 and some 0.9 ms without
+// them, get in each other's way for the rest.
 //
 // Eight warps turn K's and V's codes into the bf16 values that they stand for
 // (exactly: pkb_cache4.cuh) in the 128-byte swizzled tiles that the tensor
 // cores read: K as [keys][dk], V as [dk][keys], which is how a lane's codes
 // lie in the cache, in stores without bank conflicts. They load the codes a
-// step ahead into registers (with the bf16 tiles of two steps and Q, shared
-// memory has no room for a ring that covers a load's latency: 1.37 ms with
-// one of 96 keys' codes ahead, [TIME] so). One thread issues the products,
-// eight warps have the rows.
+// step of 128 keys ahead into registers: with the bf16 tiles of two steps and
+// Q, shared memory has no room for a ring that covers a load's latency (1.37
+// ms with one of 96 keys' codes, 1.25 so). Sixteen warps, K's and V's apart, are
+// slower (1.16 ms against 1.09). One warp issues the products, eight have the
+// rows; sixteen, half a row a thread, were no faster.
 //
 // The maximum of a row is raised only where a score passes it by 8 (a factor
 // of 2^8, far inside a float), so O is rescaled in few steps. P is rounded to
-// bf16 once, as V's type asks; l sums what was rounded.
+// bf16 once, as V's type asks; l sums the weights before that rounding, in
+// float.
 
 #include <climits>
 
@@ -36,9 +47,9 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int SOFT_WARPS = 8, CODE_WARPS = 8, MMA_WARP = SOFT_WARPS + CODE_WARPS;
 constexpr int THREADS = 640;    // five warpgroups; the last one's three spare warps wait for the end
 // A thread's registers: 96 at launch (61,440 of the SM's 65,536), then the
-// rows' warps take what the others leave: 256 x 152 + 256 x 64 + 128 x 40 =
+// rows' warps take what the others leave: 256 x 136 + 256 x 80 + 128 x 40 =
 // 60,416.
-constexpr int SOFT_REGS = 152, CODE_REGS = 64, ISSUE_REGS = 40;
+constexpr int SOFT_REGS = 136, CODE_REGS = 80, ISSUE_REGS = 40;
 constexpr int ROWS = 256;       // of a block, two tiles of 128
 constexpr int KEYS = 128;       // of a step of K and V
 constexpr int HALF = 64;        // of a product
@@ -188,9 +199,9 @@ struct VCodes {
     // Into 16 columns of a slab of 64 keys (quarter 0 .. 3 of it). Keys from
     // `left` on become zeros: what lies there may be anything.
     __device__ __forceinline__ void store(uint8_t* slab, uint32_t quarter, int32_t left) const {
-        const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
-        uint8_t* const lo_at = slab + g * 128 + 4 * t + (((2 * quarter) ^ g) << 4);      // keys 2t, 2t + 1
-        uint8_t* const hi_at = slab + g * 128 + 4 * t + (((2 * quarter + 1) ^ g) << 4);  // keys 8 + 2t, 9 + 2t
+        const uint32_t lane = threadIdx.x & 31, t = lane & 3, row = lane & 7;
+        // the row of a store's four 8 x 8 tiles that this lane names: dimensions from 0 and 8 on of keys 0 .. 7, then of 8 .. 15
+        const uint32_t at = smem_u32(slab) + (row + (lane & 8)) * 128 + (((2 * quarter + lane / 16) ^ row) << 4);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             uint32_t s2[2], ms[2];
@@ -207,11 +218,10 @@ struct VCodes {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const uint32_t x = j ? w[b].y : w[b].x;
-                const int at = (32 * b + 16 * j) * 128;  // dimensions 32 b + 16 j + g, and 8 on
-                *reinterpret_cast<uint32_t*>(lo_at + at) = c4_pair<0>(x, s2[0], ms[0]);
-                *reinterpret_cast<uint32_t*>(lo_at + at + 1024) = c4_pair<1>(x, s2[0], ms[0]);
-                *reinterpret_cast<uint32_t*>(hi_at + at) = c4_pair<2>(x, s2[1], ms[1]);
-                *reinterpret_cast<uint32_t*>(hi_at + at + 1024) = c4_pair<3>(x, s2[1], ms[1]);
+                asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + (32 * b + 16 * j) * 128),
+                             "r"(c4_pair<0>(x, s2[0], ms[0])), "r"(c4_pair<1>(x, s2[0], ms[0])), "r"(c4_pair<2>(x, s2[1], ms[1])),
+                             "r"(c4_pair<3>(x, s2[1], ms[1]))
+                             : "memory");
             }
         }
     }
