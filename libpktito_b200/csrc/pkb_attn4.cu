@@ -622,11 +622,15 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 
 // Joins the parts of the items that several shares have. A warp takes 16
 // dimensions of eight rows (a float4 a lane) over every `ways`-th of an
-// item's parts; `ways` warps then join theirs, always in the same order. Many
-// items have few parts each and take one way, a few long ones take up to
-// eight, so that no warp reads many parts one after another.
-// BATCH parts are loaded together: four (and 64 registers, so that four blocks
-// share an SM) for many items, eight for a few long ones.
+// item's parts; `ways` warps then join theirs, always in the same order. It
+// is bound by latency: the item, then its parts, one load behind the other.
+// Up to eight parts an item go one way (a step of 32 sequences of 400 tokens,
+// five parts each: 15.9 us with its join, 21 two ways), a few long items'
+// take up to eight, so that no warp reads many parts one after another. Four
+// parts are loaded together (in 64 registers, so that four blocks share an
+// SM), or eight where each way still has more than six (one sequence of 2,000
+// tokens 11.4 -> 10.0 us, three of 120,000 61.5 -> 58.1; 8 of 400 tokens, five
+// parts a way, 11.4 and 13.5 with eight).
 template <typename T, int NB, int NT, int BATCH>
 __global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kernel(Attn4Args a, uint32_t ways) {
     constexpr int QUADS = 2 * NB * NT, STRIDE = part_regs<NB, NT>() / 4;  // float4s of a lane: [dims 16][eight rows], then m and l
@@ -871,13 +875,14 @@ cudaError_t launch_split(Attn4Args a, uint32_t grid, cudaStream_t s) {
     cudaError_t e = c4_launch(split_kernel<T, NB, NT, PARTS>, grid, workers<NB, NT>() * 32, split_smem<NB, NT>(a.n), s, a);
     if (e != cudaSuccess) return e;
     count_launch();
-    // parts an item has about, if all have as many: more than four go two ways and so on
+    // Parts an item has about, if all have as many: more than eight go two ways
+    // and so on, more than 48 eight at a time.
     const uint64_t items = static_cast<uint64_t>(a.n) * a.teams * a.max_blocks, most = grid * workers<NB, NT>() / a.team;
     const uint64_t shares = most < a.max_shares ? most : a.max_shares;
     uint32_t ways = 1;
-    while (ways < 8 && shares > 4 * ways * items) ways *= 2;
+    while (ways < 8 && shares > 8 * ways * items) ways *= 2;
     const uint32_t quads = JOIN_WARPS / ways;
-    e = c4_launch(ways > 1 ? join_kernel<T, NB, NT, 8> : join_kernel<T, NB, NT, 4>,
+    e = c4_launch(shares > 48 * items ? join_kernel<T, NB, NT, 8> : join_kernel<T, NB, NT, 4>,
                   dim3(static_cast<uint32_t>(items * a.team), (2 * NB * NT + quads - 1) / quads), JOIN_WARPS * 32, 0, s, a, ways);
     if (e == cudaSuccess) count_launch();
     return e;
@@ -888,9 +893,19 @@ cudaError_t launch_one(const Attn4Args& a, uint32_t grid, bool split, cudaStream
     return split ? launch_split<T, NB, NT, PARTS>(a, grid, s) : launch_rows<T, NB, NT, PARTS>(a, s);
 }
 
+// Rows of a block: two blocks of eight share the codes' conversion where there
+// are more than eight rows (64 sequences of 2,048 tokens, 16 bf16 rows a head
+// of 128: 67 us, 78 in eights; 4 rows 66, 52 in eights). 17 to 24 float rows, whose
+// five products a 16 values are most of the work, are three eights (32
+// sequences of 1,500 tokens, 23 rows: 66 us, 73 in sixteens; 12 rows 48 and 42).
+uint32_t block_rows(const Attn4Args& a, bool float_rows) {
+    const uint64_t rows = static_cast<uint64_t>(a.max_rows) * a.G;
+    return a.c.dk == 256 || rows <= 8 || (float_rows && rows > 16 && rows <= 24) ? 8 : 16;
+}
+
 template <typename T, int PARTS>
 cudaError_t launch_type(const Attn4Args& a, uint32_t grid, bool split, cudaStream_t s) {
-    const bool two = static_cast<uint64_t>(a.max_rows) * a.G > 8;  // more than eight rows: two blocks of eight share the codes' conversion
+    const bool two = block_rows(a, PARTS == 3) == 16;
     switch (a.c.dk) {
         case 32: return two ? launch_one<T, 1, 2, PARTS>(a, grid, split, s) : launch_one<T, 1, 1, PARTS>(a, grid, split, s);
         case 64: return two ? launch_one<T, 2, 2, PARTS>(a, grid, split, s) : launch_one<T, 2, 1, PARTS>(a, grid, split, s);
@@ -927,7 +942,7 @@ bool splits(const Attn4Args& a, int type, uint32_t n, uint32_t grid) {
     const uint64_t rows = static_cast<uint64_t>(a.max_rows) * a.G, heads = static_cast<uint64_t>(n) * a.teams * a.team;
     if (rows > SPLIT_ROWS) return false;
     const bool tc = attention4_tc_takes(a, type);
-    const uint64_t block = a.c.dk == 256 || rows <= 8 ? 8 : 16, blocks = (rows + block - 1) / block;
+    const uint64_t block = block_rows(a, type == PKB_F32), blocks = (rows + block - 1) / block;
     if (!tc && rows <= 128) return true;
     const uint64_t many = tc ? 256 : ROW_WARPS * block, waves = (heads * ((rows + many - 1) / many) + grid - 1) / grid;
     return heads * blocks <= (tc ? 2 : 4) * grid * waves;
