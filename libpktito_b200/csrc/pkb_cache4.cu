@@ -2,18 +2,25 @@
 // pages and back, and its page operations.
 //
 // Rows. Append reads each value once (2 or 4 bytes) and writes 4.5 bits of
-// it, read does the reverse: both are bound by memory. A warp takes one
-// unit's K or V (16 tokens of one head), 8 blocks of 32 values a pass, four
-// lanes a block, so that a lane's eight values are one word of K's codes. V's
-// words mix 4 tokens and are put together from bytes in shared memory; a
-// byte is one token's, so a unit that the call covers in part is written a
-// byte at a time beside the tokens it leaves alone.
+// it, read does the reverse: many rows are bound by memory (24 segments'
+// 28.8 M float values appended and read back: 260 MB in 61 us, 4.3 TB/s, of 40
+// at the rate of a copy), few by the latency of some dependent loads
+// (an entry's rows, its length, its page, the row). A warp takes one unit's K
+// or V (16 tokens of one head), four lanes a token, so that a lane's eight
+// values of a block are one word of K's codes. V's words mix 4 tokens: append puts
+// them together from bytes in shared memory, read takes them apart with 8 x 8
+// transposes in registers. A byte is one token's, so a unit that the call
+// covers in part is written a byte at a time beside the tokens it leaves
+// alone.
 //
 // Page operations. One block plans (it checks the lists, finds the lowest
 // free pages by a scan of refs, and refuses before anything is changed), a
 // grid applies: table rows, references and the pages' bytes. They are bound
-// by the copied bytes where pages are copied, else by the latency of the
-// plan's few dependent reads.
+// by the copied bytes where pages are copied (192 sessions of up to 4,001
+// tokens freed, compacted and some copied: 1.07 GB each way in 0.40 ms, of 0.33 at a
+// copy's rate), else by the launches and the latency of the plan's few
+// dependent reads (32 hypotheses' step of free, fork and grow: 18.6 us in a
+// graph, 47 from Python).
 
 #include <climits>
 
@@ -28,33 +35,6 @@ namespace {
 constexpr int ROW_WARPS = 8;
 constexpr uint32_t FULL = 0xFFFFFFFFu;
 
-// The entry i of a call that slot x belongs to. Entry i's units are counted
-// from starts[i] / 16 + 2 i: it has at most (rows + 30) / 16 of them, two
-// fewer than the distance to the next entry's first when rounded down, so
-// no scan over the entries is needed. Thirty-two probes a step.
-__device__ __forceinline__ uint32_t slot_entry(const int32_t* starts, uint32_t n, uint32_t x) {
-    const uint32_t lane = threadIdx.x & 31;
-    if (n <= 256) {  // eight entries a lane, all asked for at once
-        uint32_t below = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            const uint32_t i = j * 32 + lane;
-            below += i < n && static_cast<uint32_t>(starts[i]) / C4_UNIT + 2 * i <= x;
-        }
-        below = __reduce_add_sync(FULL, below);
-        return below ? below - 1 : 0;
-    }
-    uint32_t lo = 0, hi = n;  // the answer is in [lo, hi)
-    while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 31) / 32, i = lo + lane * step;
-        const bool below = i < hi && static_cast<uint32_t>(starts[i]) / C4_UNIT + 2 * i <= x;
-        const uint32_t last = 31 - __clz(__ballot_sync(FULL, below) | 1u);
-        lo += last * step;
-        hi = lo + step < hi ? lo + step : hi;
-    }
-    return lo;
-}
-
 struct RowArgs {
     Cache4 c;
     const int32_t *seqs, *starts;
@@ -62,6 +42,31 @@ struct RowArgs {
     size_t ks, vs;
     uint32_t layer, n, rows, slots;
 };
+
+// The last entry whose first row is at most row 16 x + 15: thirty-two probes
+// a step, or all at once.
+__device__ __forceinline__ uint32_t entry_at(const int32_t* starts, uint32_t n, uint32_t x) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (n <= 256) {  // eight entries a lane, all asked for at once
+        uint32_t below = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            const uint32_t i = j * 32 + lane;
+            below += i < n && static_cast<uint32_t>(starts[i]) / C4_UNIT <= x;
+        }
+        below = __reduce_add_sync(FULL, below);
+        return below ? below - 1 : 0;
+    }
+    uint32_t lo = 0, hi = n;  // the answer is in [lo, hi)
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const bool below = i < hi && static_cast<uint32_t>(starts[i]) / C4_UNIT <= x;
+        const uint32_t last = 31 - __clz(__ballot_sync(FULL, below) | 1u);
+        lo += last * step;
+        hi = lo + step < hi ? lo + step : hi;
+    }
+    return lo;
+}
 
 // Where a warp's unit lies, and which of its tokens the call has: token r is
 // row `row0 + r` for r in [first, last).
@@ -71,9 +76,23 @@ struct UnitRows {
     int first, last;
 };
 
+// The unit of a slot. The first 2 n slots are the entries' first two units each
+// (all there are of up to 17 rows), found without a search; the others those
+// that longer entries have beside them, (rows - 2) / 16 at most, so that
+// counting them from starts[i] / 16 leaves every entry room. (One row of each
+// of 256 sequences appended and read: 16.6 us, 18.5 with a search for every
+// slot, 14.5 with one warp for an entry's two units, whose loop costs the long
+// entries 62 -> 67.)
 __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, uint32_t h) {
     UnitRows u = {nullptr, 0, 0, 0};
-    const uint32_t i = slot_entry(a.starts, a.n, slot);
+    uint32_t i = slot / 2, k = slot % 2;
+    if (i >= a.n) {
+        const uint32_t x = slot - 2 * a.n;
+        i = entry_at(a.starts, a.n, x);
+        const uint32_t at = static_cast<uint32_t>(a.starts[i]) / C4_UNIT;
+        if (x < at) return u;
+        k = 2 + x - at;
+    }
     uint32_t seq, r0;
     const uint32_t rows = c4_rows(a.c, a.seqs, a.starts, i, a.rows, &seq, &r0, a.err);
     if (!rows) return u;
@@ -82,8 +101,8 @@ __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, u
         if ((threadIdx.x & 31) == 0) atomicOr(a.err, PKB_DEVERR_ARGS);
         return u;
     }
-    const uint32_t pos0 = len - rows, at = r0 / C4_UNIT + 2 * i, unit = pos0 / C4_UNIT + (slot - at);
-    if (slot < at || unit > (len - 1) / C4_UNIT) return u;  // the entry has no such unit
+    const uint32_t pos0 = len - rows, unit = pos0 / C4_UNIT + k;
+    if (unit > (len - 1) / C4_UNIT) return u;  // the entry has no such unit
     u.bytes = c4_unit(a.c, a.layer, seq, h, unit, a.err);
     const int64_t t0 = static_cast<int64_t>(unit) * C4_UNIT - pos0;
     u.row0 = r0 + t0;
@@ -139,25 +158,14 @@ __device__ __forceinline__ float quantize_block(float (&f)[8], uint32_t (&nib)[8
     return scaled ? s : 0.0f;
 }
 
+// One unit's K or V; x: the head's values of row 0, xs apart.
 template <typename T, int NB, bool VEC>
-__global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* k, const T* v, RowArgs a) {
+__device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRows& u, bool is_v, uint8_t* vb) {
     constexpr int DK = NB * 32;
-    __shared__ alignas(16) uint8_t stage[ROW_WARPS][C4_UNIT * v_row<NB>()];
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane / 4, t = lane & 3;
-    const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + warp;
-    const bool is_v = item & 1;
-    const uint32_t h = static_cast<uint32_t>((item >> 1) % a.c.heads);
-    const size_t slot = (item >> 1) / a.c.heads;
-    if (slot >= a.slots) return;
-    const UnitRows u = warp_unit(a, static_cast<uint32_t>(slot), h);
-    if (!u.bytes) return;
-    const size_t xs = is_v ? a.vs : a.ks;
-    const T* x = (is_v ? v : k) + h * DK + 8 * t;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+    x += 8 * t;
     uint8_t* codes = u.bytes + (is_v ? 8 * DK : 0);
     __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(u.bytes + (is_v ? 17 * DK : 16 * DK));
-    uint8_t* vb = stage[warp];
 #pragma unroll
     for (int r = 0; r < 2; r++) {
         // lanes 4 g .. 4 g + 3 have token g or g + 8, eight values of each block
@@ -231,6 +239,30 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) append_kernel(const T* k, cons
     }
 }
 
+// A warp's slot, head, and whether its V: K's and V's warps of a unit are neighbours
+struct RowItem {
+    size_t slot;
+    uint32_t h;
+    bool is_v;
+    __device__ __forceinline__ explicit RowItem(const RowArgs& a) {
+        const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + threadIdx.x / 32;
+        is_v = item & 1;
+        h = static_cast<uint32_t>((item >> 1) % a.c.heads);
+        slot = (item >> 1) / a.c.heads;
+    }
+};
+
+template <typename T, int NB, bool VEC>
+__global__ void __launch_bounds__(ROW_WARPS * 32, NB == 8 ? 2 : 4) append_kernel(const T* k, const T* v, RowArgs a) {
+    __shared__ alignas(16) uint8_t stage[ROW_WARPS][C4_UNIT * v_row<NB>()];
+    pdl_trigger();
+    pdl_wait();
+    const RowItem me(a);
+    if (me.slot >= a.slots) return;
+    const UnitRows u = warp_unit(a, static_cast<uint32_t>(me.slot), me.h);
+    if (u.bytes) append_unit<T, NB, VEC>((me.is_v ? v : k) + me.h * (NB * 32), me.is_v ? a.vs : a.ks, u, me.is_v, stage[threadIdx.x / 32]);
+}
+
 // a bf16 pair's two values at p (8-byte, or 4-byte aligned for 16-bit types, where VEC)
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_pair(T* p, uint32_t pair) {
@@ -246,19 +278,11 @@ __device__ __forceinline__ void store_pair(T* p, uint32_t pair) {
     }
 }
 
+// One unit's K or V, to the head's values of row 0, xs apart
 template <typename T, int NB, bool VEC>
-__global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* k, T* v, RowArgs a) {
+__device__ __forceinline__ void read_unit(T* x, size_t xs, const UnitRows& u, bool is_v) {
     constexpr int DK = NB * 32;
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane / 4, t = lane & 3;
-    const size_t item = static_cast<size_t>(blockIdx.x) * ROW_WARPS + warp;
-    const bool is_v = item & 1;
-    const uint32_t h = static_cast<uint32_t>((item >> 1) % a.c.heads);
-    const size_t slot = (item >> 1) / a.c.heads;
-    if (slot >= a.slots) return;
-    const UnitRows u = warp_unit(a, static_cast<uint32_t>(slot), h);
-    if (!u.bytes) return;
+    const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     if (!is_v) {
         // a lane's words of tokens g and g + 8: eight values of each block
         uint32_t w[2][NB];
@@ -274,7 +298,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* k, T* v, RowArg
         for (int r = 0; r < 2; r++) {
             const int token = static_cast<int>(g) + 8 * r;
             if (token < u.first || token >= u.last) continue;
-            T* to = k + (u.row0 + token) * a.ks + h * DK + 8 * t;
+            T* to = x + (u.row0 + token) * xs + 8 * t;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const uint32_t s2 = s[r][b] | static_cast<uint32_t>(s[r][b]) << 16;
@@ -300,21 +324,31 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) read_kernel(T* k, T* v, RowArg
         for (int c = 0; c < 2; c++) s2[c] = *reinterpret_cast<const uint32_t*>(u.bytes + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const uint32_t x = j ? w.y : w.x;
-            uint32_t p[2][2] = {{c4_pair_any<0>(x, s2[0]), c4_pair_any<1>(x, s2[0])}, {c4_pair_any<2>(x, s2[1]), c4_pair_any<3>(x, s2[1])}};
+            const uint32_t y = j ? w.y : w.x;
+            uint32_t p[2][2] = {{c4_pair_any<0>(y, s2[0]), c4_pair_any<1>(y, s2[0])}, {c4_pair_any<2>(y, s2[1]), c4_pair_any<3>(y, s2[1])}};
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int token = static_cast<int>(g) + 8 * c;
                 const bool valid = token >= u.first && token < u.last;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    uint32_t y;
-                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(p[c][r]));
-                    if (valid) store_pair<T, VEC>(v + (u.row0 + token) * a.vs + h * DK + 32 * b + 16 * j + 8 * r + 2 * t, y);
+                    uint32_t pair;
+                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pair) : "r"(p[c][r]));
+                    if (valid) store_pair<T, VEC>(x + (u.row0 + token) * xs + 32 * b + 16 * j + 8 * r + 2 * t, pair);
                 }
             }
         }
     }
+}
+
+template <typename T, int NB, bool VEC>
+__global__ void __launch_bounds__(ROW_WARPS * 32, NB == 8 ? 5 : 8) read_kernel(T* k, T* v, RowArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const RowItem me(a);
+    if (me.slot >= a.slots) return;
+    const UnitRows u = warp_unit(a, static_cast<uint32_t>(me.slot), me.h);
+    if (u.bytes) read_unit<T, NB, VEC>((me.is_v ? v : k) + me.h * (NB * 32), me.is_v ? a.vs : a.ks, u, me.is_v);
 }
 
 // ------------------------------------------------------------ page operations --
