@@ -451,7 +451,7 @@ size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t
  * those with j <= p, and where `window` is not 0 to those with
  * j > p - window:
  *     o = sum_j softmax_j(scale q.k_j) v_j,
- * zeros where there is no such j. A sequence has at most max_rows rows (one
+ * zeros where there is no such j; scale log2 e has to be finite. A sequence has at most max_rows rows (one
  * that has more is out of range). Products are exact to the type of q, sums
  * are float32, o is rounded once. Rows of o behind starts[n] are left as they
  * were; o must not overlap q. work as for the page operations. What is out

@@ -23,6 +23,17 @@
 // one another. An item that one share has whole is written at once; of
 // the others each share leaves its part (m, l, O) in the work area, and a
 // second kernel joins an item's parts in a fixed order.
+//
+// What bounds it. The cache's bytes (1.125 dk a token and cached head) and the
+// instructions that unpack them, which take about as long: a tile of 32 keys
+// of a head of 128 is some 520 instructions of a warp, 60 % of all issue slots.
+// One step of 64 sequences of up to 4,099 tokens (161 MB, 8 heads of 128 with 4
+// query heads each, bf16): 51 us with its join, 3.1 TB/s; three sequences of up
+// to 120,001 tokens with 8 query heads each: 58 us, 3.4 TB/s. Of that some 7 us pass
+// before the first tile (the entries' lengths, their scan, the first pages) and
+// 5 in the join: short calls (12 us for one sequence of 377 tokens) are nothing else.
+// Scaled bf16 values for K too took 66 us for the 64 sequences, one warp that
+// fetches for all of a block's 55 and for itself each 52.
 
 #include <climits>
 
@@ -37,7 +48,7 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int JOIN_WARPS = 8;
 constexpr int TILE = 32;            // keys of a tile: two units
 constexpr uint32_t MAX_ENTRIES = 1024;  // sequences of one launch
-constexpr uint32_t MAX_TEAM = 16;
+constexpr uint32_t MAX_TEAM = 16;       // (teams of 4 and 8 take as long: 64 sequences of 2,048 tokens, 16 heads, 78 us)
 constexpr uint32_t SPLIT_ROWS = 1024;   // rows of an entry and cached head that may be split along the keys
 constexpr int MAX_GRID = 160;
 constexpr int MAX_WORKERS = 16;
@@ -721,8 +732,10 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kern
 // entry and head, a warp each, and its warps read the same tiles from one
 // ring, so that a tile is fetched once for 64 or 128 rows. Nothing is split
 // along the keys. A warp leaves out the tiles that its own rows cannot see.
-// Bound by mma.sync's rate: 2 (bf16), 3 (f16) or 5 (float rows) products of
-// 16 keys and 8 rows a 16 values.
+// For f16 and float rows, and bf16 rows of 256 values (others: pkb_attn4_tc.cu).
+// Bound by the tile's instructions and mma.sync's rate: 2 (bf16), 3 (f16) or 5
+// (float rows) products of 16 keys and 8 rows a 16 values. 8 sequences of 2,048
+// tokens, 8 heads of 128, 256 float rows a head: 188 us.
 
 constexpr int ROW_WARPS = 8;
 constexpr int ROW_STAGES = 8;

@@ -124,7 +124,8 @@ __device__ __forceinline__ float rescale(float from, float to) { return from == 
 
 // What it costs to begin and end an item, in tiles: shares are of equal
 // cost, not of equal tiles. An item is START places of no work, then its
-// tiles.
+// tiles (200 streams of 250 tokens: 26.1 us with none, 24.7 with two, 26.8 with
+// four; 64 sequences of up to 4,099: 52.3, 51.4, 52.4).
 constexpr uint32_t START = 2;
 
 // One entry's rows and tokens, and of what its rows can see the first unit,
