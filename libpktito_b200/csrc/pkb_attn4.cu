@@ -962,10 +962,10 @@ bool splits(const Attn4Args& a, int type, uint32_t n, uint32_t grid) {
 }
 
 // The work area of a call, over any lengths and max_rows: a join an item (an
-// entry, head and block of rows), two parts a share and head. Where more than
-// 128 rows are split, `splits` holds heads times blocks below
-// 4 (16 heads + MAX_GRID) for blocks of eight rows, 4 (8 heads + MAX_GRID) for
-// sixteen.
+// entry, head and block of rows), two parts a share and head. Up to 128 rows
+// are 16 blocks at most. More are nine or more, and `splits` wants them to be
+// at most 4 (blocks / 8, rounded up) a head and 4 grids beside, so that heads times
+// blocks stay within 36 grids (nine blocks; fewer for others and on tcgen05's side).
 struct Bounds {
     uint64_t shares, join_bytes, bytes;
 };
@@ -973,8 +973,9 @@ struct Bounds {
 Bounds bounds_of(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
     uint32_t team, teams;
     teams_of(c->n_heads, &team, &teams);
-    const uint64_t all = static_cast<uint64_t>(rows) * (H / c->n_heads), blocks = all < 512 ? (all + 7) / 8 : 64;
-    const uint64_t items = static_cast<uint64_t>(n < MAX_ENTRIES ? n : MAX_ENTRIES) * teams * team * blocks + (all > 128 ? 4 * MAX_GRID : 0);
+    const uint64_t all = static_cast<uint64_t>(rows) * (H / c->n_heads), blocks = all < 128 ? (all + 7) / 8 : 16;
+    uint64_t items = static_cast<uint64_t>(n < MAX_ENTRIES ? n : MAX_ENTRIES) * teams * team * blocks;
+    if (all > 128 && items < 36 * MAX_GRID) items = 36 * MAX_GRID;
     const uint64_t most = static_cast<uint64_t>(MAX_GRID) * MAX_WORKERS / team, places = items / team * places_of(c);
     Bounds b;
     b.shares = places < most ? places : most;

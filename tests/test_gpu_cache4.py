@@ -312,6 +312,27 @@ def test_more_heads_than_a_team(kind, heads, G, dk):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,heads,G,dk,rows,page", [(1, 1, 1, 32, 1024, 16), (1, 8, 4, 64, 130, 32), (3, 20, 1, 32, 129, 16), (4, 33, 1, 32, 140, 16),
+                                                    (2, 2, 3, 256, 43, 16), (1, 1, 8, 128, 128, 64), (9, 4, 1, 96, 300, 16), (70, 8, 1, 32, 17, 16)])
+def test_the_work_area_is_enough(kind, n, heads, G, dk, rows, page):
+    """Nothing is written behind the bytes asked for, whichever way the rows are divided; more rows than a wave, and fewer."""
+    lens = [rows + 37 * (i % 5) for i in range(n)]
+    c = filled(lens, page, heads, dk, seed=rows)
+    H, total = heads * G, n * rows
+    q = torch.randn((total, H * dk), generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(KIND[kind])
+    o = torch.empty_like(q)
+    size = P.attention_cache4_work_bytes(c, H, total, n)
+    work = torch.full((size + (1 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    for most in (rows, total):  # max_rows may say more than there are
+        P.attention_cache4_dev(o, H * dk, q, H * dk, H, c, 0, ints(range(n)), ints([i * rows for i in range(n + 1)]), n, total, most,
+                               dk ** -0.5, True, 0, work[:size])
+        no_errors()
+        assert (work[size:] == 0xA5).all()
+    assert check_attention(c, lens, [rows] * n, list(range(n)), G, kind, True, 0, q=q) <= 1
+    assert check_attention(c, lens, [rows] * n, list(range(n)), G, kind, False, 0, q=q, max_rows=total) <= 1
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows", [1, 3, 150])  # one part, some rows, a prompt
 def test_padded_entries_and_a_sequence_listed_twice(kind, rows):
     lens = [160, 400, 151]
