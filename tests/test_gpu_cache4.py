@@ -311,6 +311,16 @@ def test_more_heads_than_a_team(kind, heads, G, dk):
     check_attention(c, lens, [1, 5, 2, 1, 3], [4, 1, 3, 0, 2], G, kind, True, 70)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_table_with_room_for_a_billion_tokens(kind):
+    # places are counted in 32 bits: three entries take two launches, or the way of many rows
+    lens = [300, 129, 1000]
+    c = filled(lens, 256, 33, 32, seed=21, max_pages=2 ** 22 - 1)
+    check_attention(c, lens, [128, 1, 100], [0, 1, 2], 1, kind, True, 0)
+    check_attention(c, lens, [1, 1, 1], [2, 0, 1], 2, kind, True, 2 ** 29)
+    check_attention(c, lens, [300, 1, 100], [0, 1, 2], 2, kind, False, 2 ** 30 + 500)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,heads,G,dk,rows,page", [(1, 1, 1, 32, 1024, 16), (1, 8, 4, 64, 130, 32), (3, 20, 1, 32, 129, 16), (4, 33, 1, 32, 140, 16),
                                                     (2, 2, 3, 256, 43, 16), (1, 1, 8, 128, 128, 64), (9, 4, 1, 96, 300, 16), (70, 8, 1, 32, 17, 16)])
