@@ -335,8 +335,8 @@ uint64_t pkb_tdt_last_rounds(void);
  * What is held. A block is 32 consecutive values of one head of one row.
  * With amax its largest magnitude: a block that holds a NaN or an infinity,
  * or whose amax is below 2^-121, is held as zeros (scale 0). Otherwise the
- * scale s is the largest number of 5 significant bits that is not above
- * amax / 7 (the float quotient), each value is the code c = rint(x / s),
+ * scale s is amax times the float nearest to 1/7, rounded to float and cut to
+ * its 5 first significant bits, each value is the code c = rint(x / s),
  * ties to even, within [-7, 7], and stands for c s, which is exactly a bf16.
  *
  * How it lies. A unit is 16 tokens of one head, 18 dk bytes: K's codes

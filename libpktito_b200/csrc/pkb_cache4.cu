@@ -115,9 +115,9 @@ template <int NB> __host__ __device__ constexpr int v_row() { return NB * 16 + 8
 
 // A block's scale and its codes + 8, from four lanes' eight values each.
 //
-// The scale is the largest s of 5 significant bits with 7 s <= amax: amax / 7
-// cut to 5 bits, or the one before where the product rounded up (7 s has 8
-// bits, so the comparison is exact). A code is rint(x / s), ties to even:
+// The scale is amax times the float nearest to 1 / 7, rounded and cut to 5
+// significant bits (the quotient's own, but where amax lies within a step
+// below 7 s). A code is rint(x / s), ties to even:
 // from x times an approximate 1 / s, whose remainder x - c s is exact in
 // one FMA and says whether c is the nearest. It is not, or may be a tie, in
 // few warps: the others skip the correction. No division: with a correctly
@@ -130,7 +130,6 @@ __device__ __forceinline__ float quantize_block(float (&f)[8], uint32_t (&nib)[8
     m = max(m, __shfl_xor_sync(FULL, m, 2));
     const bool scaled = block_scaled(m);
     float s = __uint_as_float(__float_as_uint(__fmul_rn(__uint_as_float(m), 0.14285714924335479736f)) & 0xFFF80000u);
-    if (__fmul_rn(s, 7.0f) > __uint_as_float(m)) s = __uint_as_float(__float_as_uint(s) - 0x80000u);
     if (__any_sync(FULL, !scaled)) {  // zeros, with a scale that divides
         s = scaled ? s : 1.0f;
 #pragma unroll

@@ -11,7 +11,8 @@ def quantize(x):
     b = np.asarray(x, np.float64).reshape(*x.shape[:-1], -1, BLOCK)
     amax = np.abs(b).max(-1)
     good = np.isfinite(b).all(-1) & (np.where(np.isnan(amax), 0, amax) >= 2.0 ** -121)
-    m, e = np.frexp(np.where(good, amax, 1.0) / 7)
+    seventh = np.where(good, amax, 1.0).astype(np.float32) * (np.float32(1) / np.float32(7))  # rounded to float
+    m, e = np.frexp(seventh.astype(np.float64))
     s = np.where(good, np.ldexp(np.floor(m * 32) / 32, e), 0.0)
     c = np.rint(np.where(good[..., None], b, 0.0) / np.where(good, s, 1.0)[..., None])
     assert np.abs(c).max(initial=0) <= 7
