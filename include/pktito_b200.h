@@ -451,13 +451,13 @@ size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t
  * those with j <= p, and where `window` is not 0 to those with
  * j > p - window:
  *     o = sum_j softmax_j(scale q.k_j) v_j,
- * zeros where there is no such j; scale log2 e has to be finite. A sequence has at most max_rows rows (one
- * that has more is out of range). Products are exact to the type of q, sums
- * are float32, o is rounded once. Rows of o behind starts[n] are left as they
- * were; o must not overlap q. work as for the page operations. What is out
- * of range sets the device error word's bit 1, and such rows of o are not
- * defined. A block of 2^126 or more is held and read back, but makes the rows
- * that see it infinite or NaN. */
+ * zeros where there is no such j; scale log2 e has to be finite. A sequence
+ * has at most max_rows rows (one that has more is out of range). Products are
+ * exact to the type of q, sums are float32, o is rounded once. Rows of o
+ * behind starts[n] are left as they were; o must not overlap q. work as for
+ * the page operations. What is out of range sets the device error word's bit
+ * 1, and such rows of o are not defined. A block of 2^126 or more is held and
+ * read back, but makes the rows that see it infinite or NaN. */
 int pkb_attention_cache4_dev(void *stream, void *o, size_t os, const void *q, size_t qs, int type, uint32_t H,
                              const pkb_cache4 *c, uint32_t layer, const int32_t *seqs, const int32_t *starts,
                              uint32_t n, uint32_t rows, uint32_t max_rows, float scale, int causal, uint32_t window,

@@ -117,11 +117,11 @@ template <int NB> __host__ __device__ constexpr int v_row() { return NB * 16 + 8
 //
 // The scale is amax times the float nearest to 1 / 7, rounded and cut to 5
 // significant bits (the quotient's own, but where amax lies within a step
-// below 7 s). A code is rint(x / s), ties to even:
-// from x times an approximate 1 / s, whose remainder x - c s is exact in
-// one FMA and says whether c is the nearest. It is not, or may be a tie, in
-// few warps: the others skip the correction. No division: with a correctly
-// rounded one a value the kernel took 49 us for 28.8 M float values, 30 so.
+// below 7 s). A code is rint(x / s), ties to even: from x times an approximate
+// 1 / s, whose remainder x - c s is exact in one FMA and says whether c is the
+// nearest. It is not, or may be a tie, in few warps: the others skip the
+// correction. No division: with a correctly rounded one a value the kernel
+// took 49 us for 28.8 M float values, 30 so.
 __device__ __forceinline__ float quantize_block(float (&f)[8], uint32_t (&nib)[8]) {
     uint32_t m = 0;
 #pragma unroll
