@@ -453,7 +453,11 @@ size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t
  *     o = sum_j softmax_j(scale q.k_j) v_j,
  * zeros where there is no such j; scale log2 e has to be finite. A sequence
  * has at most max_rows rows (one that has more is out of range). Products are
- * exact to the type of q, sums are float32, o is rounded once. Rows of o
+ * exact to the type of q, sums are float32, o is rounded once. The softmax's
+ * weights meet V with 24 bits for float rows and 16 for others, but with 8 for
+ * bf16 rows of up to 128 values a head that are many (prompts and long
+ * chunks), where they are an operand of the tensor cores' bf16 products; their
+ * sum is that of the unrounded ones. Rows of o
  * behind starts[n] are left as they were; o must not overlap q. work as for
  * the page operations. What is out of range sets the device error word's bit
  * 1, and such rows of o are not defined. A block of 2^126 or more is held and

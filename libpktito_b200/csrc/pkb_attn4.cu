@@ -11,7 +11,11 @@
 // a step of decoding with up to eight query heads a cached head wastes
 // none. The codes become exact bf16 values in registers, three instructions
 // a pair (pkb_cache4.cuh); their order in the cache is that operand's, so
-// no value crosses a lane.
+// no value crosses a lane. V is exact, and P is two bf16 parts for f16 and
+// bf16 rows (16 bits), three for float rows (24). One part, P rounded to bf16
+// before it meets V, is as far off as o's own rounding: 2.3e-3 of the result for
+// bf16 rows against 1.65e-3 for two parts and for weights in float, of which
+// 1.65e-3 is o's; it takes a tenth less time (64 sequences 49.7 us against 54.7).
 //
 // The split. A team of up to 16 cached heads' warps goes over the same
 // tiles of 32 keys side by side, each for its own head, so that what they
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kern
 // ring, so that a tile is fetched once for 64 or 128 rows. Nothing is split
 // along the keys. A warp leaves out the tiles that its own rows cannot see.
 // For f16 and float rows, and bf16 rows of 256 values (others: pkb_attn4_tc.cu).
-// Bound by the tile's instructions and mma.sync's rate: 2 (bf16), 3 (f16) or 5
+// Bound by the tile's instructions and mma.sync's rate: 3 (f16 and bf16) or 5
 // (float rows) products of 16 keys and 8 rows a 16 values. 8 sequences of 2,048
 // tokens, 8 heads of 128, 256 float rows a head: 188 us.
 
@@ -989,7 +993,7 @@ Bounds bounds_of(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
 cudaError_t prepare_attention4() {
     cudaError_t e = prepare_type<float, 3>();
     if (e == cudaSuccess) e = prepare_type<__half, 2>();
-    if (e == cudaSuccess) e = prepare_type<__nv_bfloat16, 1>();
+    if (e == cudaSuccess) e = prepare_type<__nv_bfloat16, 2>();
     if (e == cudaSuccess) e = prepare_attention4_tc();
     return e;
 }
@@ -1069,7 +1073,7 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
         const cudaError_t e = !split && attention4_tc_takes(a, type) ? launch_attention4_tc(a, s)
                               : type == PKB_F32 ? launch_type<float, 3>(a, grid, split, s)
                               : type == PKB_F16 ? launch_type<__half, 2>(a, grid, split, s)
-                                                : launch_type<__nv_bfloat16, 1>(a, grid, split, s);
+                                                : launch_type<__nv_bfloat16, 2>(a, grid, split, s);
         if (e != cudaSuccess)
             return set_error(e == cudaErrorMemoryAllocation ? PKB_ENOMEM : PKB_ECUDA, "%s launch: %s", who, cudaGetErrorString(e));
     }
