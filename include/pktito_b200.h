@@ -393,7 +393,10 @@ int pkb_cache4_reset_dev(void *stream, const pkb_cache4 *c);
 
 /* Room for add[i] >= 0 more tokens at the end of sequence seqs[i], i < n
  * (device arrays): lens grows, and new pages are the lowest free ones, in
- * the order listed. The tokens' rows are then appended layer by layer. */
+ * the order listed. The tokens' rows are then appended layer by layer, by
+ * pkb_cache4_append_if_dev where nobody looks at *status before: where it is
+ * not 0 no sequence has the new tokens, and rows appended all the same would
+ * replace those of its last ones. */
 int pkb_cache4_grow_dev(void *stream, const pkb_cache4 *c, const int32_t *seqs, const int32_t *add, uint32_t n,
                         int32_t *status, void *work, size_t work_bytes);
 
@@ -428,10 +431,18 @@ int pkb_cache4_compact_dev(void *stream, const pkb_cache4 *c, int32_t *used, int
  * counts already. seqs [n] and starts [n+1] are device arrays, starts from
  * 0 to at most rows; rows behind starts[n] are not read. A sequence
  * listed twice has no defined content. A sequence out of range, more rows
- * than tokens or a table entry that is no page sets the device error word's
- * bit 1, and nothing is written there. */
+ * than tokens, a table entry that is no page or a page that other sequences
+ * hold too (refs not 1) sets the device error word's bit 1, and nothing is
+ * written there. */
 int pkb_cache4_append_dev(void *stream, const pkb_cache4 *c, uint32_t layer, const void *k, size_t ks, const void *v,
                           size_t vs, int type, const int32_t *seqs, const int32_t *starts, uint32_t n, uint32_t rows);
+
+/* The same after a page operation: where *status (on the device, as that
+ * call on the stream left it) is not 0, nothing is written and no error set.
+ * A null status is pkb_cache4_append_dev. */
+int pkb_cache4_append_if_dev(void *stream, const pkb_cache4 *c, uint32_t layer, const void *k, size_t ks, const void *v,
+                             size_t vs, int type, const int32_t *seqs, const int32_t *starts, uint32_t n, uint32_t rows,
+                             const int32_t *status);
 
 /* The reverse: what the last starts[i+1] - starts[i] tokens of sequence
  * seqs[i] stand for, into rows of k and v (rounded once for PKB_F16). Rows

@@ -141,6 +141,10 @@ _SIGS = {
     "pkb_cache4_append_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
                                              ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int,
                                              ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32]),
+    "pkb_cache4_append_if_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
+                                                ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int,
+                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
+                                                ctypes.c_void_p]),
     "pkb_cache4_read_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
                                            ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int,
                                            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32]),
@@ -539,12 +543,12 @@ def cache4_compact_dev(cache: Cache4, used, status, work, stream=None) -> None:
 
 
 def cache4_append_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
-                      stream=None) -> None:
+                      stream=None, status=None) -> None:
     """K and V rows, ks and vs values apart, into the layer: rows starts[i] .. starts[i+1] - 1 are the last
-    tokens of sequence seqs[i]."""
-    _check(lib().pkb_cache4_append_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
-                                       _rows_type(cache, k, v), _ints(cache, seqs, n),
-                                       _ints(cache, starts, n + 1 if n else 0), n, rows))
+    tokens of sequence seqs[i]. With the status (device int32) of the grow before it: nothing where that is not 0."""
+    _check(lib().pkb_cache4_append_if_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
+                                          _rows_type(cache, k, v), _ints(cache, seqs, n),
+                                          _ints(cache, starts, n + 1 if n else 0), n, rows, _ints(cache, status, 1)))
 
 
 def cache4_read_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,

@@ -37,7 +37,7 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 
 struct RowArgs {
     Cache4 c;
-    const int32_t *seqs, *starts;
+    const int32_t *seqs, *starts, *status;  // status: of the page operation before, or null
     uint32_t* err;
     size_t ks, vs;
     uint32_t layer, n, rows, slots;
@@ -72,6 +72,7 @@ __device__ __forceinline__ uint32_t entry_at(const int32_t* starts, uint32_t n, 
 // row `row0 + r` for r in [first, last).
 struct UnitRows {
     uint8_t* bytes;
+    const int32_t* users;  // of its page
     int64_t row0;
     int first, last;
 };
@@ -84,7 +85,7 @@ struct UnitRows {
 // slot, 14.5 with one warp for an entry's two units, whose loop costs the long
 // entries 62 -> 67.)
 __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, uint32_t h) {
-    UnitRows u = {nullptr, 0, 0, 0};
+    UnitRows u = {nullptr, nullptr, 0, 0, 0};
     uint32_t i = slot / 2, k = slot % 2;
     if (i >= a.n) {
         const uint32_t x = slot - 2 * a.n;
@@ -103,7 +104,7 @@ __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, u
     }
     const uint32_t pos0 = len - rows, unit = pos0 / C4_UNIT + k;
     if (unit > (len - 1) / C4_UNIT) return u;  // the entry has no such unit
-    u.bytes = c4_unit(a.c, a.layer, seq, h, unit, a.err);
+    u.bytes = c4_unit(a.c, a.layer, seq, h, unit, &u.users, a.err);
     const int64_t t0 = static_cast<int64_t>(unit) * C4_UNIT - pos0;
     u.row0 = r0 + t0;
     u.first = t0 < 0 ? static_cast<int>(-t0) : 0;
@@ -157,11 +158,14 @@ __device__ __forceinline__ float quantize_block(float (&f)[8], uint32_t (&nib)[8
     return scaled ? s : 0.0f;
 }
 
-// One unit's K or V; x: the head's values of row 0, xs apart.
+// One unit's K or V; x: the head's values of row 0, xs apart. A page that
+// other sequences hold too keeps its bytes: how many do is read beside the
+// rows and looked at before the first store.
 template <typename T, int NB, bool VEC>
-__device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRows& u, bool is_v, uint8_t* vb) {
+__device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRows& u, bool is_v, uint8_t* vb, uint32_t* err) {
     constexpr int DK = NB * 32;
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
+    const int32_t users = *u.users;
     x += 8 * t;
     uint8_t* codes = u.bytes + (is_v ? 8 * DK : 0);
     __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(u.bytes + (is_v ? 17 * DK : 16 * DK));
@@ -178,6 +182,7 @@ __device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRow
             for (int i = 0; i < 8; i++) f[b][i] = 0.0f;
             if (valid) c4_load8<T, VEC>(x + (u.row0 + token) * xs + b * 32, f[b]);
         }
+        const bool write = valid && users == 1;
         uint32_t words[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -188,7 +193,7 @@ __device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRow
 #pragma unroll
                 for (int i = 0; i < 8; i++) w |= nib[i] << (4 * (i / 2) + 16 * (i % 2));
                 words[b] = w;
-                if (valid && t == 0) scales[token * NB + b] = s;
+                if (write && t == 0) scales[token * NB + b] = s;
             } else {
                 const uint32_t lo = nib[0] | nib[1] << 8 | nib[2] << 16 | nib[3] << 24;
                 const uint32_t hi = nib[4] | nib[5] << 8 | nib[6] << 16 | nib[7] << 24;
@@ -196,10 +201,10 @@ __device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRow
                 const uint32_t got = __shfl_xor_sync(FULL, t & 1 ? lo : hi, 1);
                 const uint32_t w = t & 1 ? got | hi << 4 : lo | got << 4;
                 *reinterpret_cast<uint32_t*>(vb + token * v_row<NB>() + (b * 2 + t / 2) * 8 + (t & 1) * 4) = w;
-                if (valid && t == 0) scales[b * C4_UNIT + token] = s;
+                if (write && t == 0) scales[b * C4_UNIT + token] = s;
             }
         }
-        if (!is_v && valid) {
+        if (!is_v && write) {
             uint32_t* at = reinterpret_cast<uint32_t*>(codes) + (token * 4 + t) * NB;
             if constexpr (NB % 4 == 0) {
 #pragma unroll
@@ -209,6 +214,10 @@ __device__ __forceinline__ void append_unit(const T* x, size_t xs, const UnitRow
                 for (int b = 0; b < NB; b++) at[b] = words[b];
             }
         }
+    }
+    if (users != 1) {
+        if (lane == 0) atomicOr(err, PKB_DEVERR_ARGS);
+        return;
     }
     if (!is_v) return;
     __syncwarp();
@@ -256,10 +265,12 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, NB == 8 ? 2 : 4) append_kernel
     __shared__ alignas(16) uint8_t stage[ROW_WARPS][C4_UNIT * v_row<NB>()];
     pdl_trigger();
     pdl_wait();
+    if (a.status && *a.status) return;  // the tokens that the rows are for were not taken
     const RowItem me(a);
     if (me.slot >= a.slots) return;
     const UnitRows u = warp_unit(a, static_cast<uint32_t>(me.slot), me.h);
-    if (u.bytes) append_unit<T, NB, VEC>((me.is_v ? v : k) + me.h * (NB * 32), me.is_v ? a.vs : a.ks, u, me.is_v, stage[threadIdx.x / 32]);
+    if (u.bytes)
+        append_unit<T, NB, VEC>((me.is_v ? v : k) + me.h * (NB * 32), me.is_v ? a.vs : a.ks, u, me.is_v, stage[threadIdx.x / 32], a.err);
 }
 
 // a bf16 pair's two values at p (8-byte, or 4-byte aligned for 16-bit types, where VEC)
@@ -785,7 +796,7 @@ cudaError_t launch_rows_dk(bool append, bool vec, void* k, void* v, const RowArg
 }
 
 int rows_call(cudaStream_t stream, bool append, const pkb_cache4* c, uint32_t layer, void* k, size_t ks, void* v, size_t vs,
-              int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows) {
+              int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows, const int32_t* status) {
     const char* who = append ? "cache4_append" : "cache4_read";
     RowArgs a = {};
     int rc = c4_view(c, who, &a.c);
@@ -797,7 +808,7 @@ int rows_call(cudaStream_t stream, bool append, const pkb_cache4* c, uint32_t la
     const size_t width = static_cast<size_t>(c->n_heads) * c->head_dim, size = c4_type_bytes(type);
     if (rows > 1 && (ks < width || vs < width)) return set_error(PKB_EINVAL, "%s: a row stride below %zu values", who, width);
     if (rows == 1) ks = vs = width;
-    if (!is_aligned(k, size) || !is_aligned(v, size) || !is_aligned(seqs, 4) || !is_aligned(starts, 4))
+    if (!is_aligned(k, size) || !is_aligned(v, size) || !is_aligned(seqs, 4) || !is_aligned(starts, 4) || !is_aligned(status, 4))
         return set_error(PKB_EINVAL, "%s: misaligned buffer", who);
     const uint64_t slots = static_cast<uint64_t>(rows) / C4_UNIT + 2 * static_cast<uint64_t>(n);
     if (rows > INT_MAX || slots * 2 * c->n_heads / ROW_WARPS >= INT_MAX)
@@ -807,6 +818,7 @@ int rows_call(cudaStream_t stream, bool append, const pkb_cache4* c, uint32_t la
     if ((rc = current_device_info(&sms, &err))) return rc;
     a.seqs = seqs;
     a.starts = starts;
+    a.status = status;
     a.err = err;
     a.ks = ks;
     a.vs = vs;
@@ -936,12 +948,19 @@ int pkb_cache4_compact_dev(void* stream, const pkb_cache4* c, int32_t* used, int
 int pkb_cache4_append_dev(void* stream, const pkb_cache4* c, uint32_t layer, const void* k, size_t ks, const void* v,
                           size_t vs, int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows) {
     return rows_call(static_cast<cudaStream_t>(stream), true, c, layer, const_cast<void*>(k), ks, const_cast<void*>(v), vs,
-                     type, seqs, starts, n, rows);
+                     type, seqs, starts, n, rows, nullptr);
+}
+
+int pkb_cache4_append_if_dev(void* stream, const pkb_cache4* c, uint32_t layer, const void* k, size_t ks, const void* v,
+                             size_t vs, int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows,
+                             const int32_t* status) {
+    return rows_call(static_cast<cudaStream_t>(stream), true, c, layer, const_cast<void*>(k), ks, const_cast<void*>(v), vs,
+                     type, seqs, starts, n, rows, status);
 }
 
 int pkb_cache4_read_dev(void* stream, const pkb_cache4* c, uint32_t layer, void* k, size_t ks, void* v, size_t vs,
                         int type, const int32_t* seqs, const int32_t* starts, uint32_t n, uint32_t rows) {
-    return rows_call(static_cast<cudaStream_t>(stream), false, c, layer, k, ks, v, vs, type, seqs, starts, n, rows);
+    return rows_call(static_cast<cudaStream_t>(stream), false, c, layer, k, ks, v, vs, type, seqs, starts, n, rows, nullptr);
 }
 
 }  // extern "C"

@@ -25,16 +25,17 @@ struct Cache4 {
     size_t page_bytes, layer_bytes;
 };
 
-// Token `unit`'s sixteen of head h: the unit's bytes, or null (*err set)
-// where the table names no page.
+// Token `unit`'s sixteen of head h: the unit's bytes (*users: how many
+// sequences hold its page), or null (*err set) where the table names no page.
 __device__ __forceinline__ uint8_t* c4_unit(const Cache4& c, uint32_t layer, uint32_t seq, uint32_t h, uint32_t unit,
-                                            uint32_t* err) {
+                                            const int32_t** users, uint32_t* err) {
     const uint32_t per = c.pshift - 4;  // log2 of the units of a page
     const int32_t page = c.table[static_cast<size_t>(seq) * c.max_pages + (unit >> per)];
     if (page < 0 || static_cast<uint32_t>(page) >= c.n_pages) {
         atomicOr(err, 2u);
         return nullptr;
     }
+    *users = c.refs + page;
     return c.pages + layer * c.layer_bytes + static_cast<size_t>(page) * c.page_bytes + h * c.head_bytes +
            (unit & ((1u << per) - 1)) * static_cast<size_t>(c.unit_bytes);
 }

@@ -20,3 +20,76 @@ def test_weights_of_bf16_rows_have_sixteen_bits(dk, G, rows, monkeypatch):
     c = T.filled(lens, 32, 2, dk, seed=dk + rows)
     T.check_attention(c, lens, [rows] * 3, [1, 0, 2], G, "bf16", True, 0)
     T.check_attention(c, lens, [rows] * 3, [0, 2, 1], G, "bf16", False, 0, scale=0.05)
+
+
+def two_layers_of_four(kind="f32", page=16):
+    """Books with sequences 0 (40 tokens), 1 (16) and 2 (16, a fork that shares 1's page), rows in both layers, and no page left."""
+    x = T.Both(5, 4, 3, page, 2, 64, 2)
+    assert x.grow([0, 1], [40, 16]) == 0
+    g = torch.Generator("cuda").manual_seed(3)
+    for layer in range(2):
+        k, v = torch.randn((2, 56, 128), generator=g, device="cuda").to(T.KIND[kind])
+        T.append(x.c, layer, k, v, [0, 1], [40, 16])
+    x.raw = x.c.tensors[0].cpu().numpy().copy()
+    assert x.fork([1], [2], [16]) == 0 and x.grow([3], [5]) == 0
+    return x, g
+
+
+@pytest.mark.parametrize("add,status", [([1, 1, 1], R.Books.FULL), ([9, 0, 0], R.Books.LONG), ([0, -1, 0], R.Books.BAD)])
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("each", [1, 3])
+def test_a_step_that_found_no_room_leaves_every_token(add, status, graph, each):
+    # grow, append and attention in a row, as a decoder runs them: rows for tokens that were not taken go nowhere
+    x, g = two_layers_of_four()
+    n, seqs, add = 3 * each, T.ints([0, 1, 2]), T.ints(add)
+    k, v, q = torch.randn((3, n, 128), generator=g, device="cuda")
+    o, starts = torch.empty_like(q), T.ints([0, each, 2 * each, n])
+    work = torch.empty(P.attention_cache4_work_bytes(x.c, 2, n, 3), dtype=torch.uint8, device="cuda")
+
+    def step():
+        P.cache4_grow_dev(x.c, seqs, add, 3, x.status, x.work)
+        for layer in range(2):
+            P.cache4_append_dev(x.c, layer, k, 128, v, 128, seqs, starts, 3, n, status=x.status)
+            P.attention_cache4_dev(o, 128, q, 128, 2, x.c, layer, seqs, starts, 3, n, each, 0.125, True, 0, work)
+    if graph:
+        replay = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(replay):
+            step()
+        step = replay.replay
+    step()
+    assert x.b.grow([0, 1, 2], add.tolist()) == status
+    x.same(status)  # books, and every byte of every page
+    x.free([3])
+    x.free([2])
+    add.copy_(T.ints([1, 1, 0]))
+    seqs[2] = 3  # empty: none of its rows is a token
+    starts.copy_(T.ints([0, 1, 2, 2]))
+    step()
+    assert x.b.grow([0, 1, 3], [1, 1, 0]) == 0
+    T.no_errors()
+    assert int(x.status) == 0
+    for layer in range(2):
+        pages = R.Pages(x.c.tensors[0][layer].cpu().numpy().reshape(-1), 16, 2, 64)
+        for i, s in enumerate((0, 1)):
+            kk, vv = pages.read(x.c.tensors[1][s].cpu().numpy(), x.b.lens[s])
+            assert np.array_equal(kk[:, -1], R.held(k[i].double().cpu().numpy().reshape(2, 64)))
+            assert np.array_equal(vv[:, -1], R.held(v[i].double().cpu().numpy().reshape(2, 64)))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_a_page_that_others_hold_keeps_its_bytes(kind):
+    x, g = two_layers_of_four(kind)
+    k, v = torch.randn((2, 5, 128), generator=g, device="cuda").to(T.KIND[kind])
+    P.cache4_append_dev(x.c, 1, k, 128, v, 128, T.ints([1, 0, 2]), T.ints([0, 2, 3, 5]), 3, 5)
+    torch.cuda.synchronize()
+    assert P.device_errors(0) == 2
+    pages = R.Pages(x.raw[1].reshape(-1), 16, 2, 64)  # sequence 0's row is written, those of 1 and 2 are not
+    for which, y in enumerate((k, v)):
+        pages.write(x.b.rows[0][2], 39 % 16, which, *R.quantize(y[2].double().cpu().numpy().reshape(2, 64)))
+    x.raw[1] = pages.raw.reshape(x.raw[1].shape)
+    x.status.zero_()
+    x.same(0)
+    x.free([2])  # alone again
+    P.cache4_append_dev(x.c, 1, k, 128, v, 128, T.ints([1]), T.ints([0, 2]), 1, 5)
+    T.no_errors()
+    assert not np.array_equal(x.c.tensors[0].cpu().numpy(), x.raw)
