@@ -248,8 +248,12 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, volati
 
 // The same wait without the abort flag, still bounded: for a role that has
 // given up and must let its own copies or MMAs in flight land before the CTA
-// frees its shared memory and TMEM.
+// frees its shared memory and TMEM. However short the kernel's own waits may
+// be (PKB_WAIT_CYCLES), this one lasts a second: a copy that lands after its
+// CTA has gone writes into another's memory.
+constexpr long long DRAIN_CYCLES = 1ll << 31;
 __device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, long long limit) {
+    limit = limit < DRAIN_CYCLES ? DRAIN_CYCLES : limit;
     const long long t0 = clock64();
     for (;;) {
         if (mbar_try_wait(bar, parity)) return true;
