@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 #pragma unroll
             for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
             int32_t key0 = static_cast<int32_t>((e.unit0 + 2 * first) * C4_UNIT);
-            for (uint32_t left = stop - START - first; left; left--) {
+            for (uint32_t todo = stop - START - first; todo; todo--) {
                 if (!warp_wait(&full[warp][stage], phase, &gave_up, a.timeout)) {
                     // a copy that does not come: say so, let those in flight land, leave
                     gave_up = 1;
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
                 tile_step<NB, NT, PARTS>(mask, a, e, block, buf, q, key0, static_cast<int32_t>(e.len), o, m, l);
                 __syncwarp();
                 if (left) fetch(stage);
-                else flying--;
+                else flying--;  // nothing more to fetch: one copy fewer under way
                 key0 += TILE;
                 if (++stage == STAGES) stage = 0, phase ^= 1;
             }
