@@ -545,6 +545,7 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
         enter();
         int stage = 0, flying = 0;
         uint32_t phase = 0;
+        bool lost = false;  // a wait ran out: the rest of the share is not computed
         for (; flying < STAGES && left; flying++) fetch(flying);
         while (x < end) {
             // one item, or the part of it in this share
@@ -578,16 +579,17 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 #pragma unroll
             for (int i = 0; i < 2 * NT; i++) m[i] = NEG_INF, l[i] = 0.0f;
             int32_t key0 = static_cast<int32_t>((e.unit0 + 2 * first) * C4_UNIT);
-            for (uint32_t todo = stop - START - first; todo; todo--) {
+            for (uint32_t todo = lost ? 0 : stop - START - first; todo; todo--) {
                 if (!warp_wait(&full[warp][stage], phase, &gave_up, a.timeout)) {
-                    // a copy that does not come: say so, let those in flight land, leave
+                    // a copy that does not come: say so, and let those in flight land
                     gave_up = 1;
                     if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
                     for (; flying; flying--) {
                         mbar_drain(&full[warp][stage], phase, a.timeout);
                         if (++stage == STAGES) stage = 0, phase ^= 1;
                     }
-                    return;
+                    lost = true;
+                    break;
                 }
                 uint8_t* buf = ring + stage * BYTES;
                 // warp-uniform: tiles at the window's start, the causal edge and the last token
@@ -602,9 +604,9 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 #pragma unroll
             for (int i = 0; i < 2 * NT; i++) l[i] = column_sum(l[i]);
             const bool entire = first == 0 && stop == it.places;
-            if (entire) {
+            if (entire && !lost) {
                 write_rows<T, NB, NT>(a, e, h, block, o, l);
-            } else {
+            } else if (!lost) {
                 float4* part = reinterpret_cast<float4*>(a.part) + static_cast<size_t>(2 * v + (first == 0)) * (part_regs<NB, NT>() / 4) * 32 + lane;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; d++)
@@ -613,11 +615,12 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 #pragma unroll
                 for (int j = 0; j < NT; j++) part[(NB * 2 * NT + j) * 32] = make_float4(m[2 * j], m[2 * j + 1], l[2 * j], l[2 * j + 1]);
             }
-            // the share with an item's last tile says which shares have parts of it
+            // the share with an item's last tile says which shares have parts of
+            // it, whatever became of them: the join reads what this call wrote alone
             if (stop == it.places && lane == 0) {
                 const uint32_t team = it.head0 / a.team;
                 a.joins[((static_cast<size_t>(it.entry) * a.teams + team) * a.max_blocks + block) * a.team + member] =
-                    Attn4Join{entire ? Attn4Join::NONE : split.of(x0 + START), share, e.r0, e.rows};
+                    Attn4Join{entire || lost ? Attn4Join::NONE : split.of(x0 + START), share, e.r0, e.rows};
             }
         }
     }

@@ -1,6 +1,10 @@
 """The 4-bit cache and its attention on a B200 where they go wrong most easily:
 precision, ranges, shared and full pages. The helpers, and what each
 tolerance is made of, are test_gpu_cache4's."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -93,3 +97,44 @@ def test_a_page_that_others_hold_keeps_its_bytes(kind):
     P.cache4_append_dev(x.c, 1, k, 128, v, 128, T.ints([1]), T.ints([0, 2]), 1, 5)
     T.no_errors()
     assert not np.array_equal(x.c.tensors[0].cpu().numpy(), x.raw)
+
+
+SHORT_WAITS = """
+import time, torch
+import libpktito_b200 as P
+from tests import test_gpu_cache4 as T
+lens = [40011, 5, 9000, 0, 700]
+c = T.filled(lens, 64, 4, 128, seed=3)
+P.device_errors(0)
+cold, seen = torch.empty(256 << 20, dtype=torch.uint8, device="cuda"), 0
+for kind, G, each in (("bf16", 4, 1), ("f32", 1, 3), ("f16", 2, 9)) * 4:
+    H, n = 4 * G, 5 * each
+    q = torch.randn((n, H * 128), device="cuda").to(T.KIND[kind])
+    o = torch.full((n + 3, H * 128 + 8), 5.0, device="cuda").to(T.KIND[kind])
+    size = P.attention_cache4_work_bytes(c, H, n, 5)
+    work = torch.zeros((size + 4096,), dtype=torch.uint8, device="cuda")
+    cold.fill_(1)
+    torch.cuda.synchronize()
+    t = time.perf_counter()
+    P.attention_cache4_dev(o, H * 128 + 8, q, H * 128, H, c, 0, T.ints([0, 1, 2, 3, 4]), T.ints([each * i for i in range(6)]), 5, n, each,
+                           0.1, True, 0, work[:size])
+    torch.cuda.synchronize()
+    t = time.perf_counter() - t
+    word = P.device_errors(0)
+    assert word in (0, 1), word
+    assert not word or t < 0.5, t  # nobody waits for copies that were never asked for, a second each
+    assert (work[size:] == 0).all() and (o[n:] == 5).all() and (o[:, H * 128:] == 5).all()
+    assert (o[3 * each:4 * each, :H * 128] == 0).all()  # no tokens: zeros, whatever became of the others
+    if not word:
+        assert T.check_attention(c, lens, [each] * 5, [0, 1, 2, 3, 4], G, kind, True, 0, scale=0.1) <= 1
+    seen += word
+print("gave up", seen, "of 12")
+"""
+
+
+def test_short_waits_end_in_results_or_in_an_error():
+    # a process whose waits may last one cycle: what gives up says so, and nothing is read that the call did not write
+    r = subprocess.run([sys.executable, "-c", SHORT_WAITS], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, PKB_WAIT_CYCLES="1"), cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    print(r.stdout)
+    assert r.returncode == 0, r.stdout + r.stderr
