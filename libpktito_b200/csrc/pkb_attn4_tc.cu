@@ -363,7 +363,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     uint8_t* q_tile = smem;
     uint8_t* k_tile = q_tile + 2 * row_tile<NB>();
     uint8_t* v_tiles = k_tile + KV_STAGES * row_tile<NB>();
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    // the warp's index from one lane, so that the roles' branches are uniform to the compiler too
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(FULL, tid / 32, 0);
     if (tid == 0) {
         for (int i = 0; i < KV_STAGES; i++) {
             mbar_init(&bars.k_full[i], CODE_WARPS), mbar_init(&bars.v_full[i], CODE_WARPS);
@@ -428,63 +429,64 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
     tc_fence_after();
     constexpr uint32_t tmem = 0;  // where an allocation of all 512 columns begins
 
-    if (warp > MMA_WARP) {
+    // one instruction sets a warpgroup's registers, and all of its warps run it: the last one's spare warps too
+    if (warp >= MMA_WARP) {
         set_registers<ISSUE_REGS, false>();
-    } else if (warp == MMA_WARP) {
-        set_registers<ISSUE_REGS, false>();
-        // descriptors hold addresses in units of 16 bytes, in their low bits
-        const uint64_t q_at = sw128_kmajor_desc(smem_u32(q_tile)), k_at = sw128_kmajor_desc(smem_u32(k_tile)),
-                       v_at = sw128_kmajor_desc(smem_u32(v_tiles));
-        constexpr uint32_t QK = bf16_instr_desc(128, HALF), PV = bf16_instr_desc(128, DK);
-        const uint32_t me = elected();
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && warp_wait(bar, parity, &gave_up, a.timeout);
-            if (ok) tc_fence_after();
-            return ok;
-        };
-        auto scores = [&](uint32_t t, uint32_t i) {
-            const uint64_t qd = q_at + t * (row_tile<NB>() / 16), kd = k_at + i / 2 % KV_STAGES * (row_tile<NB>() / 16) + i % 2 * (HALF * 8);
-            const uint32_t to = S_COL + 128 * t + HALF * (i % 2);
-#pragma unroll
-            for (int k = 0; k < DK / 16; k++) mma_ss(me, to, qd + k / 4 * 1024 + k % 4 * 2, kd + k / 4 * 1024 + k % 4 * 2, QK, k > 0);
-            commit(me, &bars.s_full[t][i % 2]);
-            if (t + 1 == tiles && i % 2) commit(me, &bars.k_empty[i / 2 % KV_STAGES]);
-        };
-        auto values = [&](uint32_t t, uint32_t i) {
-            const uint64_t vd = v_at + i / 2 % KV_STAGES * (v_tile<NB>() / 16) + i % 2 * (DK * 8);
-            const uint32_t from = S_COL + 128 * t + HALF * (i % 2) + 32;
-#pragma unroll
-            for (int k = 0; k < HALF / 16; k++) mma_ts(me, O_COL + 128 * t, from + 8 * k, vd + 2 * k, PV, i > 0 || k > 0);
-            commit(me, &bars.o_full[t][i % 2]);
-            if (t + 1 == tiles && i % 2) commit(me, &bars.v_empty[i / 2 % KV_STAGES]);
-        };
-        if (halves && wait(&bars.k_full[0], 0)) {
-            for (uint32_t i = 0; i < halves && i < 2; i++)
-                for (uint32_t t = 0; t < tiles; t++) scores(t, i);
-        }
-        // a tile's scores of the half step after next follow its values: they
-        // take P's place in TMEM, and products of one thread run in their order
-        for (uint32_t i = 0; ok && i < halves; i++) {
-            const uint32_t j = i / 2, st = j % KV_STAGES, ph = j / KV_STAGES & 1, st1 = (j + 1) % KV_STAGES, ph1 = (j + 1) / KV_STAGES & 1;
-            if (i % 2 == 0 && !wait(&bars.v_full[st], ph)) break;
-            for (uint32_t t = 0; t < tiles; t++) {
-                if (!wait(&bars.p_full[t][i % 2], j & 1)) break;
-                values(t, i);
-                if (i + 2 >= halves) continue;
-                if (t == 0 && i % 2 == 0 && !wait(&bars.k_full[st1], ph1)) break;
-                scores(t, i + 2);
+        if (warp == MMA_WARP) {
+            // descriptors hold addresses in units of 16 bytes, in their low bits
+            const uint64_t q_at = sw128_kmajor_desc(smem_u32(q_tile)), k_at = sw128_kmajor_desc(smem_u32(k_tile)),
+                           v_at = sw128_kmajor_desc(smem_u32(v_tiles));
+            constexpr uint32_t QK = bf16_instr_desc(128, HALF), PV = bf16_instr_desc(128, DK);
+            const uint32_t me = elected();
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                ok = ok && warp_wait(bar, parity, &gave_up, a.timeout);
+                if (ok) tc_fence_after();
+                return ok;
+            };
+            auto scores = [&](uint32_t t, uint32_t i) {
+                const uint64_t qd = q_at + t * (row_tile<NB>() / 16), kd = k_at + i / 2 % KV_STAGES * (row_tile<NB>() / 16) + i % 2 * (HALF * 8);
+                const uint32_t to = S_COL + 128 * t + HALF * (i % 2);
+    #pragma unroll
+                for (int k = 0; k < DK / 16; k++) mma_ss(me, to, qd + k / 4 * 1024 + k % 4 * 2, kd + k / 4 * 1024 + k % 4 * 2, QK, k > 0);
+                commit(me, &bars.s_full[t][i % 2]);
+                if (t + 1 == tiles && i % 2) commit(me, &bars.k_empty[i / 2 % KV_STAGES]);
+            };
+            auto values = [&](uint32_t t, uint32_t i) {
+                const uint64_t vd = v_at + i / 2 % KV_STAGES * (v_tile<NB>() / 16) + i % 2 * (DK * 8);
+                const uint32_t from = S_COL + 128 * t + HALF * (i % 2) + 32;
+    #pragma unroll
+                for (int k = 0; k < HALF / 16; k++) mma_ts(me, O_COL + 128 * t, from + 8 * k, vd + 2 * k, PV, i > 0 || k > 0);
+                commit(me, &bars.o_full[t][i % 2]);
+                if (t + 1 == tiles && i % 2) commit(me, &bars.v_empty[i / 2 % KV_STAGES]);
+            };
+            if (halves && wait(&bars.k_full[0], 0)) {
+                for (uint32_t i = 0; i < halves && i < 2; i++)
+                    for (uint32_t t = 0; t < tiles; t++) scores(t, i);
+            }
+            // a tile's scores of the half step after next follow its values: they
+            // take P's place in TMEM, and products of one thread run in their order
+            for (uint32_t i = 0; ok && i < halves; i++) {
+                const uint32_t j = i / 2, st = j % KV_STAGES, ph = j / KV_STAGES & 1, st1 = (j + 1) % KV_STAGES, ph1 = (j + 1) / KV_STAGES & 1;
+                if (i % 2 == 0 && !wait(&bars.v_full[st], ph)) break;
+                for (uint32_t t = 0; t < tiles; t++) {
+                    if (!wait(&bars.p_full[t][i % 2], j & 1)) break;
+                    values(t, i);
+                    if (i + 2 >= halves) continue;
+                    if (t == 0 && i % 2 == 0 && !wait(&bars.k_full[st1], ph1)) break;
+                    scores(t, i + 2);
+                }
+            }
+            if (!ok) {
+                gave_up = 1;
+                if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
+                // what was issued finishes before TMEM is freed
+                commit(me, &bars.drain);
+                if (me) mbar_drain(&bars.drain, 0, a.timeout);
+                __syncwarp();
             }
         }
-        if (!ok) {
-            gave_up = 1;
-            if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
-            // what was issued finishes before TMEM is freed
-            commit(me, &bars.drain);
-            if (me) mbar_drain(&bars.drain, 0, a.timeout);
-            __syncwarp();
-        }
-    } else if (warp >= SOFT_WARPS && warp < MMA_WARP) {
+    } else if (warp >= SOFT_WARPS) {
         // codes to values: a warp a unit of each step
         set_registers<CODE_REGS, false>();
         const uint32_t w = warp - SOFT_WARPS, per = a.c.pshift - 4;
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
                 break;
             }
         }
-    } else if (warp < SOFT_WARPS && warp / 4 < tiles) {
+    } else if (warp / 4 < tiles) {
         // the rows: thread i of a tile's four warps has row i
         set_registers<SOFT_REGS, true>();
         const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
