@@ -109,8 +109,8 @@ __device__ __forceinline__ void write_rows(const Attn4Args& a, const Entry& e, u
         const Column c = column<NT>(a, e, block, i);
         if (!c.valid) continue;
         T* out = static_cast<T*>(a.o) + static_cast<size_t>(e.r0 + c.tok) * a.os + (h * a.G + c.r - c.tok * a.G) * (NB * 32) + g;
-        // a row that sees nothing has sum 0 and is zeros; a NaN sum gives NaNs
-        const float inv = l[i] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[i]);
+        // V came as quarters; a row that sees nothing has sum 0 and is zeros; a NaN sum gives NaNs
+        const float inv = l[i] == 0.0f ? 0.0f : __fdiv_rn(4.0f, l[i]);
 #pragma unroll
         for (int m = 0; m < 2 * NB; m++)
 #pragma unroll
@@ -369,16 +369,16 @@ __device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, cons
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 s2[c] = *reinterpret_cast<const uint32_t*>(unit + 17 * DK + (b * C4_UNIT + 8 * c + 2 * t) * 2);
-                ms[c] = c4_m24(s2[c]);
+                ms[c] = c4_m6(s2[c]);
             }
 #pragma unroll
             for (int d = 0; d < 2; d++) {
                 const uint32_t x = d ? w.y : w.x;
                 uint32_t a[4];
-                a[0] = c4_pair<0>(x, s2[0], ms[0]);
-                a[1] = c4_pair<1>(x, s2[0], ms[0]);
-                a[2] = c4_pair<2>(x, s2[1], ms[1]);
-                a[3] = c4_pair<3>(x, s2[1], ms[1]);
+                a[0] = c4_quarter<0>(x, s2[0], ms[0]);
+                a[1] = c4_quarter<1>(x, s2[0], ms[0]);
+                a[2] = c4_quarter<2>(x, s2[1], ms[1]);
+                a[3] = c4_quarter<3>(x, s2[1], ms[1]);
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kern
     for (int i = 0; i < 2; i++) {
         const Column c = column<NT>(a, e, block, 2 * j + i);
         if (!c.valid) continue;
-        const float l = i ? l1 : l0, inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        const float l = i ? l1 : l0, inv = l == 0.0f ? 0.0f : __fdiv_rn(4.0f, l);
         T* out = static_cast<T*>(a.o) + static_cast<size_t>(e.r0 + c.tok) * a.os + (h * a.G + c.r - c.tok * a.G) * (NB * 32) + d * 16 + g;
         out[0] = c4_round<T>(__fmul_rn(o[i], inv));
         out[8] = c4_round<T>(__fmul_rn(o[2 + i], inv));

@@ -19,8 +19,8 @@
 // codes' warps and the softmax, which end in 0.70 and some 0.9 ms without
 // them, get in each other's way for the rest.
 //
-// Eight warps turn K's and V's codes into the bf16 values that they stand for
-// (exactly: pkb_cache4.cuh) in the 128-byte swizzled tiles that the tensor
+// Eight warps turn K's and V's codes into bf16, quarters of the values that they
+// stand for (exactly: pkb_cache4.cuh) in the 128-byte swizzled tiles that the tensor
 // cores read: K as [keys][dk], V as [dk][keys], which is how a lane's codes
 // lie in the cache, in stores without bank conflicts. They load the codes a
 // step of 128 keys ahead into registers: with the bf16 tiles of two steps and
@@ -181,8 +181,8 @@ struct KCodes {
                 const bool pair = b < PAIRED;
                 const uint32_t x = pair && odd ? w[r][pair ? b ^ 1 : b] : w[r][b];
                 // the block's scale in both halves: the low or the high one of its pair's word
-                const uint32_t s2 = __byte_perm(s[r][b / 2], 0, pair && odd ? (b % 2 ? 0x1010 : 0x3232) : (b % 2 ? 0x3232 : 0x1010)), ms = c4_m24(s2);
-                const uint4 v = make_uint4(c4_pair<0>(x, s2, ms), c4_pair<1>(x, s2, ms), c4_pair<2>(x, s2, ms), c4_pair<3>(x, s2, ms));
+                const uint32_t s2 = __byte_perm(s[r][b / 2], 0, pair && odd ? (b % 2 ? 0x1010 : 0x3232) : (b % 2 ? 0x3232 : 0x1010)), ms = c4_m6(s2);
+                const uint4 v = make_uint4(c4_quarter<0>(x, s2, ms), c4_quarter<1>(x, s2, ms), c4_quarter<2>(x, s2, ms), c4_quarter<3>(x, s2, ms));
                 *reinterpret_cast<uint4*>((!pair ? last_at : b % 2 ? second_at : first_at) + b / 2 * 16384 + r * 1024) = v;
             }
     }
@@ -220,14 +220,14 @@ struct VCodes {
                     if (key >= left) s2[c] = 0;
                     else if (key + 1 >= left) s2[c] &= 0xFFFFu;
                 }
-                ms[c] = c4_m24(s2[c]);
+                ms[c] = c4_m6(s2[c]);
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const uint32_t x = j ? w[b].y : w[b].x;
                 asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + (32 * b + 16 * j) * 128),
-                             "r"(c4_pair<0>(x, s2[0], ms[0])), "r"(c4_pair<1>(x, s2[0], ms[0])), "r"(c4_pair<2>(x, s2[1], ms[1])),
-                             "r"(c4_pair<3>(x, s2[1], ms[1]))
+                             "r"(c4_quarter<0>(x, s2[0], ms[0])), "r"(c4_quarter<1>(x, s2[0], ms[0])), "r"(c4_quarter<2>(x, s2[1], ms[1])),
+                             "r"(c4_quarter<3>(x, s2[1], ms[1]))
                              : "memory");
             }
         }
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
         const Keys span = keys_of(a, e, min(tok, e.rows - 1));  // rows there are none of see what the last one does
         const uint32_t at = tmem + ((warp % 4) * 32 << 16), s_at = at + S_COL + 128 * t, o_at = at + O_COL + 128 * t;
-        const float scale = fmaxf(fabsf(a.scale), 1e-37f);  // of a scale 0 too
+        const float scale = fminf(fmaxf(__fmul_rn(4.0f, fabsf(a.scale)), 1e-37f), 3.0e38f);  // K comes as quarters; of a scale 0 too
         float m = NEG_INF, l = 0.0f;
         bool ok = true;
         // the values up to half step i are in O
@@ -581,8 +581,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
             gave_up = 1;
             if (lane == 0) atomicOr(a.err, PKB_DEVERR_TIMEOUT);
         } else {
-            // a row that sees nothing has sum 0 and is zeros; a NaN sum gives NaNs
-            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+            // V came as quarters; a row that sees nothing has sum 0 and is zeros; a NaN sum gives NaNs
+            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(4.0f, l);
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + static_cast<size_t>(e.r0 + tok) * a.os +
                                  static_cast<size_t>(h * a.G + row - tok * a.G) * DK;
 #pragma unroll

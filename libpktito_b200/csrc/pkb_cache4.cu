@@ -312,7 +312,7 @@ __device__ __forceinline__ void read_unit(T* x, size_t xs, const UnitRows& u, bo
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const uint32_t s2 = s[r][b] | static_cast<uint32_t>(s[r][b]) << 16;
-                const uint32_t p[4] = {c4_pair_any<0>(w[r][b], s2), c4_pair_any<1>(w[r][b], s2), c4_pair_any<2>(w[r][b], s2), c4_pair_any<3>(w[r][b], s2)};
+                const uint32_t p[4] = {c4_whole_pair<0>(w[r][b], s2), c4_whole_pair<1>(w[r][b], s2), c4_whole_pair<2>(w[r][b], s2), c4_whole_pair<3>(w[r][b], s2)};
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -335,7 +335,7 @@ __device__ __forceinline__ void read_unit(T* x, size_t xs, const UnitRows& u, bo
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const uint32_t y = j ? w.y : w.x;
-            uint32_t p[2][2] = {{c4_pair_any<0>(y, s2[0]), c4_pair_any<1>(y, s2[0])}, {c4_pair_any<2>(y, s2[1]), c4_pair_any<3>(y, s2[1])}};
+            uint32_t p[2][2] = {{c4_whole_pair<0>(y, s2[0]), c4_whole_pair<1>(y, s2[0])}, {c4_whole_pair<2>(y, s2[1]), c4_whole_pair<3>(y, s2[1])}};
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int token = static_cast<int>(g) + 8 * c;

@@ -66,38 +66,40 @@ __device__ __forceinline__ uint32_t c4_rows(const Cache4& c, const int32_t* seqs
     return static_cast<uint32_t>(b - a);
 }
 
-// The four pairs of a word's eight codes as bf16 pairs: a nibble n in the
-// top four mantissa bits of 16.0 is 16 + n, and the one fused (16 + n) s
-// - 24 s is c s exactly (24 s has 7 significant bits, c s 8), so neither
-// the conversion nor the scale rounds. Three instructions a pair. For scales
-// below 2^123 (24 s is finite).
-template <int J>
-__device__ __forceinline__ uint32_t c4_sixteens(uint32_t w) {
+// The four pairs of a word's eight codes as bf16 pairs, each a quarter of
+// what it stands for: a nibble n in the top four mantissa bits of 4.0 is
+// (16 + n) / 4, and the one fused (16 + n) / 4 s - 6 s is c s / 4 exactly (6 s
+// has 7 significant bits, c s 8), so neither the conversion nor the scale
+// rounds. Three instructions a pair. The quarter keeps 6 s finite for every
+// scale (24 s is not from 2^123 on, and a masked weight's 0 times it is a NaN in rows that do
+// not see the key), and c s / 4 normal for the smallest.
+template <int J, uint32_t BASE>
+__device__ __forceinline__ uint32_t c4_placed(uint32_t w) {
     const uint32_t at = J == 0 ? w << 3 : w >> (4 * J - 3);
     uint32_t r;
-    asm("lop3.b32 %0, %1, 0x00780078, 0x41804180, 0xEA;" : "=r"(r) : "r"(at));  // (at & mask) | 16.0
+    asm("lop3.b32 %0, %1, 0x00780078, %2, 0xEA;" : "=r"(r) : "r"(at), "n"(BASE));  // (at & mask) | BASE
     return r;
 }
 template <int J>
-__device__ __forceinline__ uint32_t c4_pair(uint32_t w, uint32_t s2, uint32_t m24s2) {
-    uint32_t r = c4_sixteens<J>(w);
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(r), "r"(s2), "r"(m24s2));
+__device__ __forceinline__ uint32_t c4_quarter(uint32_t w, uint32_t s2, uint32_t m6s2) {
+    uint32_t r = c4_placed<J, 0x40804080u>(w);  // 4.0
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(r), "r"(s2), "r"(m6s2));
     return r;
 }
 
-// The same for any scale: 16 + n less 24 first.
+// The whole of it, in four instructions: 16 + n less 24 first.
 template <int J>
-__device__ __forceinline__ uint32_t c4_pair_any(uint32_t w, uint32_t s2) {
+__device__ __forceinline__ uint32_t c4_whole_pair(uint32_t w, uint32_t s2) {
     uint32_t r;
-    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(c4_sixteens<J>(w)), "r"(0xC1C0C1C0u));
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(c4_placed<J, 0x41804180u>(w)), "r"(0xC1C0C1C0u));
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(s2));
     return r;
 }
 
-// -24 s of both halves
-__device__ __forceinline__ uint32_t c4_m24(uint32_t s2) {
+// -6 s of both halves
+__device__ __forceinline__ uint32_t c4_m6(uint32_t s2) {
     uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(s2), "r"(0xC1C0C1C0u));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(s2), "r"(0xC0C0C0C0u));
     return r;
 }
 

@@ -138,3 +138,32 @@ def test_short_waits_end_in_results_or_in_an_error():
                        env=dict(os.environ, PKB_WAIT_CYCLES="1"), cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     print(r.stdout)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dk,G,rows,at,causal_window", [(64, 2, 5, 268, 0), (128, 1, 40, 250, 17), (32, 1, 200, 150, 0), (128, 4, 150, 200, 0),
+                                                        (64, 1, 260, 30, 25), (256, 2, 70, 230, 9), (96, 1, 270, 133, 50)])
+def test_a_huge_value_reaches_the_rows_that_see_it_alone(kind, dk, G, rows, at, causal_window):
+    # masked weights are 0, so a held value has to be finite in the product: 0 times an infinity is a NaN
+    L, heads = 270, 2
+    c = T.make([L], 32, heads, dk, seed=5)
+    g = torch.Generator("cuda").manual_seed(5)
+    k, v = torch.randn((2, L, heads * dk), generator=g, device="cuda")
+    q = torch.randn((rows, heads * G * dk), generator=g, device="cuda").to(T.KIND[kind])
+    work = torch.empty(P.attention_cache4_work_bytes(c, heads * G, rows, 1), dtype=torch.uint8, device="cuda")
+
+    def run():
+        T.append(c, 0, k, v, [0], [L])
+        o = torch.empty_like(q)
+        P.attention_cache4_dev(o, heads * G * dk, q, heads * G * dk, heads * G, c, 0, T.ints([0]), T.ints([0, rows]), 1, rows, rows,
+                               dk ** -0.5, True, causal_window, work)
+        T.no_errors()
+        return o
+    clean = run()
+    v[at, 3], v[at, dk] = 3.3e38, -2.0 ** 126
+    got = run()
+    pos = L - rows + torch.arange(rows, device="cuda")
+    sees = (pos >= at) & ((pos < at + causal_window) if causal_window else True)
+    assert sees.any() and not sees.all()
+    assert torch.equal(got[~sees], clean[~sees])
+    assert not torch.equal(got[sees], clean[sees])
