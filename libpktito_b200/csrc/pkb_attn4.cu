@@ -151,19 +151,20 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
 }
 
 // A block's rows of q as the second operand of the products with K, which
-// are taken in f16: K's codes are whole numbers there (c4_whole), two thirds
-// of the instructions of scaled bf16 values, and their scales multiply the
-// sums of a block of 32. A row is brought to a largest value in [2^14, 2^15)
+// are taken in f16: K's codes are whole numbers there (c4_whole), fewer
+// instructions than scaled bf16 values, and their scales multiply the sums of
+// a block of 32. (Codes + 8, and + 72 in every other pair, with sums that start
+// at what that adds, save four of a word's instructions and cost as many moves:
+// 16 rows a head 48.0 us against 46.2, single tokens the same. And the large sums cut
+// off what small values of q add.) A row is brought to a largest value in [2^14, 2^15)
 // by a power of two, which its sums get back with the softmax's scale, and
 // is one f16 (bf16 and f16 rows) or two (float rows, PARTS 3): exact but for
 // 2^-24 of a float, and for 2^-39 of the row's largest value.
 template <int NB, int NT, int PARTS>
 struct Query {
-    static constexpr bool EXACT = PARTS == 3;
-    static constexpr int P = EXACT ? 2 : 1;
+    static constexpr int P = PARTS == 3 ? 2 : 1;
     uint32_t w[NB][2][NT][P][2];
-    float bias[NB][2 * NT];  // unless EXACT: where the sums start, -8 and -72 times the elements
-    float scale[2 * NT];     // of each of the lane's columns
+    float scale[2 * NT];  // of each of the lane's columns
 };
 
 template <typename T, int NB, int NT, int PARTS>
@@ -203,14 +204,6 @@ __device__ __forceinline__ void load_query(const Attn4Args& a, const Entry& e, u
 #pragma unroll
                 for (int z = 0; z < P; z++) q.w[b][y / 2][j][z][y % 2] = parts[z];
             }
-            if constexpr (!Query<NB, NT, PARTS>::EXACT) {
-                const uint32_t c[4] = {0xC800C800u, 0xC800C800u, 0xD480D480u, 0xD480D480u};  // -8, -72
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int step = 0; step < 2; step++) mma_f16(d, c, q.w[b][step][j][0][0], q.w[b][step][j][0][1]);
-                q.bias[b][2 * j] = d[0];
-                q.bias[b][2 * j + 1] = d[1];
-            }
         }
         const float back = fminf(fmaxf(__fmul_rn(a.scale * 6.103515625e-5f, __uint_as_float(static_cast<uint32_t>(min(x, 127) + 127) << 23)),
                                        -3.0e38f), 3.0e38f);  // scale 2^(x - 14)
@@ -223,7 +216,6 @@ __device__ __forceinline__ void load_query(const Attn4Args& a, const Entry& e, u
 template <int NB, int NT, int PARTS>
 __device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB, NT, PARTS>& q, float (&s)[NT][4]) {
     constexpr int DK = NB * 32, P = Query<NB, NT, PARTS>::P;
-    constexpr bool EXACT = Query<NB, NT, PARTS>::EXACT;
     const uint32_t lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     uint32_t w[2][NB];
     lds_words<NB>(unit + (g * 4 + t) * NB * 4, w[0]);
@@ -247,12 +239,11 @@ __device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB,
         float k[2];
 #pragma unroll
         for (int r = 0; r < 2; r++) k[r] = __uint_as_float(b % 2 ? sc[r][b / 2] & 0xFFFF0000u : sc[r][b / 2] << 16);
-        const uint32_t a0[4] = {c4_whole<0, EXACT>(w[0][b]), c4_whole<0, EXACT>(w[1][b]), c4_whole<1, EXACT>(w[0][b]), c4_whole<1, EXACT>(w[1][b])};
-        const uint32_t a1[4] = {c4_whole<2, EXACT>(w[0][b]), c4_whole<2, EXACT>(w[1][b]), c4_whole<3, EXACT>(w[0][b]), c4_whole<3, EXACT>(w[1][b])};
+        const uint32_t a0[4] = {c4_whole<0>(w[0][b]), c4_whole<0>(w[1][b]), c4_whole<1>(w[0][b]), c4_whole<1>(w[1][b])};
+        const uint32_t a1[4] = {c4_whole<2>(w[0][b]), c4_whole<2>(w[1][b]), c4_whole<3>(w[0][b]), c4_whole<3>(w[1][b])};
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (!EXACT) d[0] = d[2] = q.bias[b][2 * j], d[1] = d[3] = q.bias[b][2 * j + 1];
 #pragma unroll
             for (int p = P - 1; p >= 0; p--) {
                 mma_f16(d, a0, q.w[b][0][j][p][0], q.w[b][0][j][p][1]);

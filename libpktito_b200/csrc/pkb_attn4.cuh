@@ -87,21 +87,19 @@ __device__ __forceinline__ void f16_parts(float lo, float hi, uint32_t (&r)[PART
     }
 }
 
-// The codes of a word as f16 pairs of small whole numbers, without the
-// scale: the nibbles in place in the mantissa of 1024 (pairs 0 and 2) and of
-// 64 (pairs 1 and 3), so that a word takes one shift and four ANDs. EXACT:
-// c itself; else n (c + 8) of pairs 0 and 2 and 64 + n of 1 and 3, where the
-// accumulator starts at what that adds to the sum.
-template <int J, bool EXACT>
+// The codes of a word as f16 pairs of the whole numbers c, without the scale:
+// the nibbles in place in the mantissa of 1024 (pairs 0 and 2) and of 64
+// (pairs 1 and 3), so that a word takes one shift, four ANDs and four sums.
+template <int J>
 __device__ __forceinline__ uint32_t c4_whole(uint32_t w) {
     const uint32_t at = J < 2 ? w : w >> 8;
     uint32_t r;
     if constexpr (J % 2 == 0) {
         asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r) : "r"(at));
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(EXACT ? 0xE408E408u : 0xE400E400u));  // -1032, -1024
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xE408E408u));  // -1032
     } else {
         asm("lop3.b32 %0, %1, 0x00F000F0, 0x54005400, 0xEA;" : "=r"(r) : "r"(at));
-        if constexpr (EXACT) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xD480D480u));  // -72
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xD480D480u));  // -72
     }
     return r;
 }

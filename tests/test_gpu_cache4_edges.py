@@ -167,3 +167,18 @@ def test_a_huge_value_reaches_the_rows_that_see_it_alone(kind, dk, G, rows, at, 
     assert sees.any() and not sees.all()
     assert torch.equal(got[~sees], clean[~sees])
     assert not torch.equal(got[sees], clean[sees])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dk,G,rows", [(32, 1, 1), (64, 4, 1), (128, 8, 1), (96, 3, 4), (128, 1, 40), (256, 2, 1), (256, 1, 200), (64, 1, 300)])
+def test_sums_are_as_exact_as_what_they_add(kind, dk, G, rows):
+    # half of q is large and of one sign, and meets zeros of K: what it does not add may not cost bits of what the rest does
+    lens, heads = [700, 320], 2
+    c = T.make(lens, 32, heads, dk, seed=dk)
+    g = torch.Generator("cuda").manual_seed(dk + rows)
+    k, v = torch.randn((2, sum(lens), heads * dk), generator=g, device="cuda")
+    k[:, ::2] = 0
+    T.append(c, 0, k, v, [0, 1], lens)
+    q = torch.randn((2 * rows, heads * G * dk), generator=g, device="cuda") * 2.0 ** -9
+    q[:, ::2] = 1
+    T.check_attention(c, lens, [rows] * 2, [1, 0], G, kind, True, 0, scale=2.0 ** 9 * 2 / (dk / 2) ** 0.5, q=q.to(T.KIND[kind]))
