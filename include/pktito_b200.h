@@ -471,8 +471,9 @@ size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t
  * sum is that of the unrounded ones. Rows of o
  * behind starts[n] are left as they were; o must not overlap q. work as for
  * the page operations. What is out of range sets the device error word's bit
- * 1, and such rows of o are not defined. A block of 2^126 or more is held and
- * read back, but may make the rows that see it, and no others, infinite or NaN. */
+ * 1, and such rows of o are not defined. Scores and sums are floats: a row
+ * whose scores pass a float's range, or that sees values whose sum does 2^8
+ * times over, is infinite or NaN, and no other row is. */
 int pkb_attention_cache4_dev(void *stream, void *o, size_t os, const void *q, size_t qs, int type, uint32_t H,
                              const pkb_cache4 *c, uint32_t layer, const int32_t *seqs, const int32_t *starts,
                              uint32_t n, uint32_t rows, uint32_t max_rows, float scale, int causal, uint32_t window,

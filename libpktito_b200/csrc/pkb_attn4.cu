@@ -157,14 +157,17 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
 // at what that adds, save four of a word's instructions and cost as many moves:
 // 16 rows a head 48.0 us against 46.2, single tokens the same. And the large sums cut
 // off what small values of q add.) A row is brought to a largest value in [2^14, 2^15)
-// by a power of two, which its sums get back with the softmax's scale, and
-// is one f16 (bf16 and f16 rows) or two (float rows, PARTS 3): exact but for
-// 2^-24 of a float, and for 2^-39 of the row's largest value.
+// by a power of two. What that and the softmax's scale are together, up to 2^0,
+// goes into K's scales before they multiply the sums, which alone pass a float's
+// range for K from 2^104 on; the rest multiplies the scores (23 float rows of
+// 32 sequences 26.7 -> 27.7 us in a graph, single tokens 1 %). A row is one f16 (bf16 and f16
+// rows) or two (float rows, PARTS 3): exact but for 2^-24 of a float, and for
+// 2^-39 of the row's largest value.
 template <int NB, int NT, int PARTS>
 struct Query {
     static constexpr int P = PARTS == 3 ? 2 : 1;
     uint32_t w[NB][2][NT][P][2];
-    float scale[2 * NT];  // of each of the lane's columns
+    uint64_t k_scale[NT], scale[NT];  // of each pair of the lane's columns
 };
 
 template <typename T, int NB, int NT, int PARTS>
@@ -205,14 +208,16 @@ __device__ __forceinline__ void load_query(const Attn4Args& a, const Entry& e, u
                 for (int z = 0; z < P; z++) q.w[b][y / 2][j][z][y % 2] = parts[z];
             }
         }
-        const float back = fminf(fmaxf(__fmul_rn(a.scale * 6.103515625e-5f, __uint_as_float(static_cast<uint32_t>(min(x, 127) + 127) << 23)),
-                                       -3.0e38f), 3.0e38f);  // scale 2^(x - 14)
-        q.scale[2 * j] = __shfl_sync(FULL, back, static_cast<int>(2 * t * 4));
-        q.scale[2 * j + 1] = __shfl_sync(FULL, back, static_cast<int>((2 * t + 1) * 4));
+        // scale 2^(x - 14) as a power of two in [2^-126, 1] and the rest
+        const int e0 = min(x, 127) - 14, e1 = max(min(e0 + max(static_cast<int>(__float_as_uint(a.scale) >> 23 & 255), 1) - 127, 0), -126);
+        const float k_scale = __uint_as_float(static_cast<uint32_t>(e1 + 127) << 23), rest = fminf(fmaxf(ldexpf(a.scale, e0 - e1), -3.0e38f), 3.0e38f);
+        const int c0 = static_cast<int>(2 * t * 4), c1 = c0 + 4;
+        q.k_scale[j] = pack2(__shfl_sync(FULL, k_scale, c0), __shfl_sync(FULL, k_scale, c1));
+        q.scale[j] = pack2(__shfl_sync(FULL, rest, c0), __shfl_sync(FULL, rest, c1));
     }
 }
 
-// Scores of one unit, before the scale: S^T[keys g, g + 8][columns 2t, 2t + 1].
+// Scores of one unit: S^T[keys g, g + 8][columns 2t, 2t + 1].
 template <int NB, int NT, int PARTS>
 __device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB, NT, PARTS>& q, float (&s)[NT][4]) {
     constexpr int DK = NB * 32, P = Query<NB, NT, PARTS>::P;
@@ -236,9 +241,12 @@ __device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB,
     }
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        float k[2];
+        uint64_t k[2];
 #pragma unroll
-        for (int r = 0; r < 2; r++) k[r] = __uint_as_float(b % 2 ? sc[r][b / 2] & 0xFFFF0000u : sc[r][b / 2] << 16);
+        for (int r = 0; r < 2; r++) {
+            const float x = __uint_as_float(b % 2 ? sc[r][b / 2] & 0xFFFF0000u : sc[r][b / 2] << 16);
+            k[r] = pack2(x, x);
+        }
         const uint32_t a0[4] = {c4_whole<0>(w[0][b]), c4_whole<0>(w[1][b]), c4_whole<1>(w[0][b]), c4_whole<1>(w[1][b])};
         const uint32_t a1[4] = {c4_whole<2>(w[0][b]), c4_whole<2>(w[1][b]), c4_whole<3>(w[0][b]), c4_whole<3>(w[1][b])};
 #pragma unroll
@@ -250,7 +258,12 @@ __device__ __forceinline__ void unit_scores(const uint8_t* unit, const Query<NB,
                 mma_f16(d, a1, q.w[b][1][j][p][0], q.w[b][1][j][p][1]);
             }
 #pragma unroll
-            for (int x = 0; x < 4; x++) s[j][x] = b ? __fmaf_rn(d[x], k[x / 2], s[j][x]) : __fmul_rn(d[x], k[x / 2]);
+            for (int r = 0; r < 2; r++) {
+                const uint64_t ks = mul2_r<0>(k[r], q.k_scale[j]), y = pack2(d[2 * r], d[2 * r + 1]);
+                uint64_t sum = b ? fma2_r<0>(y, ks, pack2(s[j][2 * r], s[j][2 * r + 1])) : mul2_r<0>(y, ks);
+                if (b + 1 == NB) sum = mul2_r<0>(sum, q.scale[j]);
+                unpack2(sum, s[j][2 * r], s[j][2 * r + 1]);
+            }
         }
     }
 }
@@ -278,13 +291,6 @@ __device__ __forceinline__ void tile_step(bool mask, const Attn4Args& args, cons
     unit_scores<NB, NT, PARTS>(buf, q, s[0]);
     unit_scores<NB, NT, PARTS>(buf + 18 * DK, q, s[1]);
     bool above = false;
-#pragma unroll
-    for (int i = 0; i < 2 * NT; i++) {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) s[u][i / 2][i % 2 + 2 * r] = __fmul_rn(s[u][i / 2][i % 2 + 2 * r], q.scale[i]);
-    }
     if (mask) {
 #pragma unroll
         for (int i = 0; i < 2 * NT; i++) {

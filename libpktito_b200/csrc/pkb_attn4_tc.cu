@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(Attn4Args a) {
         const uint32_t t = warp / 4, row = row0 + tid, tok = row / a.G;
         const Keys span = keys_of(a, e, min(tok, e.rows - 1));  // rows there are none of see what the last one does
         const uint32_t at = tmem + ((warp % 4) * 32 << 16), s_at = at + S_COL + 128 * t, o_at = at + O_COL + 128 * t;
-        const float scale = fminf(fmaxf(__fmul_rn(4.0f, fabsf(a.scale)), 1e-37f), 3.0e38f);  // K comes as quarters; of a scale 0 too
+        const float scale = fminf(fmaxf(__fmul_rn(4.0f, fabsf(a.scale)), 0x1p-149f), 3.0e38f);  // K comes as quarters; a scale of 0 as the least there is
         float m = NEG_INF, l = 0.0f;
         bool ok = true;
         // the values up to half step i are in O

@@ -182,3 +182,19 @@ def test_sums_are_as_exact_as_what_they_add(kind, dk, G, rows):
     q = torch.randn((2 * rows, heads * G * dk), generator=g, device="cuda") * 2.0 ** -9
     q[:, ::2] = 1
     T.check_attention(c, lens, [rows] * 2, [1, 0], G, kind, True, 0, scale=2.0 ** 9 * 2 / (dk / 2) ** 0.5, q=q.to(T.KIND[kind]))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dk,G,rows", [(32, 1, 1), (64, 4, 1), (128, 8, 1), (96, 3, 4), (128, 1, 40), (256, 2, 1), (256, 1, 200), (64, 1, 300)])
+@pytest.mark.parametrize("big,small,scale", [(124, -13, -111), (107, 0, -107), (124, -100, -24), (-118, 10, 108)])
+def test_keys_of_any_size(kind, dk, G, rows, big, small, scale):
+    # keys of some 2^big, queries of 2^small and a scale that makes scores of them: what a float holds comes out right
+    if kind == "f16" and small < -13:
+        pytest.skip("f16 rows end at 2^-14")
+    lens, heads = [300, 303], 1
+    c = T.make(lens, 32, heads, dk, seed=dk)
+    g = torch.Generator("cuda").manual_seed(dk + rows)
+    k, v = torch.randn((2, sum(lens), heads * dk), generator=g, device="cuda").clamp_(-3.5, 3.5)
+    T.append(c, 0, k * 2.0 ** big, v, [0, 1], lens)
+    q = (torch.randn((2 * rows, heads * G * dk), generator=g, device="cuda") * 2.0 ** small).to(T.KIND[kind])
+    T.check_attention(c, lens, [rows] * 2, [1, 0], G, kind, True, 0, scale=2.0 ** scale * dk ** -0.5, q=q)
