@@ -454,9 +454,14 @@ class Cache4(ctypes.Structure):
                       torch.zeros(n_pages, dtype=torch.int32, device=device), page_tokens, n_heads, head_dim)
 
 
+_types: dict = {}  # torch's types of rows: filled by the first call, as torch is loaded by then
+
+
 def _type(a) -> int:
-    import torch
-    kind = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(a.dtype)
+    if not _types:
+        import torch
+        _types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    kind = _types.get(a.dtype)
     if kind is None:
         raise PkbError(1, f"a tensor of {a.dtype}: float32, float16 or bfloat16")
     return kind
@@ -491,11 +496,31 @@ def _stream_of(cache: Cache4, stream) -> int:
     return torch._C._cuda_getCurrentRawStream(at)
 
 
-def _rows_type(cache: Cache4, a, b) -> int:
+def _holds(t, rows: int, stride: int, width: int) -> bool:
+    """Whether the tensor has rows of `width` values in one piece, `stride` values apart, from its first value on."""
+    need = (rows - 1) * stride + width
+    if t.is_contiguous():  # the most of calls: a microsecond less than to look at each dimension
+        return t.numel() >= need
+    dense, reach = 1, 1
+    for size, step in zip(reversed(t.shape), reversed(t.stride())):
+        if size != 1 and dense < width:
+            if step != dense:
+                return False
+            dense *= size
+        reach += (size - 1) * step
+    return t.numel() > 0 and reach >= need
+
+
+def _rows_type(cache: Cache4, rows: int, width: int, a, a_stride: int, b, b_stride: int) -> int:
+    """The type of two tensors that hold the rows of a call."""
     if a.dtype != b.dtype:
         raise PkbError(1, f"tensors of {a.dtype} and {b.dtype}")
-    if cache.int32 is not None and not a.get_device() == b.get_device() == cache.device:
-        raise PkbError(1, f"tensors on {a.device} and {b.device}: not the cache's device")
+    if cache.int32 is not None:
+        if not a.get_device() == b.get_device() == cache.device:
+            raise PkbError(1, f"tensors on {a.device} and {b.device}: not the cache's device")
+        if rows > 0 and not (_holds(a, rows, a_stride, width) and _holds(b, rows, b_stride, width)):
+            raise PkbError(1, f"tensors of {tuple(a.shape)} and {tuple(b.shape)}, strides {a.stride()} and {b.stride()}: {rows} rows "
+                              f"of {width} values in one piece, {a_stride} and {b_stride} values apart, expected")
     return _type(a)
 
 
@@ -547,16 +572,17 @@ def cache4_append_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, s
     """K and V rows, ks and vs values apart, into the layer: rows starts[i] .. starts[i+1] - 1 are the last
     tokens of sequence seqs[i]. With the status (device int32) of the grow before it: nothing where that is not 0."""
     _check(lib().pkb_cache4_append_if_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
-                                          _rows_type(cache, k, v), _ints(cache, seqs, n),
-                                          _ints(cache, starts, n + 1 if n else 0), n, rows, _ints(cache, status, 1)))
+                                          _rows_type(cache, rows, cache.n_heads * cache.head_dim, k, ks, v, vs),
+                                          _ints(cache, seqs, n), _ints(cache, starts, n + 1 if n else 0), n, rows,
+                                          _ints(cache, status, 1)))
 
 
 def cache4_read_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
                     stream=None) -> None:
     """What the last tokens of the sequences stand for, into rows of k and v."""
     _check(lib().pkb_cache4_read_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
-                                     _rows_type(cache, k, v), _ints(cache, seqs, n),
-                                     _ints(cache, starts, n + 1 if n else 0), n, rows))
+                                     _rows_type(cache, rows, cache.n_heads * cache.head_dim, k, ks, v, vs),
+                                     _ints(cache, seqs, n), _ints(cache, starts, n + 1 if n else 0), n, rows))
 
 
 def attention_cache4_work_bytes(cache: Cache4, H: int, rows: int, n: int) -> int:
@@ -567,7 +593,8 @@ def attention_cache4_dev(o, os_: int, q, qs: int, H: int, cache: Cache4, layer: 
                          max_rows: int, scale: float, causal: bool, window: int, work, stream=None) -> None:
     """Attention of q's rows (H heads) over the cache's layer: rows starts[i] .. starts[i+1] - 1 are the last
     positions of sequence seqs[i]; window 0: the whole history."""
-    _check(lib().pkb_attention_cache4_dev(_stream_of(cache, stream), _ptr(o), os_, _ptr(q), qs, _rows_type(cache, o, q),
-                                          H, ctypes.byref(cache), layer, _ints(cache, seqs, n),
+    _check(lib().pkb_attention_cache4_dev(_stream_of(cache, stream), _ptr(o), os_, _ptr(q), qs,
+                                          _rows_type(cache, rows, H * cache.head_dim, o, os_, q, qs), H, ctypes.byref(cache),
+                                          layer, _ints(cache, seqs, n),
                                           _ints(cache, starts, n + 1 if n else 0), n, rows, max_rows, scale,
                                           int(causal), window, *_work(cache, work)))

@@ -29,3 +29,46 @@ def test_append_checks_its_status():
     for bad in (good.long(), good[:0], good.float()):
         with pytest.raises(P.PkbError, match="int32"):
             P.cache4_append_dev(c, 0, rows, 64, rows, 64, good, good, 2, 4, 0, status=bad)
+
+
+def small():
+    import torch
+    return P.Cache4.of(torch.zeros((1, 5, P.cache4_page_bytes(16, 2, 32)), dtype=torch.uint8), torch.zeros((3, 4), dtype=torch.int32),
+                       torch.zeros(3, dtype=torch.int32), torch.zeros(5, dtype=torch.int32), 16, 2, 32)
+
+
+def short_rows():
+    """Tensors that do not hold 4 rows of 64 values, 80 values apart."""
+    import torch
+    x = torch.zeros((8, 160))
+    return [x[:2, :80], x[:4, :63], x[:2, :80].flatten()[:303], x[:4, :128:2], x[:4].t(), x[4:, :0], x[:4, :80].t().contiguous().t(),
+            x[:4].view(4, 4, 40)[:, :2, :32], x[7:, 100:], x[:1, :64].expand(4, 64)]
+
+
+@pytest.mark.parametrize("at", range(10))
+def test_calls_check_that_tensors_hold_their_rows(at):
+    import torch
+    c, n, bad, good = small(), torch.zeros(4, dtype=torch.int32), short_rows()[at], torch.zeros((4, 80))
+    work = torch.zeros(1 << 16, dtype=torch.uint8)
+    for a, b in ((bad, good), (good, bad)):
+        for call in (lambda: P.cache4_append_dev(c, 0, a, 80, b, 80, n, n, 2, 4, 0), lambda: P.cache4_read_dev(c, 0, a, 80, b, 80, n, n, 2, 4, 0),
+                     lambda: P.attention_cache4_dev(a, 80, b, 80, 2, c, 0, n, n, 2, 4, 4, 0.1, True, 0, work, 0)):
+            with pytest.raises(P.PkbError, match="4 rows of 64 values"):
+                call()
+
+
+def test_tensors_that_hold_their_rows_pass():
+    # as far as the device, which is not there
+    import torch
+    c, n, work = small(), torch.zeros(4, dtype=torch.int32), torch.zeros(1 << 16, dtype=torch.uint8)
+    x = torch.zeros((8, 160))
+    good = [x[:4], x[:4, 80:], x[:4, :64], x.view(8, 5, 32)[:4, 1:3], x.flatten()[:3 * 160 + 64], x[:4, None, :64], x.view(16, 80)[::2][:4, :64]]
+    if torch.cuda.is_available():
+        pytest.skip("host memory is no place for a device's rows")
+    for a in good:
+        b = torch.zeros((4, 160))
+        for call in (lambda: P.cache4_append_dev(c, 0, a, 160, b, 160, n, n, 2, 4, 0), lambda: P.cache4_read_dev(c, 0, a, 160, b, 160, n, n, 2, 4, 0),
+                     lambda: P.cache4_append_dev(c, 0, a[:1] if a.dim() > 1 else a, 1, b[:1], 0, n, n, 1, 1, 0)):
+            with pytest.raises(P.PkbError) as e:
+                call()
+            assert "ENODEV" in str(e.value), (a.shape, a.stride(), e.value)
