@@ -486,14 +486,12 @@ def _ints(cache: Cache4, t, n: int) -> int:
 
 
 def _stream_of(cache: Cache4, stream) -> int:
-    """The stream, by default the current one of the cache's device, which has to be the current device."""
-    if stream is not None:
-        return int(stream)
+    """The stream, by default the current one. The cache's device has to be the current one: that is where kernels run."""
     import torch
-    at = torch.cuda.current_device()
-    if cache.device not in (None, at):
-        raise PkbError(1, f"a cache on device {cache.device}, the current one is {at}")
-    return torch._C._cuda_getCurrentRawStream(at)
+    # (host memory is refused where there is a device that could be given it)
+    if cache.device is not None and (cache.device >= 0 or torch.cuda.is_available()) and cache.device != torch.cuda.current_device():
+        raise PkbError(1, f"a cache on device {cache.device}, the current one is {torch.cuda.current_device()}")
+    return int(stream) if stream is not None else torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _holds(t, rows: int, stride: int, width: int) -> bool:
@@ -551,6 +549,8 @@ def cache4_fork_dev(cache: Cache4, src, dst, lens, n: int, status, work, stream=
 
 def cache4_copy_dev(to: Cache4, cache: Cache4, src, dst, lens, n: int, status, work, stream=None) -> None:
     """The empty sequences dst of `to` take the first lens tokens of src in pages of their own."""
+    if None not in (to.device, cache.device) and to.device != cache.device:
+        raise PkbError(1, f"caches on devices {cache.device} and {to.device}")
     _check(lib().pkb_cache4_copy_dev(_stream_of(cache, stream), ctypes.byref(to), ctypes.byref(cache),
                                      _ints(cache, src, n), _ints(to, dst, n), _ints(cache, lens, n), n,
                                      _ints(cache, status, 1), *_work(cache, work)))

@@ -72,3 +72,28 @@ def test_tensors_that_hold_their_rows_pass():
             with pytest.raises(P.PkbError) as e:
                 call()
             assert "ENODEV" in str(e.value), (a.shape, a.stride(), e.value)
+
+
+@pytest.mark.parametrize("stream", [None, 0])
+def test_a_cache_on_another_device_than_the_current_one_is_refused(stream, monkeypatch):
+    import torch
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    c, n, x, work = small(), torch.zeros(4, dtype=torch.int32), torch.zeros((4, 64)), torch.zeros(1 << 16, dtype=torch.uint8)
+    for c.device in (-1, 1):  # host memory; a second GPU
+        for call in (lambda: P.cache4_reset_dev(c, stream), lambda: P.cache4_grow_dev(c, n, n, 2, n, work, stream),
+                     lambda: P.cache4_fork_dev(c, n, n, n, 2, n, work, stream), lambda: P.cache4_free_dev(c, n, 2, n, work, stream),
+                     lambda: P.cache4_copy_dev(c, c, n, n, n, 2, n, work, stream), lambda: P.cache4_compact_dev(c, None, n, work, stream),
+                     lambda: P.cache4_append_dev(c, 0, x, 64, x, 64, n, n, 2, 4, stream),
+                     lambda: P.cache4_read_dev(c, 0, x, 64, x, 64, n, n, 2, 4, stream),
+                     lambda: P.attention_cache4_dev(x, 64, x, 64, 2, c, 0, n, n, 2, 4, 4, 0.1, True, 0, work, stream)):
+            with pytest.raises(P.PkbError, match="a cache on device"):
+                call()
+
+
+def test_a_copy_between_devices_is_refused():
+    import torch
+    c, to, n, work = small(), small(), torch.zeros(4, dtype=torch.int32), torch.zeros(1 << 16, dtype=torch.uint8)
+    to.device = 1
+    with pytest.raises(P.PkbError, match="caches on devices"):
+        P.cache4_copy_dev(to, c, n, n, n, 2, n, work, 0)
