@@ -1026,6 +1026,7 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
     // one that reaches past every sequence's first token from its last row on is none
     if (window >= static_cast<uint64_t>(c->max_pages) * c->page_tokens + max_rows) window = 0;
     if (!n || !rows) return PKB_OK;
+    if (n > INT_MAX) return set_error(PKB_EINVAL, "%s: %u sequences", who, n);
     if (!o || !q || !seqs || !starts || !work) return set_error(PKB_EINVAL, "%s: null pointer", who);
     if (!max_rows || max_rows > rows) return set_error(PKB_EINVAL, "%s: max_rows = %u of %u rows", who, max_rows, rows);
     const size_t width = static_cast<size_t>(H) * c->head_dim, size = c4_type_bytes(type);

@@ -811,7 +811,7 @@ int rows_call(cudaStream_t stream, bool append, const pkb_cache4* c, uint32_t la
     if (!is_aligned(k, size) || !is_aligned(v, size) || !is_aligned(seqs, 4) || !is_aligned(starts, 4) || !is_aligned(status, 4))
         return set_error(PKB_EINVAL, "%s: misaligned buffer", who);
     const uint64_t slots = static_cast<uint64_t>(rows) / C4_UNIT + 2 * static_cast<uint64_t>(n);
-    if (rows > INT_MAX || slots * 2 * c->n_heads / ROW_WARPS >= INT_MAX)
+    if (rows > INT_MAX || slots > UINT_MAX || slots * 2 * c->n_heads / ROW_WARPS >= INT_MAX)
         return set_error(PKB_EINVAL, "%s: %u rows of %u sequences are too many for one launch", who, rows, n);
     uint32_t* err;
     int sms;

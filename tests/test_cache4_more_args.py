@@ -97,3 +97,9 @@ def test_a_copy_between_devices_is_refused():
     to.device = 1
     with pytest.raises(P.PkbError, match="caches on devices"):
         P.cache4_copy_dev(to, c, n, n, n, 2, n, work, 0)
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) - 1])
+def test_lists_past_what_is_counted_in_32_bits_are_refused(n):
+    one = A.cache(n_heads=1)
+    assert A.rows(one, n=n) == A.rows(one, append=False, n=n) == A.attend(one, H=1, n=n) == EINVAL
