@@ -40,6 +40,7 @@
 // fetches for all of a block's 55 and for itself each 52.
 
 #include <climits>
+#include <type_traits>
 
 #include "pkb_attn4.cuh"
 #include "pkb_internal.h"
@@ -858,11 +859,16 @@ template <int NB, int NT> size_t split_smem(uint32_t n) {
     return workers<NB, NT>() * stages<NB, NT>() * tile_bytes<NB>() + static_cast<size_t>(n) * (sizeof(Entry) + 4) + 4;
 }
 
+// What attention4_tc_takes leaves to rows_kernel: the others are not built.
+template <typename T, int NB> constexpr bool has_rows_kernel() { return !std::is_same<T, __nv_bfloat16>::value || NB == 8; }
+
 template <typename T, int NB, int NT, int PARTS>
 cudaError_t prepare_one() {
-    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, NB, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               ROW_STAGES * tile_bytes<NB>());
-    if (e != cudaSuccess) return e;
+    if constexpr (has_rows_kernel<T, NB>()) {
+        const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, NB, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   ROW_STAGES * tile_bytes<NB>());
+        if (e != cudaSuccess) return e;
+    }
     return cudaFuncSetAttribute(split_kernel<T, NB, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 static_cast<int>(split_smem<NB, NT>(MAX_ENTRIES)));
 }
@@ -907,7 +913,9 @@ cudaError_t launch_split(Attn4Args a, uint32_t grid, cudaStream_t s) {
 
 template <typename T, int NB, int NT, int PARTS>
 cudaError_t launch_one(const Attn4Args& a, uint32_t grid, bool split, cudaStream_t s) {
-    return split ? launch_split<T, NB, NT, PARTS>(a, grid, s) : launch_rows<T, NB, NT, PARTS>(a, s);
+    if (split) return launch_split<T, NB, NT, PARTS>(a, grid, s);
+    if constexpr (has_rows_kernel<T, NB>()) return launch_rows<T, NB, NT, PARTS>(a, s);
+    return cudaErrorInvalidValue;
 }
 
 // Rows of a block: two blocks of eight share the codes' conversion where there

@@ -198,3 +198,27 @@ def test_keys_of_any_size(kind, dk, G, rows, big, small, scale):
     T.append(c, 0, k * 2.0 ** big, v, [0, 1], lens)
     q = (torch.randn((2 * rows, heads * G * dk), generator=g, device="cuda") * 2.0 ** small).to(T.KIND[kind])
     T.check_attention(c, lens, [rows] * 2, [1, 0], G, kind, True, 0, scale=2.0 ** scale * dk ** -0.5, q=q)
+
+
+def test_large_lists_of_page_operations():
+    # 1,500 sequences of up to 16 pages in a pool of 40,003: forks of hundreds, and frees of more places than one block takes
+    x = T.Both(40003, 3000, 16, 16, 1, 32, 1)
+    rng = np.random.default_rng(2)
+    lens = rng.integers(1, 257, 1500).tolist()
+    assert x.grow(list(range(1500)), lens) == 0
+    assert x.free(list(range(0, 1500, 7))) == 0
+    live = [s for s in range(1500) if s % 7]
+    src = rng.choice(live, 1200).tolist()
+    dst = rng.permutation(list(range(1500, 3000)) + list(range(0, 1500, 7)))[:1200].tolist()
+    assert x.fork(src, dst, [int(rng.integers(0, lens[s] + 1)) for s in src]) == 0
+    held = [d for d in dst if x.b.lens[d]]
+    assert x.grow(held, [int(rng.integers(0, 257 - x.b.lens[s])) for s in held]) == 0
+    gone = rng.permutation(live)[:1100].tolist()
+    assert len(gone) * 16 > 16384
+    assert x.free(gone + gone[:1]) == x.free(gone + [3000]) == R.Books.BAD  # nothing of it
+    assert x.free(gone) == 0  # pages that forks hold stay
+    x.compact()
+    assert x.free(rng.permutation(dst).tolist()) == 0
+    assert x.copy([s for s in live if s not in set(gone)][:50], gone[:50], [0] * 50) == 0
+    x.compact()
+    assert x.free([s for s in range(3000)]) == 0 and int(x.c.tensors[3].sum()) == 0
