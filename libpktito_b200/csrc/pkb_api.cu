@@ -104,7 +104,6 @@ int current_device(Device** out) {
             d.err = static_cast<uint32_t*>(sym);
             PKB_CUDA(prepare_gemm_q8(), "kernel attributes");
             PKB_CUDA(prepare_attention(), "kernel attributes");
-            PKB_CUDA(prepare_attention4(), "kernel attributes");
             prepare_quantize();
             d.sms = prop.multiProcessorCount;
             wait_limit();

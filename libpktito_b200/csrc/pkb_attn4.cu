@@ -39,7 +39,9 @@
 // Scaled bf16 values for K too took 66 us for the 64 sequences, one warp that
 // fetches for all of a block's 55 and for itself each 52.
 
+#include <atomic>
 #include <climits>
+#include <mutex>
 #include <type_traits>
 
 #include "pkb_attn4.cuh"
@@ -996,15 +998,27 @@ Bounds bounds_of(const pkb_cache4* c, uint32_t H, uint32_t rows, uint32_t n) {
     return b;
 }
 
-}  // namespace
+// The kernels' attributes, at the first call on a device: it loads them all,
+// some 15 ms that a program without a cache does not pay at its own first call.
+constexpr int MAX_DEV = 16;  // current_device_info has checked that the device is below it
+std::mutex g_mu;
+std::atomic<bool> g_ready[MAX_DEV];
 
-cudaError_t prepare_attention4() {
-    cudaError_t e = prepare_type<float, 3>();
+cudaError_t prepare() {
+    int dev;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || g_ready[dev].load(std::memory_order_acquire)) return e;
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (g_ready[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    e = prepare_type<float, 3>();
     if (e == cudaSuccess) e = prepare_type<__half, 2>();
     if (e == cudaSuccess) e = prepare_type<__nv_bfloat16, 2>();
     if (e == cudaSuccess) e = prepare_attention4_tc();
+    if (e == cudaSuccess) g_ready[dev].store(true, std::memory_order_release);
     return e;
 }
+
+}  // namespace
 
 }  // namespace pkb
 
@@ -1051,6 +1065,8 @@ int pkb_attention_cache4_dev(void* stream, void* o, size_t os, const void* q, si
         return set_error(PKB_EINVAL, "%s: work area of %zu bytes (%zu needed, 256-byte aligned)", who, work_bytes, static_cast<size_t>(bounds.bytes));
     int sms;
     if ((rc = current_device_info(&sms, &a.err))) return rc;
+    const cudaError_t set_up = prepare();
+    if (set_up != cudaSuccess) return set_error(PKB_ECUDA, "%s kernel attributes: %s", who, cudaGetErrorString(set_up));
     a.q = q;
     a.o = o;
     a.qs = qs;

@@ -152,10 +152,6 @@ cudaError_t prepare_attention();
 // The dynamic shared memory an attention CTA may take (set by prepare_attention).
 size_t attention_smem_max();
 
-// The attention over a 4-bit cache's launch attributes (pkb_attn4.cu), once
-// a device at its set-up.
-cudaError_t prepare_attention4();
-
 // ------------------------------------------------ the TDT search (pkb_tdt.cu) --
 
 enum { TDT_LSTM = 0, TDT_JOINT_IN = 1, TDT_STEP = 2 };

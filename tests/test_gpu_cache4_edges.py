@@ -222,3 +222,36 @@ def test_large_lists_of_page_operations():
     assert x.copy([s for s in live if s not in set(gone)][:50], gone[:50], [0] * 50) == 0
     x.compact()
     assert x.free([s for s in range(3000)]) == 0 and int(x.c.tensors[3].sum()) == 0
+
+
+FIRST_CALLS = """
+import sys, torch
+import libpktito_b200 as P
+from tests import test_gpu_cache4 as T
+kind, rows = sys.argv[1], int(sys.argv[2])
+c = T.filled([300, 270], 32, 2, 64, seed=1)
+q = torch.randn((2 * rows, 256), device="cuda").to(T.KIND[kind])
+o, again = torch.empty_like(q), torch.empty_like(q)
+work = torch.empty(P.attention_cache4_work_bytes(c, 4, 2 * rows, 2), dtype=torch.uint8, device="cuda")
+seqs, starts = T.ints([0, 1]), T.ints([0, rows, 2 * rows])
+torch.cuda.synchronize()
+
+def call(to):
+    P.attention_cache4_dev(to, 256, q, 256, 4, c, 0, seqs, starts, 2, 2 * rows, rows, 0.125, True, 0, work)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    call(o)
+graph.replay()
+call(again)
+T.no_errors()
+assert torch.equal(o, again)
+assert T.check_attention(c, [300, 270], [rows] * 2, [0, 1], 2, kind, True, 0, scale=0.125, q=q) <= 1
+"""
+
+
+@pytest.mark.parametrize("kind,rows", [("f32", 1), ("bf16", 200), ("f16", 200)])
+def test_a_process_first_attention_may_be_a_captured_one(kind, rows):
+    # the kernels are set up by the first call, here inside a capture
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, kind, str(rows)], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout + r.stderr
