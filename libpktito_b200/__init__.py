@@ -488,10 +488,15 @@ def _ints(cache: Cache4, t, n: int) -> int:
 def _stream_of(cache: Cache4, stream) -> int:
     """The stream, by default the current one. The cache's device has to be the current one: that is where kernels run."""
     import torch
+    at = None
     # (host memory is refused where there is a device that could be given it)
-    if cache.device is not None and (cache.device >= 0 or torch.cuda.is_available()) and cache.device != torch.cuda.current_device():
-        raise PkbError(1, f"a cache on device {cache.device}, the current one is {torch.cuda.current_device()}")
-    return int(stream) if stream is not None else torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if cache.device is not None and (cache.device >= 0 or torch.cuda.is_available()):
+        at = torch.cuda.current_device()
+        if at != cache.device:
+            raise PkbError(1, f"a cache on device {cache.device}, the current one is {at}")
+    if stream is not None:
+        return int(stream)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if at is None else at)
 
 
 def _holds(t, rows: int, stride: int, width: int) -> bool:
@@ -574,7 +579,7 @@ def cache4_append_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, s
     _check(lib().pkb_cache4_append_if_dev(_stream_of(cache, stream), ctypes.byref(cache), layer, _ptr(k), ks, _ptr(v), vs,
                                           _rows_type(cache, rows, cache.n_heads * cache.head_dim, k, ks, v, vs),
                                           _ints(cache, seqs, n), _ints(cache, starts, n + 1 if n else 0), n, rows,
-                                          _ints(cache, status, 1)))
+                                          0 if status is None else _ints(cache, status, 1)))
 
 
 def cache4_read_dev(cache: Cache4, layer: int, k, ks: int, v, vs: int, seqs, starts, n: int, rows: int,
