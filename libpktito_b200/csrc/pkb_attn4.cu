@@ -921,13 +921,15 @@ cudaError_t launch_one(const Attn4Args& a, uint32_t grid, bool split, cudaStream
 }
 
 // Rows of a block: two blocks of eight share the codes' conversion where there
-// are more than eight rows (64 sequences of 2,048 tokens, 16 bf16 rows a head
-// of 128: 67 us, 78 in eights; 4 rows 66, 52 in eights). 17 to 24 float rows, whose
-// five products a 16 values are most of the work, are three eights (32
-// sequences of 1,500 tokens, 23 rows: 66 us, 73 in sixteens; 12 rows 48 and 42).
+// are more than eight rows (64 sequences of 2,048 tokens, heads of 128, bf16: 16
+// rows 72 us, 88 in eights; 4 rows 71, 52 in eights). Half of the last sixteen
+// is empty for 17 to 24 rows, which are three eights (32 sequences of 1,500
+// tokens: f16 54 us, 55.5 in sixteens; float 67 and 74.5), and for 33 to 40, which are five where they
+// are float, whose five products a 16 values are most of the work (103 us, 107 in
+// sixteens; f16 82.6 and 78); 52 rows are better off in sixteens (float 163 and 143).
 uint32_t block_rows(const Attn4Args& a, bool float_rows) {
-    const uint64_t rows = static_cast<uint64_t>(a.max_rows) * a.G;
-    return a.c.dk == 256 || rows <= 8 || (float_rows && rows > 16 && rows <= 24) ? 8 : 16;
+    const uint64_t rows = static_cast<uint64_t>(a.max_rows) * a.G, eights = (rows + 7) / 8;
+    return a.c.dk == 256 || eights == 1 || eights == 3 || (eights == 5 && float_rows) ? 8 : 16;
 }
 
 template <typename T, int PARTS>
@@ -957,22 +959,23 @@ uint64_t places_of(const pkb_cache4* c) { return static_cast<uint64_t>(c->max_pa
 // by blocks that go over all of an entry's keys. Lengths are not known here,
 // but both ways' times are proportional to them, so only the grids count:
 //  - bf16 on tcgen05: 16 rows of a split take the GPU as long as half an SM
-//    takes to do 256 (8 sequences of 2,048 tokens, 8 heads of 128 with 4 query
-//    heads each: 16 tokens 43 us split and 41 so, 32 tokens 64 and 42; one
-//    sequence of 8,192 tokens: 64 tokens 67 and 160).
+//    takes to do 256, or, where those are one tile of 128 and of heads so wide
+//    that unpacking bounds the split, as two thirds of one take (8 sequences of 2,048 tokens, 8 heads of 128
+//    with 4 query heads each: 16 tokens 41 us split and 33 so, heads of 64 28.5
+//    and 29.5; 2 sequences of 4,096, 64 tokens: 68 and 77; one of 8,192: 67 and 142).
 //  - others: rows_kernel's warps are as fast as the split's, and leave out what
 //    a prompt's rows cannot see, half of it at most: it is worth an
 //    SM's eight warps where half of all SMs' have work (float rows of 24
-//    sequences of 600 tokens, 100 tokens each: 53 us split and 61 so; of one
-//    sequence of 8,192, 64 tokens with 4 query heads each: 92 and 728).
+//    sequences of 600 tokens, 100 tokens each: 106 us split and 117 so; of one
+//    sequence of 8,192, 64 tokens with 4 query heads each: 89 and 735).
 bool splits(const Attn4Args& a, int type, uint32_t n, uint32_t grid) {
     const uint64_t rows = static_cast<uint64_t>(a.max_rows) * a.G, heads = static_cast<uint64_t>(n) * a.teams * a.team;
     if (rows > SPLIT_ROWS) return false;
     const bool tc = attention4_tc_takes(a, type);
-    const uint64_t block = block_rows(a, type == PKB_F32), blocks = (rows + block - 1) / block;
     if (!tc && rows <= 128) return true;
+    const uint64_t block = tc ? 16 : block_rows(a, type == PKB_F32), blocks = (rows + block - 1) / block;
     const uint64_t many = tc ? 256 : ROW_WARPS * block, waves = (heads * ((rows + many - 1) / many) + grid - 1) / grid;
-    return heads * blocks <= (tc ? 2 : 4) * grid * waves;
+    return 2 * heads * blocks <= (!tc ? 8 : rows <= 128 && a.c.dk >= 96 ? 3 : 4) * grid * waves;
 }
 
 // The work area of a call, over any lengths and max_rows: a join an item (an

@@ -255,3 +255,17 @@ def test_a_process_first_attention_may_be_a_captured_one(kind, rows):
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS, kind, str(rows)], capture_output=True, text=True, timeout=300,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dk,G", [(128, 1), (96, 3), (32, 8)])
+@pytest.mark.parametrize("rows", [8, 9, 16, 17, 24, 25, 32, 33, 40, 41, 48, 64, 65, 127, 128, 129])
+def test_every_way_rows_are_put_into_blocks(kind, dk, G, rows):
+    # of query heads and tokens; as few sequences as are split along the keys, and as many as may not be
+    most = -(-rows // G)
+    lens = [most + 40, 333, 1]
+    c = T.filled(lens, 32, 2, dk, seed=rows)
+    T.check_attention(c, lens, [most, max(1, most - 3), 1], [1, 0, 2], G, kind, True, 0)
+    many = [1 + (37 * i) % 150 for i in range(60)]
+    c = T.filled(many, 32, 3, dk, seed=rows)
+    T.check_attention(c, many, [most if i % 3 == 0 else 1 for i in range(60)], list(range(60)), G, kind, True, 20)
