@@ -15,7 +15,7 @@
 // bf16 rows (16 bits), three for float rows (24). One part, P rounded to bf16
 // before it meets V, is as far off as o's own rounding: 2.3e-3 of the result for
 // bf16 rows against 1.65e-3 for two parts and for weights in float, of which
-// 1.65e-3 is o's; it takes a tenth less time (64 sequences 49.7 us against 54.7).
+// 1.65e-3 is o's; it takes a tenth less time (64 sequences 49.9 us against 55).
 //
 // The split. A team of up to 16 cached heads' warps goes over the same
 // tiles of 32 keys side by side, each for its own head, so that what they
@@ -28,16 +28,18 @@
 // the others each share leaves its part (m, l, O) in the work area, and a
 // second kernel joins an item's parts in a fixed order.
 //
-// What bounds it. The cache's bytes (1.125 dk a token and cached head) and the
-// instructions that unpack them, which take about as long: a tile of 32 keys
-// of a head of 128 is some 520 instructions of a warp, 60 % of all issue slots.
+// What bounds it. Neither the cache's bytes (1.125 dk a token and cached head) nor
+// the issue slots (57 % of them), but each warp's chain from the codes to the
+// products: a tile of 32 keys of a head of 128 is some 560 instructions of a warp,
+// seven cycles each, of which two are fixed latencies and one a busy pipe, and the
+// four warps that a quarter of an SM has registers for do not cover that.
 // One step of 64 sequences of up to 4,099 tokens (161 MB, 8 heads of 128 with 4
-// query heads each, bf16): 51 us with its join, 3.1 TB/s; three sequences of up
-// to 120,001 tokens with 8 query heads each: 58 us, 3.4 TB/s. Of that some 7 us pass
+// query heads each, bf16): 55 us with its join, 2.9 TB/s; three sequences of up
+// to 120,001 tokens with 8 query heads each: 62 us, 3.2 TB/s. Of that some 7 us pass
 // before the first tile (the entries' lengths, their scan, the first pages) and
 // 5 in the join: short calls (12 us for one sequence of 377 tokens) are nothing else.
-// Scaled bf16 values for K too took 66 us for the 64 sequences, one warp that
-// fetches for all of a block's 55 and for itself each 52.
+// (With weights in one part, 52 us then: scaled bf16 values for K too 66 us for
+// the 64 sequences, one warp that fetches for all of a block's 55.)
 
 #include <atomic>
 #include <climits>
@@ -55,7 +57,7 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int JOIN_WARPS = 8;
 constexpr int TILE = 32;            // keys of a tile: two units
 constexpr uint32_t MAX_ENTRIES = 1024;  // sequences of one launch
-constexpr uint32_t MAX_TEAM = 16;       // (teams of 4 and 8 take as long: 64 sequences of 2,048 tokens, 16 heads, 78 us)
+constexpr uint32_t MAX_TEAM = 16;       // (teams of 4 and 8 take as long: 64 sequences of 2,048 tokens, 16 heads, 88 us)
 constexpr uint32_t SPLIT_ROWS = 1024;   // rows of an entry and cached head that may be split along the keys
 constexpr int MAX_GRID = 160;
 constexpr int MAX_WORKERS = 16;
@@ -449,8 +451,8 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
     }
     // Where no item is longer than one and a half shares, shares take whole
     // items: there is nothing to join then (200 sequences of 512 tokens, 8
-    // heads of 64, 4 rows each: 29.3 us in equal shares, 28.1 in whole items;
-    // 40 of 700 tokens, one row each: 15.5 and 15.9).
+    // heads of 64, 4 bf16 rows each: 30.9 us in equal shares, 29.8 in whole items;
+    // 40 of 700 tokens, heads of 128, one row each: 20.4 and 35.8).
     const uint32_t room = min(gridDim.x * WORKERS / a.team, a.max_shares), places = static_cast<uint32_t>(total);
     const bool whole = 2ull * longest * room <= 3ull * places;
 #pragma unroll
@@ -642,13 +644,13 @@ __global__ void __launch_bounds__(workers<NB, NT>() * 32, 1) split_kernel(Attn4A
 // dimensions of eight rows (a float4 a lane) over every `ways`-th of an
 // item's parts; `ways` warps then join theirs, always in the same order. It
 // is bound by latency: the item, then its parts, one load behind the other.
-// Up to eight parts an item go one way (a step of 32 sequences of 400 tokens,
-// five parts each: 15.9 us with its join, 21 two ways), a few long items'
-// take up to eight, so that no warp reads many parts one after another. Four
-// parts are loaded together (in 64 registers, so that four blocks share an
-// SM), or eight where each way still has more than six (one sequence of 2,000
-// tokens 11.4 -> 10.0 us, three of 120,000 61.5 -> 58.1; 8 of 400 tokens, five
-// parts a way, 11.4 and 13.5 with eight).
+// Up to eight parts an item go one way (a step of 32 sequences of 400 tokens, 16
+// heads, five parts each: 20.1 us with its join, 21.5 two ways; 8 heads, nine parts
+// each: 17.5, 15.8 two ways), a few long items' take up to eight, so that no
+// warp reads many parts one after another (three sequences of up to 120,001 tokens 62.7
+// us, 72.5 two ways). Four parts are loaded together (in 64 registers, so that
+// four blocks share an SM), or eight where each way still has more than six (the same three
+// 65.6 -> 62.7 us; 8 of 400 tokens, five parts a way, 12.8 and 15.0 with eight, in graphs).
 template <typename T, int NB, int NT, int BATCH>
 __global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kernel(Attn4Args a, uint32_t ways) {
     constexpr int QUADS = 2 * NB * NT, STRIDE = part_regs<NB, NT>() / 4;  // float4s of a lane: [dims 16][eight rows], then m and l
@@ -742,7 +744,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, BATCH == 4 ? 4 : 2) join_kern
 // For f16 and float rows, and bf16 rows of 256 values (others: pkb_attn4_tc.cu).
 // Bound by the tile's instructions and mma.sync's rate: 3 (f16 and bf16) or 5
 // (float rows) products of 16 keys and 8 rows a 16 values. 8 sequences of 2,048
-// tokens, 8 heads of 128, 256 float rows a head: 188 us.
+// tokens, 8 heads of 128, 256 float rows a head: 193 us.
 
 constexpr int ROW_WARPS = 8;
 constexpr int ROW_STAGES = 8;

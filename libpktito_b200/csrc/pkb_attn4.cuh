@@ -87,7 +87,9 @@ __device__ __forceinline__ void f16_parts(float lo, float hi, uint32_t (&r)[PART
     }
 }
 
-// The codes of a word as f16 pairs of the whole numbers c, without the scale:
+// The codes of a word as f16 pairs of the whole numbers c, without the scale
+// (the known way from a few bits to a float without a conversion: they become low
+// bits of a number whose exponent is known, which is then subtracted):
 // the nibbles in place in the mantissa of 1024 (pairs 0 and 2) and of 64
 // (pairs 1 and 3), so that a word takes one shift, four ANDs and four sums.
 template <int J>
@@ -122,8 +124,8 @@ __device__ __forceinline__ float rescale(float from, float to) { return from == 
 
 // What it costs to begin and end an item, in tiles: shares are of equal
 // cost, not of equal tiles. An item is START places of no work, then its
-// tiles (200 streams of 250 tokens: 26.1 us with none, 24.7 with two, 26.8 with
-// four; 64 sequences of up to 4,099: 52.3, 51.4, 52.4).
+// tiles (200 streams of 250 tokens, 4 f16 rows each: 24.4 us with none, 23.5 with two, 25.0
+// with four; 64 sequences of up to 4,099: 55.2, 54.7, 55.8).
 constexpr uint32_t START = 2;
 
 // One entry's rows and tokens, and of what its rows can see the first unit,

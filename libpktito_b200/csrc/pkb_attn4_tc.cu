@@ -11,8 +11,10 @@
 // the next. With O of both tiles that is all of TMEM. Products of 128 keys at a
 // time, which have one place a tile, wait for the softmax and it for them:
 // 1.18 ms against 1.09 for two prompts of 8,191 tokens, 8 heads of 128 with 4
-// query heads each (1,007 TFLOP/s, of the 1,662 that a library's bf16 product
-// reaches; leaving out the powers of two changes 1%).
+// query heads each. They take 1.06 ms now (1,037 TFLOP/s, of the 1,662 that a library's
+// bf16 product reaches; leaving out the powers of two changes 1%), and 1.17 where
+// calls follow one another for so long that the power cap brings the clock
+// from 1,965 to 1,770 MHz.
 //
 // What bounds it: the products alone take 0.94 ms. Q's 4 KB are read anew for
 // every 64 keys x 16, as many cycles as the product of 128 keys takes; the

@@ -20,7 +20,7 @@
 // tokens freed, compacted and some copied: 1.07 GB each way in 0.40 ms, of 0.33 at a
 // copy's rate), else by the launches and the latency of the plan's few
 // dependent reads (32 hypotheses' step of free, fork and grow: 18.6 us in a
-// graph, 47 from Python).
+// graph, 44 from Python).
 
 #include <climits>
 
@@ -81,7 +81,7 @@ struct UnitRows {
 // (all there are of up to 17 rows), found without a search; the others those
 // that longer entries have beside them, (rows - 2) / 16 at most, so that
 // counting them from starts[i] / 16 leaves every entry room. (One row of each
-// of 256 sequences appended and read: 16.6 us, 18.5 with a search for every
+// of 256 sequences appended and read: 16.4 us, 18.5 with a search for every
 // slot, 14.5 with one warp for an entry's two units, whose loop costs the long
 // entries 62 -> 67.)
 __device__ __forceinline__ UnitRows warp_unit(const RowArgs& a, uint32_t slot, uint32_t h) {
@@ -122,7 +122,7 @@ template <int NB> __host__ __device__ constexpr int v_row() { return NB * 16 + 8
 // 1 / s, whose remainder x - c s is exact in one FMA and says whether c is the
 // nearest. It is not, or may be a tie, in few warps: the others skip the
 // correction. No division: with a correctly rounded one a value the kernel
-// took 49 us for 28.8 M float values, 30 so.
+// took 49 us for 28.8 M float values, 32 so.
 __device__ __forceinline__ float quantize_block(float (&f)[8], uint32_t (&nib)[8]) {
     uint32_t m = 0;
 #pragma unroll
