@@ -464,16 +464,17 @@ size_t pkb_attention_cache4_work_bytes(const pkb_cache4 *c, uint32_t H, uint32_t
  *     o = sum_j softmax_j(scale q.k_j) v_j,
  * zeros where there is no such j; scale log2 e has to be finite. A sequence
  * has at most max_rows rows (one that has more is out of range). Products are
- * exact to the type of q, sums are float32, o is rounded once. The softmax's
- * weights meet V with 24 bits for float rows and 16 for others, but with 8 for
- * bf16 rows of up to 128 values a head that are many (prompts and long
- * chunks), where they are an operand of the tensor cores' bf16 products; their
- * sum is that of the unrounded ones. Rows of o
- * behind starts[n] are left as they were; o must not overlap q. work as for
- * the page operations. What is out of range sets the device error word's bit
- * 1, and such rows of o are not defined. Scores and sums are floats: a row
- * whose scores pass a float's range, or that sees values whose sum does 2^8
- * times over, is infinite or NaN, and no other row is. */
+ * exact to the type of q (but for 2^-39 of a row's largest value), sums are
+ * float32, o is rounded once. The softmax's weights meet V with 24 bits for
+ * float rows and 16 for others, but with 8 for bf16 rows of up to 128 values a
+ * head that are many (prompts and long chunks), where they are an operand of
+ * the tensor cores' bf16 products; their sum is that of the unrounded ones.
+ * Products, scores and sums are floats: a row whose q.k or scores pass a
+ * float's range, or that sees values whose sum does 2^8 times over, is
+ * infinite or NaN, and no other row is. Rows of o behind starts[n] are left as
+ * they were; o must not overlap q. work as for the page operations. What is
+ * out of range sets the device error word's bit 1, and such rows of o are not
+ * defined. */
 int pkb_attention_cache4_dev(void *stream, void *o, size_t os, const void *q, size_t qs, int type, uint32_t H,
                              const pkb_cache4 *c, uint32_t layer, const int32_t *seqs, const int32_t *starts,
                              uint32_t n, uint32_t rows, uint32_t max_rows, float scale, int causal, uint32_t window,
